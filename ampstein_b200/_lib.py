@@ -43,6 +43,10 @@ SIGNATURES = {
     "amp_b200_rms_norm_res": [_vp, _vp, _vp, _vp, _vp, ctypes.c_long, _i, ctypes.c_float, _vp],
     "amp_b200_silu_mul": [_vp, _vp, _vp, ctypes.c_long, _vp],
     "amp_b200_argmax_advance": [_vp, _i, _vp, _vp, _vp, ctypes.c_longlong, _vp, _vp],
+    "amp_b200_rope": [_vp, _vp],
+    "amp_b200_attention_workspace": [_i, _i, _i, _i, _i, _i, _l],
+    "amp_b200_attention": [_vp, _vp],
+    "amp_b200_copy_pages": [_vp, _vp, _vp, _i, _i, _i, _l, _vp, _vp, _i, _vp],
     "amp_exl3_gemv_add_res": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
     "amp_exl3_gemv_normed": [_vp, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "amp_exl3_mgemm_normed": [_vp, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp],
@@ -99,6 +103,7 @@ def lib():
             fn.restype = ctypes.c_int
         L.amp_exl3_moe_coop_ctr_len.restype = ctypes.c_long
         L.amp_exl3_moe_sorted_workspace.restype = ctypes.c_long
+        L.amp_b200_attention_workspace.restype = ctypes.c_long
         L.amp_comm_buffer_bytes.restype = ctypes.c_long
         L.amp_comm_ctl_bytes.restype = ctypes.c_long
         L.amp_b200_last_error.restype = ctypes.c_char_p

@@ -1,0 +1,97 @@
+// Attention over a paged key-value cache: what the split form (attention.cu) and the prompt form (attention_tc.cu) share.
+//
+// Query token t of sequence b stands at position p = pos[b] + t and sees the keys j <= p of its sequence, with a window W only
+// those with j > p - W or j < sinks:
+//   o = sum_j e^(scale q.k_j - m) v_j / l,   m = max_j scale q.k_j,   l = sum_j e^(scale q.k_j - m),   lse = m + ln l
+// Key j lives in row j % page_size of page table[b][j / page_size]. A token that sees nothing gets o = 0, lse = -inf; one whose
+// keys lie on a page outside the pool, or whose position is beyond the table, gets NaN (nothing outside the pool is read).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "exl3_gemv_kernel.cuh"
+#include "exl3_gemv_host.h"
+#include "host_common.h"
+#include "../../include/ampstein_b200.h"
+
+namespace amp {
+
+constexpr int AT_MAX_POS = 1 << 30;            // positions are clamped to +- this (the table holds fewer)
+
+struct AtSeq
+{
+    int first, count, row0;                    // position of the first query token, tokens, first row of q
+};
+
+// Sequence b. Whatever pos and cu hold, the rows stay inside the tensors.
+__device__ __forceinline__ AtSeq at_seq(const amp_attention_args& P, int b)
+{
+    AtSeq s;
+    const long long p = P.pos64 ? reinterpret_cast<const long long*>(P.pos)[b] : (long long) reinterpret_cast<const int*>(P.pos)[b];
+    s.first = (int) max(-(long long) AT_MAX_POS, min((long long) AT_MAX_POS, p));
+    if (P.cu)
+    {
+        s.row0 = max(0, min(P.cu[b], P.tokens));
+        s.count = max(s.row0, min(P.cu[b + 1], P.tokens)) - s.row0;
+    }
+    else
+    {
+        s.count = P.tokens / P.seqs;
+        s.row0 = b * s.count;
+    }
+    return s;
+}
+
+// Keys that some token of positions [first, first + count) sees: [0, a) and [lo, end), a <= lo <= end
+struct AtKeys
+{
+    int a, lo, end;
+    __device__ __forceinline__ int count() const { return a + end - lo; }
+    __device__ __forceinline__ int key(int i) const { return i < a ? i : i - a + lo; }     // the i-th of them
+};
+
+__device__ __forceinline__ AtKeys at_keys(const amp_attention_args& P, int first, int count)
+{
+    AtKeys k;
+    k.end = count > 0 ? max(0, min(first + count, P.max_pages * P.page_size)) : 0;
+    k.lo = P.window ? min(k.end, max(0, first - P.window + 1)) : 0;
+    k.a = P.window ? min(P.sinks, k.lo) : 0;
+    return k;
+}
+
+// Does the token at p see key j?
+__device__ __forceinline__ bool at_sees(const amp_attention_args& P, int p, int j)
+{
+    return j <= p && (!P.window || j > p - P.window || j < P.sinks);
+}
+
+template <typename T> struct AtType;
+template <> struct AtType<__half>
+{
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+    static __device__ __forceinline__ __half from(float a) { return __float2half_rn(a); }
+};
+template <> struct AtType<__nv_bfloat16>
+{
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+    static __device__ __forceinline__ __nv_bfloat16 from(float a) { return __float2bfloat16_rn(a); }
+};
+
+// 16 bytes to shared memory, or zeros
+__device__ __forceinline__ void at_copy16(uint32_t dst, const void* src, bool live)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+// Stores four values of a finished row, o / l, and with the first of them its lse. m counts in powers of two.
+template <typename T>
+__device__ __forceinline__ void at_store(const amp_attention_args& P, const AtSeq& s, int tok, int head, int c, float4 x, float m, float l)
+{
+    // (a position beyond the table: there are keys that cannot be found)
+    const float f = s.first + tok >= P.max_pages * P.page_size ? NAN : (l == 0.0f ? 0.0f : 1.0f / l);
+    T* out = reinterpret_cast<T*>(P.out) + (long long) (s.row0 + tok) * P.out_token + (long long) head * P.out_head + c;
+    *reinterpret_cast<uint2*>(out) = make_uint2(AtType<T>::pack(x.x * f, x.y * f), AtType<T>::pack(x.z * f, x.w * f));
+    if (c == 0 && P.lse)
+        P.lse[(long long) (s.row0 + tok) * P.heads + head] = f != f ? NAN : (l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f);
+}
+
+}  // namespace amp

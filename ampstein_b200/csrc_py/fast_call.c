@@ -4,6 +4,7 @@
  * released around the call, as ctypes does. Returns the entry's return code. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <string.h>
 #include <cuda_runtime_api.h>
 #include "../../include/ampstein_b200.h"
 
@@ -101,8 +102,24 @@ ENTRY(amp_b200_silu_mul)
     CALL(amp_b200_silu_mul(g, u, out, cnt, (cudaStream_t) st));
 }
 
+/* Arguments as the bytes of the entry's struct */
+#define STRUCT(name, type) \
+ENTRY(name) \
+{ \
+    type v; const char* b; void* st; \
+    if (!count(#name, n, 2) || !get_p(a[1], &st)) return NULL; \
+    if (!PyBytes_Check(a[0]) || PyBytes_GET_SIZE(a[0]) != (Py_ssize_t) sizeof v) \
+    { PyErr_SetString(PyExc_TypeError, #name " takes the " #type " struct as bytes"); return NULL; } \
+    b = PyBytes_AS_STRING(a[0]); \
+    memcpy(&v, b, sizeof v); \
+    CALL(name(&v, (cudaStream_t) st)); \
+}
+STRUCT(amp_b200_rope, amp_rope_args)
+STRUCT(amp_b200_attention, amp_attention_args)
+
 #define M(name) { #name, (PyCFunction) (void (*)(void)) py_##name, METH_FASTCALL, NULL }
 static PyMethodDef methods[] = { M(amp_exl3_gemm), M(amp_exl3_gemm_bf16), M(amp_exl3_mgemm), M(amp_exl3_mgemm_bf16), M(amp_exl3_moe_coop),
-                                 M(amp_exl3_moe_sorted), M(amp_b200_rms_norm_res), M(amp_b200_silu_mul), { NULL, NULL, 0, NULL } };
+                                 M(amp_exl3_moe_sorted), M(amp_b200_rms_norm_res), M(amp_b200_silu_mul),
+                                 M(amp_b200_rope), M(amp_b200_attention), { NULL, NULL, 0, NULL } };
 static struct PyModuleDef module = { PyModuleDef_HEAD_INIT, "_fast", NULL, -1, methods, NULL, NULL, NULL, NULL };
 PyMODINIT_FUNC PyInit__fast(void) { return PyModule_Create(&module); }

@@ -233,6 +233,80 @@ int amp_b200_rms_norm_res(const void* x, const void* r, const void* w, void* y, 
 int amp_b200_silu_mul(const void* g, const void* u, void* out, long count, cudaStream_t stream);
 int amp_b200_argmax_advance(const void* logits, int n, void* ids, void* pos, void* log, long long log_cap, void* ws,
                             cudaStream_t stream);
+
+/*
+ * Rotary positions, and the write of new keys and values into a paged cache, in one launch. No counterpart with this
+ * interface in the reference (its models rotate and append to a contiguous cache, src/ucode/ampstein/graphdec.uc:171-190).
+ *
+ * Rows are tokens. `seqs` sequences: without cu every one has tokens / seqs of them, with cu (seqs + 1 int32, ascending)
+ * sequence b has rows cu[b] .. cu[b + 1] - 1; rows behind cu[seqs] are left as they were. Token t of sequence b stands at
+ * position p = pos[b] + t (any sign). Pairs (x, y) of the first `rot` values of a head turn by the angle p * inv_freq[i], i <
+ * rot / 2: (i, i + rot / 2), or (2 i, 2 i + 1) with `interleaved`; cos and sin are multiplied by mscale, the other values pass.
+ * The angle is reduced in fp64, the turn is made in fp32, rounded once. k (rotated) and v go to row p % page_size of page
+ * table[b][p / page_size]; tokens before position 0, beyond the table or on a page outside the pool are not stored.
+ * q_out may be q. k, v, k_cache, v_cache, table may all be null: q is rotated alone. Strides count values (2 bytes).
+ */
+typedef struct amp_rope_args
+{
+    const void* q;              /* (tokens, heads, dim) */
+    const void* k;              /* (tokens, kv_heads, dim) */
+    const void* v;
+    void* q_out;
+    void* k_cache;              /* (pages, page_size, kv_heads, dim), the same type as q */
+    void* v_cache;
+    const int* table;           /* (seqs, max_pages), row stride table_row */
+    const void* pos;            /* (seqs) int32, or int64 with pos64 */
+    const int* cu;
+    const float* inv_freq;      /* (rot / 2) */
+    long q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+    long kc_page, kc_row, kc_head, vc_page, vc_row, vc_head, table_row;
+    int tokens, seqs, heads, kv_heads, dim, rot, interleaved, pages, page_size, max_pages, bf16, pos64;
+    float mscale;
+} amp_rope_args;
+int amp_b200_rope(const amp_rope_args* args, cudaStream_t stream);
+
+/*
+ * Attention of new tokens over a paged key-value cache that holds them already (amp_b200_rope). Sequences, rows and
+ * positions as there. The token at position p sees the keys j <= p of its sequence, with window > 0 only those with
+ * j > p - window or j < sinks; query head h reads key-value head h / (heads / kv_heads):
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,   lse = ln sum_j e^(scale * q . k_j)
+ * Table entries of pages that no token of the call sees are not read. A token that sees nothing (it stands before position
+ * 0: a slot without a sequence) gets 0 and an lse of -inf. A token whose visible keys lie on a page outside the pool, or
+ * that stands beyond the table, gets NaN. Scores, softmax and sums are in fp32, the weights are rounded to the values' type for the
+ * product with them. A call gives the same bits every time. dim: 64, 128 or 256.
+ * A key or value that some token of a sequence sees should be finite where another of its tokens in the call does not see it:
+ * an infinite or NaN value reaches the row of a token nearby through a weight of 0.
+ * workspace: amp_b200_attention_workspace bytes on the device, 16-byte aligned, contents of no matter (ragged: with cu; max_keys =
+ * max_pages * page_size; 0 bytes: none is needed); calls that may overlap need one each.
+ */
+typedef struct amp_attention_args
+{
+    const void* q;              /* (tokens, heads, dim) fp16, or bf16 */
+    const void* k_cache;        /* (pages, page_size, kv_heads, dim), the same type */
+    const void* v_cache;
+    void* out;                  /* (tokens, heads, dim), the same type */
+    float* lse;                 /* (tokens, heads) contiguous; may be null */
+    const int* table;           /* (seqs, max_pages), row stride table_row */
+    const void* pos;            /* (seqs) int32, or int64 with pos64 */
+    const int* cu;              /* (seqs + 1), or null */
+    void* workspace;
+    long workspace_bytes;
+    long q_token, q_head, out_token, out_head;
+    long k_page, k_row, k_head, v_page, v_row, v_head, table_row;
+    int tokens, seqs, heads, kv_heads, dim, pages, page_size, max_pages, window, sinks, bf16, pos64;
+    float scale;
+} amp_attention_args;
+long amp_b200_attention_workspace(int tokens, int seqs, int heads, int kv_heads, int dim, int ragged, long max_keys);
+int amp_b200_attention(const amp_attention_args* args, cudaStream_t stream);
+
+/*
+ * Copies whole pages inside caches: page dst[i] := page src[i] in every layer of every cache, for forks, defragmentation and
+ * moves. caches / layer_strides / page_strides: host arrays of one entry per cache (bytes; all multiples of 16), a page is
+ * page_bytes (a multiple of 16) without gaps. src, dst: host arrays; they travel with the launch. Refused: a page outside
+ * [0, pages), a destination named twice, a page that is both source and destination of different copies.
+ */
+int amp_b200_copy_pages(void* const* caches, const long* layer_strides, const long* page_strides, int n_caches, int layers,
+                        int pages, long page_bytes, const int* src, const int* dst, int n, cudaStream_t stream);
 /*
  * The residual norm split between the launches on either side of it (the form that pays: nothing
  * reads a whole row on a CTA's critical path).

@@ -1,0 +1,285 @@
+"""Paged attention against its plain 64-bit form, by element and with derived bounds: lengths from nothing to long, odd sizes, head
+layouts, windows with sinks, strides, poisoned surroundings, streams and graphs."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import attention_cases as ac  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+H, B = torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def amp():
+    import ampstein_b200
+    return ampstein_b200
+
+
+def make(pos, counts, hq, hkv, d, page, dtype, window=0, sinks=0, seed=1, **kw):
+    k, v, table = ac.paged(pos, counts, page, hkv, d, dtype, window, sinks, seed, **kw)
+    g = torch.Generator().manual_seed(seed + 1000)
+    q = torch.randn((sum(counts), hq, d), generator=g).to(dtype).cuda()
+    return q, k, v, table
+
+
+def cu_of(counts):
+    c = [0]
+    for n in counts:
+        c.append(c[-1] + n)
+    return torch.tensor(c, dtype=torch.int32, device="cuda")
+
+
+def check(amp, pos, counts, hq, hkv, d, page, dtype, window=0, sinks=0, ragged=False, scale=None, pos_dtype=torch.int32, seed=1, **kw):
+    q, k, v, table = make(pos, counts, hq, hkv, d, page, dtype, window, sinks, seed, **kw)
+    lse = torch.full((q.shape[0], hq), 7.0, device="cuda")
+    out = amp.paged_attention(q, k, v, table, torch.tensor(pos, dtype=pos_dtype, device="cuda"), cu=cu_of(counts) if ragged else None,
+                              window=window, sinks=sinks, scale=scale, lse=lse)
+    want, wlse, tol, ltol = ac.attention(q, k, v, table, pos, counts, window, sinks, d ** -0.5 if scale is None else scale)
+    assert torch.isfinite(out).all()
+    over = (out.double() - want).abs() - tol
+    assert over.max() <= 0, (float(over.max()), int(over.argmax()))
+    assert torch.equal(torch.isinf(lse), torch.isinf(wlse))
+    live = ~torch.isinf(wlse)
+    assert ((lse.double() - wlse)[live].abs() <= ltol[live]).all()
+    return out
+
+
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (8, 8), (8, 2), (6, 1), (5, 1), (14, 2), (16, 1), (40, 2)])
+def test_one_token(amp, dtype, d, hq, hkv):
+    """Every group size, rows that fill a row tile and rows that do not; lengths 1, 2, around the units' ends, none"""
+    pos = [0, 1, 14, 15, 16, 62, 63, 64, 127, 128, -1, 700]
+    check(amp, pos, [1] * len(pos), hq, hkv, d, 16, dtype)
+
+
+@pytest.mark.parametrize("page", [1, 3, 16, 24, 64, 100, 256, 1000])
+def test_pages_that_end_inside_a_unit(amp, page):
+    check(amp, [0, 99, 517, 64], [1] * 4, 8, 2, 128, page, H, wide=2)
+
+
+@pytest.mark.parametrize("length", [1, 63, 64, 65, 255, 256, 257, 1000, 9001])
+def test_one_sequence_over_the_whole_device(amp, length):
+    check(amp, [length - 1], [1], 4, 1, 128, 64, B, pos_dtype=torch.int64)
+
+
+@pytest.mark.parametrize("count", [2, 3, 4, 5, 7, 16, 33])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (6, 1, 64), (3, 3, 256), (32, 2, 128)])
+def test_several_tokens_per_sequence(amp, count, hq, hkv, d):
+    """Drafted tokens: each sees the ones in front of it; sequences that begin with the call, and one that begins inside it"""
+    pos = [0, 100, 300, 1, -1, -count]
+    check(amp, pos, [count] * len(pos), hq, hkv, d, 16, B)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (2, 4), (16, 0), (64, 4), (100, 1), (100, 200), (5000, 3)])
+@pytest.mark.parametrize("count", [1, 3, 20])
+def test_windows_and_sinks(amp, window, sinks, count):
+    """Windows of one key, longer than the sequence, sinks beyond the window; pages left behind are not read"""
+    check(amp, [0, 5, 17, 90, 400, 1000, -1], [count] * 7, 4, 2, 64, 16, H, window, sinks)
+
+
+def test_sinks_without_a_window_change_nothing(amp):
+    q, k, v, table = make([200, 50], [1, 1], 4, 2, 64, 16, H)
+    pos = torch.tensor([200, 50], dtype=torch.int32, device="cuda")
+    assert torch.equal(amp.paged_attention(q, k, v, table, pos), amp.paged_attention(q, k, v, table, pos, sinks=4))
+
+
+@pytest.mark.parametrize("d,dtype", [(64, B), (128, H), (128, B), (256, H)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
+def test_mixed_ragged(amp, d, dtype, window, sinks):
+    """Single tokens, drafts, prompts, empty sequences in one call"""
+    counts = [1, 200, 0, 3, 77, 1, 0, 129]
+    pos = [900, 0, 5, 63, 64, -1, 0, 31]
+    check(amp, pos, counts, 8, 2, d, 16, dtype, window, sinks, ragged=True)
+
+
+@pytest.mark.parametrize("count,first", [(64, 0), (300, 0), (257, 1000), (130, 7)])
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(8, 2, 128, H), (5, 1, 64, B), (4, 4, 128, B), (2, 1, 256, B), (32, 2, 64, H)])
+def test_prompt_chunks(amp, count, first, hq, hkv, d, dtype):
+    check(amp, [first], [count], hq, hkv, d, 24, dtype)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (30, 4), (128, 4), (200, 500)])
+def test_prompt_chunks_in_a_window(amp, window, sinks):
+    check(amp, [0, 600], [260, 260], 8, 2, 64, 16, B, window, sinks)
+
+
+def test_scales(amp):
+    for scale in (0.0, -0.5, 1.0, 0.003):
+        check(amp, [40, 300], [2, 2], 4, 2, 64, 16, H, scale=scale)
+
+
+def test_peaked_scores(amp):
+    """Scores far apart: every other weight vanishes, and the running maximum moves late"""
+    q, k, v, table = make([1500], [1], 4, 1, 128, 64, H)
+    q *= 8
+    k = torch.where(torch.isfinite(k), k * torch.linspace(0.5, 4, k.shape[0], device="cuda").to(H)[:, None, None, None], k)
+    out = amp.paged_attention(q, k, v, table, torch.tensor([1500], device="cuda"))
+    want, _, tol, _ = ac.attention(q, k, v, table, [1500], [1], 0, 0, 128 ** -0.5)
+    assert ((out.double() - want).abs() <= tol).all()
+
+
+def test_strides(amp):
+    """q out of a packed q|k|v row, caches stored per head, caches that are one layer of a larger tensor, out inside a larger one"""
+    pos, counts, hq, hkv, d = [333, 20], [2, 2], 8, 2, 128
+    q, k, v, table = make(pos, counts, hq, hkv, d, 16, H)
+    want = amp.paged_attention(q, k, v, table, torch.tensor(pos, device="cuda"))
+    packed = torch.randn((4, (hq + 2 * hkv) * d), device="cuda").to(H)
+    packed[:, :hq * d] = q.view(4, -1)
+    qs = packed[:, :hq * d].view(4, hq, d)
+    kh, vh = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (k, v))
+    both = torch.stack((k, v), 1)                                       # (pages, 2, page_size, ...)
+    wide = torch.zeros((4, 2 * hq, d), dtype=H, device="cuda")
+    tab = torch.cat((table, table), 1)[:, :table.shape[1]]
+    for kk, vv in ((kh, vh), (k, vh), (both[:, 0], both[:, 1])):
+        got = amp.paged_attention(qs, kk, vv, tab, torch.tensor(pos, device="cuda"), out=wide[:, hq:])
+        assert torch.equal(got, want) and not wide[:, :hq].any()
+
+
+def test_same_bits_every_time(amp):
+    q, k, v, table = make([5000, 70, 900], [1, 1, 1], 8, 2, 128, 16, H)
+    pos = torch.tensor([5000, 70, 900], device="cuda")
+    first = amp.paged_attention(q, k, v, table, pos)
+    for _ in range(5):
+        assert torch.equal(first, amp.paged_attention(q, k, v, table, pos))
+
+
+@pytest.mark.parametrize("counts", [[1, 1, 1], [3, 3, 3], [140, 2, 70]])
+def test_rows_behind_the_last_sequence_are_left(amp, counts):
+    pos = [10, 200, 0]
+    q, k, v, table = make(pos, counts, 4, 2, 128, 16, H)
+    q = torch.cat((q, torch.full((9, 4, 128), math.nan, dtype=H, device="cuda")))
+    out = torch.full_like(q, 3.0)
+    lse = torch.full(q.shape[:2], 5.0, device="cuda")
+    amp.paged_attention(q, k, v, table, torch.tensor(pos, device="cuda"), cu=cu_of(counts), out=out, lse=lse)
+    n = sum(counts)
+    assert (out[n:] == 3.0).all() and (lse[n:] == 5.0).all() and torch.isfinite(out[:n]).all()
+
+
+@pytest.mark.parametrize("count", [1, 3, 200])
+def test_pages_outside_the_pool_give_nan_in_their_rows_alone(amp, count):
+    """A table that names no page, or ends too early, is not read from; the other sequences keep their bits"""
+    pos = [500, 500, 500, 1 << 40]
+    q, k, v, table = make([500] * 4, [count] * 4, 4, 2, 128, 16, H)
+    p = torch.tensor([500] * 4, dtype=torch.int64, device="cuda")
+    want = amp.paged_attention(q, k, v, table, p)
+    broken = table.clone()
+    broken[1, 3] = -1
+    broken[2, 30] = k.shape[0]
+    got = amp.paged_attention(q, k, v, broken, torch.tensor(pos, dtype=torch.int64, device="cuda"))
+    assert torch.equal(got[:count], want[:count]) and got[count:].isnan().all()
+    short = amp.paged_attention(q, k, v, table[:, :4].contiguous(), p)
+    assert short.isnan().all()
+    none = amp.paged_attention(q, k, v, table[:, :0], torch.tensor([-count, 0, -1, 5], device="cuda"))
+    assert (none[:count] == 0).all() and none[count:2 * count].isnan().all()
+
+
+def test_far_positions_of_a_large_cache(amp):
+    """Offsets that pass 32 bits: 5 GB of keys"""
+    page, hkv, d = 64, 8, 128
+    pages = 40000
+    k = torch.zeros((pages, page, hkv, d), dtype=H, device="cuda")
+    v = torch.zeros_like(k)
+    table = torch.arange(pages - 1, pages - 9, -1, dtype=torch.int32, device="cuda").view(1, 8)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for t in (k, v):
+        t[pages - 8:] = torch.randn((8, page, hkv, d), device="cuda", generator=g).to(H)
+    q = torch.randn((1, 16, d), device="cuda", generator=g).to(H)
+    out = amp.paged_attention(q, k, v, table, torch.tensor([500], device="cuda"))
+    small = torch.arange(7, -1, -1, dtype=torch.int32, device="cuda").view(1, 8)
+    assert torch.equal(out, amp.paged_attention(q, k[pages - 8:].clone(), v[pages - 8:].clone(), small, torch.tensor([500], device="cuda")))
+
+
+def test_many_sequences(amp):
+    g = torch.Generator().manual_seed(5)
+    pos = torch.randint(-1, 90, (700,), generator=g).tolist()
+    check(amp, pos, [1] * 700, 2, 1, 64, 16, H)
+
+
+def test_captured_calls_replay_with_other_lengths_and_beside_each_other(amp):
+    """Two graphs with their own workspaces, replayed on two streams at once; the lengths change between replays"""
+    sets = []
+    for seed in (1, 2):
+        pos = [3000, 40, 1200, -1]
+        q, k, v, table = make(pos, [1] * 4, 8, 2, 128, 16, H, seed=seed, wide=3)
+        k, v = torch.nan_to_num(k, 1.0, 1.0, -1.0), torch.nan_to_num(v, 1.0, 1.0, -1.0)
+        table = table.clamp(0, k.shape[0] - 1)
+        p = torch.tensor(pos, device="cuda")
+        out = torch.empty_like(q)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            amp.paged_attention(q, k, v, table, p, out=out)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                amp.paged_attention(q, k, v, table, p, out=out)
+        sets.append((q, k, v, table, p, out, graph, stream))
+    torch.cuda.synchronize()
+    for lengths in ([3000, 40, 1200, -1], [17, 2999, -1, 3020], [0, 0, 0, 0]):
+        for s in sets:
+            s[4].copy_(torch.tensor(lengths))
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for s in sets:
+                with torch.cuda.stream(s[7]):
+                    s[6].replay()
+        torch.cuda.synchronize()
+        for q, k, v, table, p, out, _, _ in sets:
+            assert torch.equal(out, amp.paged_attention(q, k, v, table, p))
+
+
+def test_two_streams_at_once(amp):
+    a, b = make([4000], [1], 8, 2, 128, 16, H, seed=1), make([3000, 77], [1, 1], 8, 2, 128, 16, H, seed=2)
+    pa, pb = torch.tensor([4000], device="cuda"), torch.tensor([3000, 77], device="cuda")
+    wa, wb = amp.paged_attention(*a, pa), amp.paged_attention(*b, pb)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(30):
+        for s, args, p in zip(streams, (a, b), (pa, pb)):
+            with torch.cuda.stream(s):
+                got.append(amp.paged_attention(*args, p))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, wa if i % 2 == 0 else wb) for i, x in enumerate(got))
+
+
+def test_empty_calls(amp):
+    q, k, v, table = make([5], [1], 4, 2, 64, 16, H)
+    e = amp.paged_attention(q[:0], k, v, table[:0], torch.zeros(0, dtype=torch.int32, device="cuda"))
+    assert e.shape == (0, 4, 64)
+    amp.paged_attention(q[:0], k, v, table, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    out = amp.paged_attention(q, k, v, table[:0], torch.zeros(0, dtype=torch.int32, device="cuda"), cu=cu_of([]), out=torch.full_like(q, 2.0))
+    assert (out == 2.0).all()
+
+
+def test_refusals(amp):
+    q, k, v, table = make([5, 9], [1, 1], 4, 2, 64, 16, H)
+    pos = torch.tensor([5, 9], device="cuda")
+    f = amp.paged_attention
+    bad = [
+        (RuntimeError, lambda: f(q.cpu(), k, v, table, pos)),
+        (RuntimeError, lambda: f(q, k, v, table.cpu(), pos)),
+        (TypeError, lambda: f(q.float(), k, v, table, pos)),
+        (TypeError, lambda: f(q, k.to(B), v, table, pos)),
+        (TypeError, lambda: f(q, k, v, table.long(), pos)),
+        (TypeError, lambda: f(q, k, v, table, pos.float())),
+        (TypeError, lambda: f(q, k, v, table, pos, cu=torch.zeros(2, dtype=torch.int32, device="cuda"))),
+        (TypeError, lambda: f(q, k, v, table[:1], pos)),
+        (ValueError, lambda: f(q[:, :3], k, v, table, pos)),
+        (ValueError, lambda: f(q[:, :, :32], k[..., :32], v[..., :32], table, pos)),
+        (ValueError, lambda: f(q, k, v[:1], table, pos)),
+        (ValueError, lambda: f(torch.cat((q, q[:1])), k, v, table, pos)),
+        (ValueError, lambda: f(q, k, v, table, pos, window=-1)),
+        (ValueError, lambda: f(q, k, v, table, pos, scale=math.nan)),
+        (ValueError, lambda: f(q, k, v, table, pos, out=q)),
+        (ValueError, lambda: f(q, k, v, table, pos, lse=torch.zeros((2, 3), device="cuda"))),
+        (ValueError, lambda: f(q.transpose(1, 2).contiguous().transpose(1, 2), k, v, table, pos)),
+        (RuntimeError, lambda: f(torch.zeros(2 * 4 * 64 + 1, dtype=H, device="cuda")[1:].view(2, 4, 64), k, v, table, pos)),
+        (ValueError, lambda: f(q, k, v, torch.zeros((2, 1 << 27), dtype=torch.int32, device="cuda"), pos)),
+    ]
+    for i, (kind, call) in enumerate(bad):
+        with pytest.raises(kind):
+            call()
+            pytest.fail("call %d was taken" % i)
