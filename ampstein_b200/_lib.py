@@ -44,7 +44,8 @@ SIGNATURES = {
     "amp_b200_silu_mul": [_vp, _vp, _vp, ctypes.c_long, _vp],
     "amp_b200_argmax_advance": [_vp, _i, _vp, _vp, _vp, ctypes.c_longlong, _vp, _vp],
     "amp_b200_rope": [_vp, _vp],
-    "amp_b200_attention_workspace": [_i, _i, _i, _i, _i, _i, _l],
+    "amp_b200_attention_workspace": [_i, _i, _i, _i, _i, _i, _l, _i, _i],
+    "amp_b200_attention_status": [ctypes.POINTER(ctypes.c_int)],
     "amp_b200_attention": [_vp, _vp],
     "amp_b200_copy_pages": [_vp, _vp, _vp, _i, _i, _i, _l, _vp, _vp, _i, _vp],
     "amp_exl3_gemv_add_res": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],

@@ -259,12 +259,13 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
             raise ValueError("%s: lse must be contiguous float32 (rows, heads)" % name)
     if rows == 0 or seqs == 0:
         return out
-    n = _workspace_bytes(dev, rows, seqs, heads, kv_heads, dim, 0 if cu is None else 1, max_pages * page_size)
+    window, sinks = min(int(window), _MAX_POS), min(int(sinks), _MAX_POS)
+    n = _workspace_bytes(dev, rows, seqs, heads, kv_heads, dim, 0 if cu is None else 1, max_pages * page_size, window, sinks)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     args = _ATTENTION.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
                            table.data_ptr(), pos.data_ptr(), 0 if cu is None else cu.data_ptr(), 0 if ws is None else ws.data_ptr(), n,
                            *qs, *os, *ks, *vs, tr, rows, seqs, heads, kv_heads, dim, pages, page_size, max_pages,
-                           min(int(window), _MAX_POS), min(int(sinks), _MAX_POS), 1 if dtype is torch.bfloat16 else 0,
+                           window, sinks, 1 if dtype is torch.bfloat16 else 0,
                            1 if pos.dtype is torch.int64 else 0, scale)
     _launch(q, "amp_b200_attention", args)
     return out

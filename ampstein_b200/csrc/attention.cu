@@ -12,7 +12,7 @@
 // A warp owns 16 keys of every unit and a ring of stages of its own, filled with 16-byte asynchronous copies by its own lanes: the
 // loop has no barrier between warps, each keeps its own m, l and o, and the four meet when a segment ends. The rings run ahead over
 // the ends of segments.
-#include "attention.cuh"
+#include "attention_tc.cuh"
 
 namespace amp {
 
@@ -29,6 +29,7 @@ struct AtPlan
 {
     amp_attention_args P;
     int grid;                                  // CTAs of the split form
+    int split_rows;                            // with cu: sequences of more rows (tokens x group) are the prompt form's
     int whole;                                 // 1: every (sequence, head, row tile) belongs to one CTA, nothing to join
     int pdl;
     float scale2;                              // scale * log2(e)
@@ -58,9 +59,10 @@ __device__ __forceinline__ void at_mma(float (&c)[4], const uint32_t (&a)[4], ui
 }
 
 // Row tiles of a sequence, and units of each of them
-__device__ __forceinline__ int at_row_tiles(const amp_attention_args& P, const AtSeq& s)
+__device__ __forceinline__ int at_row_tiles(const AtPlan& S, const AtSeq& s)
 {
-    return (s.count * (P.heads / P.kv_heads) + AT_ROWS - 1) / AT_ROWS;
+    const int rows = s.count * (S.P.heads / S.P.kv_heads);
+    return rows > S.split_rows ? 0 : (rows + AT_ROWS - 1) / AT_ROWS;
 }
 
 __device__ __forceinline__ int at_units(const AtKeys& k) { return max(1, (k.count() + AT_UNIT - 1) / AT_UNIT); }
@@ -72,23 +74,23 @@ struct AtCursor
     AtSeq s;
     AtKeys k;
 
-    __device__ __forceinline__ void load(const amp_attention_args& P)
+    __device__ __forceinline__ void load(const AtPlan& S)
     {
-        s = at_seq(P, b);
-        k = at_keys(P, s.first, s.count);
-        tiles = at_row_tiles(P, s);
+        s = at_seq(S.P, b);
+        k = at_keys(S.P, s.first, s.count);
+        tiles = at_row_tiles(S, s);
         units = at_units(k);
     }
     // to the next unit; the caller knows that there is one
-    __device__ __forceinline__ bool advance(const amp_attention_args& P)
+    __device__ __forceinline__ bool advance(const AtPlan& S)
     {
         if (++u < units) return false;
         u = 0;
         if (++rt < tiles) return true;
         rt = 0;
-        if (++h < P.kv_heads) return true;
+        if (++h < S.P.kv_heads) return true;
         h = 0;
-        do { ++b; load(P); } while (!tiles && b + 1 < P.seqs);
+        do { ++b; load(S); } while (!tiles && b + 1 < S.P.seqs);
         return true;
     }
 };
@@ -120,10 +122,10 @@ void attention_split_kernel(const AtPlan S)
     long long left;
     if (S.whole)
     {
-        in.b = 0; in.load(P);                                // (all sequences have as many tokens)
+        in.b = 0; in.load(S);                                // (all sequences have as many tokens)
         const int per = P.kv_heads * in.tiles;
         in.b = cta / per; in.h = cta % per / in.tiles; in.rt = cta % in.tiles; in.u = 0;
-        in.load(P);
+        in.load(S);
         left = in.units;
     }
     else
@@ -134,7 +136,7 @@ void attention_split_kernel(const AtPlan S)
         for (int b = b0; b < b1; ++b)
         {
             const AtSeq s = at_seq(P, b);
-            mine += (long long) P.kv_heads * at_row_tiles(P, s) * at_units(at_keys(P, s.first, s.count));
+            mine += (long long) P.kv_heads * at_row_tiles(S, s) * at_units(at_keys(P, s.first, s.count));
         }
         long long sum = mine;
         #pragma unroll
@@ -161,7 +163,7 @@ void attention_split_kernel(const AtPlan S)
             for (int b = b0; b < b1; ++b)
             {
                 AtCursor c;
-                c.b = b; c.load(P);
+                c.b = b; c.load(S);
                 const long long n = (long long) P.kv_heads * c.tiles * c.units;
                 if (at < n)
                 {
@@ -176,7 +178,7 @@ void attention_split_kernel(const AtPlan S)
         }
         __syncthreads();
         in.b = s_place[0]; in.h = s_place[1]; in.rt = s_place[2]; in.u = s_place[3];
-        in.load(P);
+        in.load(S);
         if (t == 0)
         {
             // a segment that began before this CTA: which CTAs hold parts of it
@@ -231,7 +233,7 @@ void attention_split_kernel(const AtPlan S)
                 at_copy16(at + off, kc + k + c * 8, ok);
                 at_copy16(at + STAGE / 2 + off, vc + v + c * 8, ok);
             }
-            if (--to_load > 0) { ld.advance(P); look_up(); }
+            if (--to_load > 0) { ld.advance(S); look_up(); }
         }
         cp_async_commit();
     };
@@ -403,7 +405,7 @@ void attention_split_kernel(const AtPlan S)
         }
         issue(stage);
         stage = stage + 1 == NST ? 0 : stage + 1;
-        if (left > 0) in.advance(P);
+        if (left > 0) in.advance(S);
     }
 }
 
@@ -495,10 +497,55 @@ static const AtDevice* at_device(int* rc)
 
 // Sequences that fit into this many keys are not split: nothing is joined then
 constexpr int AT_WHOLE_KEYS = 256;
-
-static bool at_whole(bool ragged, long max_keys) { return !ragged && max_keys <= AT_WHOLE_KEYS; }
+// Rows (tokens x group) up to which a sequence takes the split form; beyond, the prompt form
+constexpr int AT_SPLIT_ROWS = 32;
 
 static int at_grid(int dim, int sms) { return sms * (dim == 64 ? at_ctas<64> : dim == 128 ? at_ctas<128> : at_ctas<256>); }
+
+// How a call is cut up: by its sizes alone (the lengths are on the device)
+struct AtCut
+{
+    bool split, tc;                            // forms that are launched
+    int whole, grid;                           // split form
+    int tiles, slices;                         // prompt form
+    size_t tc_offset, bytes;                   // of the workspace
+};
+
+// Slices of the keys of each of `items` row tiles, `kt` key tiles long at most: waves of CTAs, each its share of the key tiles and a
+// set-up of about two, and a join worth four
+static int ta_slices(long items, long kt, int sms)
+{
+    int best = 1;
+    double cost = 1e30;
+    for (int s = 1; s <= kt && s * items <= 4l * sms && s <= 256; ++s)
+    {
+        const double c = (double) ((items * s + sms - 1) / sms) * ((double) ((kt + s - 1) / s) + 2) + (s > 1 ? 4 : 0);
+        if (c < cost * 0.97) { cost = c; best = s; }
+    }
+    return best;
+}
+
+static AtCut at_cut(int tokens, int seqs, int heads, int kv_heads, int dim, bool ragged, long max_keys, int window, int sinks, int sms)
+{
+    AtCut C = {};
+    const long group = heads / kv_heads, all = tokens * group, each = all / seqs;
+    C.split = ragged || each <= AT_SPLIT_ROWS;
+    C.tc = ragged ? all > AT_SPLIT_ROWS : !C.split;
+    C.whole = C.split && !ragged && max_keys <= AT_WHOLE_KEYS;
+    C.grid = at_grid(dim, sms);
+    if (C.split && !C.whole) C.bytes = (at_desc_bytes(C.grid) + 2 * C.grid * at_part_floats(dim) * 4 + 127) / 128 * 128;
+    C.tc_offset = C.bytes;
+    C.slices = 1;
+    if (C.tc)
+    {
+        const int rows = ta_rows(dim), kb = dim <= 128 ? 128 : 64;
+        C.tiles = (int) (ragged ? all / rows + min((long) seqs, all / (AT_SPLIT_ROWS + 1)) : seqs * ((each + rows - 1) / rows));
+        const long keys = window ? min(max_keys, (long) window + sinks + rows / group + 1) : max_keys;
+        C.slices = ta_slices((long) C.tiles * kv_heads, (keys + kb - 1) / kb, sms);
+        if (C.slices > 1) C.bytes += (size_t) C.tiles * kv_heads * C.slices * ta_part_floats(dim) * 4;
+    }
+    return C;
+}
 
 template <typename T, int D>
 static int at_launch(AtPlan& S, cudaStream_t stream)
@@ -531,14 +578,13 @@ static int at_launch(AtPlan& S, cudaStream_t stream)
 
 using namespace amp;
 
-AMP_API long amp_b200_attention_workspace(int tokens, int seqs, int heads, int kv_heads, int dim, int ragged, long max_keys)
+AMP_API long amp_b200_attention_workspace(int tokens, int seqs, int heads, int kv_heads, int dim, int ragged, long max_keys, int window, int sinks)
 {
-    if (tokens <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || (dim != 64 && dim != 128 && dim != 256) || at_whole(ragged, max_keys)) return 0;
+    if (tokens <= 0 || seqs <= 0 || kv_heads <= 0 || heads < kv_heads || (dim != 64 && dim != 128 && dim != 256) || window < 0 || sinks < 0) return 0;
     int rc = 0;
     const AtDevice* d = at_device(&rc);
     if (!d) return rc < 0 ? rc : -1;
-    const int grid = at_grid(dim, d->sms);
-    return (long) (at_desc_bytes(grid) + 2 * grid * at_part_floats(dim) * 4);
+    return (long) at_cut(tokens, seqs, heads, kv_heads, dim, ragged != 0, max_keys, min(window, AT_MAX_POS), min(sinks, AT_MAX_POS), d->sms).bytes;
 }
 
 AMP_API int amp_b200_attention(const amp_attention_args* args, cudaStream_t stream)
@@ -565,15 +611,22 @@ AMP_API int amp_b200_attention(const amp_attention_args* args, cudaStream_t stre
     int rc = 0;
     const AtDevice* d = at_device(&rc);
     if (!d) return rc;
-    S.grid = at_grid(P.dim, d->sms);
-    const long max_keys = (long) P.max_pages * P.page_size;
-    S.whole = at_whole(P.cu != nullptr, max_keys);
-    S.pdl = g_pdl;
-    S.scale2 = P.scale * 1.4426950408889634f;
-    if (!S.whole)
-        AMP_REQUIRE(P.workspace && ((uintptr_t) P.workspace & 15) == 0 && P.workspace_bytes >= amp_b200_attention_workspace(P.tokens, P.seqs, P.heads, P.kv_heads, P.dim, P.cu != nullptr, max_keys),
-                    "attention: workspace too small or misaligned");
-    if (P.bf16)
-        return P.dim == 64 ? at_launch<__nv_bfloat16, 64>(S, stream) : P.dim == 128 ? at_launch<__nv_bfloat16, 128>(S, stream) : at_launch<__nv_bfloat16, 256>(S, stream);
-    return P.dim == 64 ? at_launch<__half, 64>(S, stream) : P.dim == 128 ? at_launch<__half, 128>(S, stream) : at_launch<__half, 256>(S, stream);
+    const AtCut C = at_cut(P.tokens, P.seqs, P.heads, P.kv_heads, P.dim, P.cu != nullptr, (long) P.max_pages * P.page_size, P.window, P.sinks, d->sms);
+    if (C.bytes)
+        AMP_REQUIRE(P.workspace && ((uintptr_t) P.workspace & 15) == 0 && P.workspace_bytes >= (long) C.bytes, "attention: workspace too small or misaligned");
+    if (C.split)
+    {
+        S.grid = C.grid; S.whole = C.whole; S.pdl = g_pdl; S.split_rows = P.cu ? AT_SPLIT_ROWS : 1 << 30;
+        S.scale2 = P.scale * 1.4426950408889634f;
+        if (P.bf16)
+            rc = P.dim == 64 ? at_launch<__nv_bfloat16, 64>(S, stream) : P.dim == 128 ? at_launch<__nv_bfloat16, 128>(S, stream) : at_launch<__nv_bfloat16, 256>(S, stream);
+        else
+            rc = P.dim == 64 ? at_launch<__half, 64>(S, stream) : P.dim == 128 ? at_launch<__half, 128>(S, stream) : at_launch<__half, 256>(S, stream);
+        if (rc) return rc;
+    }
+    if (!C.tc) return 0;
+    TaPlan A;
+    A.P = P; A.tiles = C.tiles; A.slices = C.slices; A.split_rows = P.cu ? AT_SPLIT_ROWS : 0; A.pdl = g_pdl;
+    A.scale2 = P.scale * 1.4426950408889634f; A.part_offset = C.tc_offset;
+    return attention_tc(A, stream);
 }

@@ -82,16 +82,34 @@ __device__ __forceinline__ void at_copy16(uint32_t dst, const void* src, bool li
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
-// Stores four values of a finished row, o / l, and with the first of them its lse. m counts in powers of two.
+// What a finished row's sums are multiplied by, 1 / l (a position beyond the table has keys that cannot be found: NaN)
+__device__ __forceinline__ float at_factor(const amp_attention_args& P, int p, float l)
+{
+    return p >= P.max_pages * P.page_size ? NAN : (l == 0.0f ? 0.0f : 1.0f / l);
+}
+
+// Stores four or eight values of a finished row, and with the first of them its lse. m counts in powers of two.
+template <typename T>
+__device__ __forceinline__ T* at_out(const amp_attention_args& P, const AtSeq& s, int tok, int head, int c, float f, float m, float l)
+{
+    if (c == 0 && P.lse)
+        P.lse[(long long) (s.row0 + tok) * P.heads + head] = f != f ? NAN : (l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f);
+    return reinterpret_cast<T*>(P.out) + (long long) (s.row0 + tok) * P.out_token + (long long) head * P.out_head + c;
+}
+
 template <typename T>
 __device__ __forceinline__ void at_store(const amp_attention_args& P, const AtSeq& s, int tok, int head, int c, float4 x, float m, float l)
 {
-    // (a position beyond the table: there are keys that cannot be found)
-    const float f = s.first + tok >= P.max_pages * P.page_size ? NAN : (l == 0.0f ? 0.0f : 1.0f / l);
-    T* out = reinterpret_cast<T*>(P.out) + (long long) (s.row0 + tok) * P.out_token + (long long) head * P.out_head + c;
-    *reinterpret_cast<uint2*>(out) = make_uint2(AtType<T>::pack(x.x * f, x.y * f), AtType<T>::pack(x.z * f, x.w * f));
-    if (c == 0 && P.lse)
-        P.lse[(long long) (s.row0 + tok) * P.heads + head] = f != f ? NAN : (l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f);
+    const float f = at_factor(P, s.first + tok, l);
+    *reinterpret_cast<uint2*>(at_out<T>(P, s, tok, head, c, f, m, l)) = make_uint2(AtType<T>::pack(x.x * f, x.y * f), AtType<T>::pack(x.z * f, x.w * f));
+}
+
+template <typename T>
+__device__ __forceinline__ void at_store8(const amp_attention_args& P, const AtSeq& s, int tok, int head, int c, float4 x, float4 y, float m, float l)
+{
+    const float f = at_factor(P, s.first + tok, l);
+    *reinterpret_cast<uint4*>(at_out<T>(P, s, tok, head, c, f, m, l)) =
+        make_uint4(AtType<T>::pack(x.x * f, x.y * f), AtType<T>::pack(x.z * f, x.w * f), AtType<T>::pack(y.x * f, y.y * f), AtType<T>::pack(y.z * f, y.w * f));
 }
 
 }  // namespace amp

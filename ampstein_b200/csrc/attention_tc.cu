@@ -1,0 +1,638 @@
+// Attention of prompt chunks over a paged key-value cache on the tensor cores (tcgen05, accumulators in tensor memory).
+//
+// The query heads that share a key-value head, times a sequence's new tokens, are the rows of one problem (row = token * group + head),
+// so that a tile of 128 rows spans few tokens, keys are fetched once for the whole group, and a short chunk fills its tiles. A CTA takes
+// NQ tiles of 128 rows (two up to 128 values per head, one at 256) and walks the keys that its tokens see in tiles of KB:
+//   S = Q K^T     both operands K-major in shared memory, S (128 x KB fp32) in tensor memory
+//   P = 2^(scale S - m), a row per thread: no exchange between threads; P goes back over S, in the operands' type
+//   O += P V      P from tensor memory, V as it lies in the cache (N-major), O (128 x D fp32) in tensor memory
+// With two tiles the tensor cores multiply for one while the other's softmax runs; with one tile S has two buffers, and the next
+// Q K^T runs under the softmax. m moves only when a row's maximum has grown by more than 2^8 (the sums stay far from fp32's and the
+// weights from fp16's range), so that O is rarely scaled again. Where the grid leaves SMs idle the keys of a tile are cut into
+// slices, whose parts a second kernel joins in order.
+//
+// Warps: four per row tile do the softmax (a thread a row, the warp's quarter of tensor memory), then one issues the MMAs, two load
+// keys and values by 16-byte asynchronous copies (a page of any size, strides of any kind), one rests.
+//
+// Every mbarrier wait is bounded: a role whose wait ran out hands nothing over any more, whatever depends on it runs out too, nothing
+// is stored (slices: their rows become NaN), the status word is set, and the CTA leaves when its copies and MMAs are done.
+#include "attention_tc.cuh"
+
+namespace amp {
+
+__device__ int g_at_status;
+
+constexpr unsigned AT_SPIN_LIMIT = 1u << 21;   // looks at a barrier before a wait is declared lost (a look lasts up to 4 us)
+constexpr int TA_AHEAD = 2;                    // tiles on their way when the next is requested
+constexpr float TA_SLACK = 8.0f;               // powers of two that a row's maximum may grow before O is scaled again
+
+__device__ __forceinline__ bool ta_wait(uint32_t bar, uint32_t parity)
+{
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+        "mov.u32 n, %3;\n"
+        "$TA_POLL_%=:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra $TA_DONE_%=;\n\t"
+        "sub.u32 n, n, 1;\n\t"
+        "setp.ne.u32 q, n, 0;\n\t"
+        "@q bra $TA_POLL_%=;\n"
+        "$TA_DONE_%=:\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r) : "r"(bar), "r"(parity), "n"(AT_SPIN_LIMIT) : "memory");
+    return r != 0;
+}
+
+__device__ __forceinline__ void ta_arrive(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void ta_commit(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ bool ta_elect()
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
+// Shared-memory descriptor of an operand in 128-byte swizzle: rows of 128 bytes, groups of eight rows 1024 bytes apart; block: bytes between
+// the blocks of 64 values along N (N-major operands only)
+__device__ __forceinline__ uint64_t ta_desc(uint32_t addr, uint32_t block)
+{
+    return (uint64_t) ((addr & 0x3ffff) >> 4) | ((uint64_t) (block >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// kind::f16 instruction descriptor: fp32 accumulator, 128 x n, A K-major, B K-major or N-major
+__host__ __device__ constexpr uint32_t ta_idesc(int n, bool bf16, bool b_n_major)
+{
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t) (n >> 3) << 17) | (8u << 24);
+}
+
+__device__ __forceinline__ void ta_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+__device__ __forceinline__ void ta_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+#define TA_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define TA_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// 32 columns of the thread's row of tensor memory
+__device__ __forceinline__ void ta_ld32(uint32_t addr, uint32_t* r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : TA_R8(r, 0), TA_R8(r, 8), TA_R8(r, 16), TA_R8(r, 24) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void ta_st32(uint32_t addr, const uint32_t* r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 :: "r"(addr), TA_W8(r, 0), TA_W8(r, 8), TA_W8(r, 16), TA_W8(r, 24) : "memory");
+}
+#undef TA_R8
+#undef TA_W8
+
+__device__ __forceinline__ void ta_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ta_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ta_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ta_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ta_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ float ta_exp2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Of row tile `tile` (NQ * 128 rows) of sequence s: tokens [tok0, tok1]
+template <int NQ>
+struct TaTile
+{
+    int b, tile, tok0, tok1;
+    AtSeq s;
+    AtKeys k;
+};
+
+// Sequence and row tile of the x-th tile of the call; false: there is none. By one warp.
+template <int NQ>
+__device__ __forceinline__ bool ta_find(const TaPlan& S, int x, int& b, int& tile)
+{
+    const amp_attention_args& P = S.P;
+    const int group = P.heads / P.kv_heads, lane = threadIdx.x & 31;
+    auto tiles = [&](int rows) { return rows <= S.split_rows ? 0 : (rows + NQ * 128 - 1) / (NQ * 128); };
+    if (!P.cu)
+    {
+        const int each = tiles(P.tokens / P.seqs * group);
+        b = each ? x / each : P.seqs;
+        tile = x - b * each;
+        return b < P.seqs;
+    }
+    for (int b0 = 0; b0 < P.seqs; b0 += 32)
+    {
+        int n = 0;
+        if (b0 + lane < P.seqs) n = tiles(at_seq(P, b0 + lane).count * group);
+        int sum = n;
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += y; }
+        const uint32_t hit = __ballot_sync(0xffffffffu, x < sum);
+        if (hit)
+        {
+            const int l = __ffs(hit) - 1;
+            b = b0 + l;
+            tile = x - (__shfl_sync(0xffffffffu, sum, l) - __shfl_sync(0xffffffffu, n, l));
+            return true;
+        }
+        x -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return false;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(ta_threads<D>, 1)
+void attention_tc_kernel(const TaPlan S)
+{
+    const amp_attention_args& P = S.P;
+    constexpr int NQ = ta_nq<D>, KB = ta_kb<D>, ST = ta_stages<D>, ROWS = NQ * 128;
+    constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = KB * D * 2, CH = D / 8;
+    constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+    constexpr int O_COL = 256;                 // tensor memory: S at 0 (two tiles or two buffers), O at 256
+    constexpr int S_STEP = NQ == 2 ? 128 : KB;
+    constexpr uint32_t IDESC_QK = ta_idesc(KB, BF, false), IDESC_PV = ta_idesc(D, BF, true);
+    extern __shared__ __align__(1024) unsigned char ta_mem[];
+    __shared__ uint64_t q_full, kv_full[ST], kv_free[ST], s_full[2], p_full[2], o_full, end;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_place[3];
+
+    const int t = threadIdx.x, lane = t & 31, warp = __shfl_sync(0xffffffffu, t >> 5, 0);
+    const int group = P.heads / P.kv_heads;
+    // (before tensor memory is taken: a CTA in front may still have to take its own here)
+    if (S.pdl) pdl_wait();
+    const int h = blockIdx.x % P.kv_heads, slice = blockIdx.x / P.kv_heads % S.slices;
+    const int x = S.tiles - 1 - (int) (blockIdx.x / P.kv_heads / S.slices);      // (the last tiles see most keys: first)
+    if (warp == 0)
+    {
+        int b = 0, tile = 0;
+        const bool have = ta_find<NQ>(S, x, b, tile);
+        if (lane == 0) { s_place[0] = have; s_place[1] = b; s_place[2] = tile; }
+    }
+    if (t == 0)
+    {
+        mbar_init(&q_full, 128 * NQ);
+        for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], 2); mbar_init(&kv_free[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); }
+        mbar_init(&o_full, 1);
+        mbar_init(&end, 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    if (!s_place[0]) { if (S.pdl) pdl_launch_dependents(); return; }
+    const AtSeq seq = at_seq(P, s_place[1]);
+    const int row0 = s_place[2] * ROWS, tok0 = row0 / group, tok1 = min((row0 + ROWS - 1) / group, seq.count - 1);
+    const AtKeys keys = at_keys(P, seq.first + tok0, tok1 - tok0 + 1);
+    const int n_all = (keys.count() + KB - 1) / KB;
+    const int j0 = (int) ((long long) n_all * slice / S.slices), n = (int) ((long long) n_all * (slice + 1) / S.slices) - j0;
+    const uint32_t q_s = smem_u32(ta_mem), kv_s = q_s + NQ * Q_BYTES;
+    const uint32_t full_s = smem_u32(&kv_full[0]), free_s = smem_u32(&kv_free[0]), sf = smem_u32(&s_full[0]), pf = smem_u32(&p_full[0]);
+    const bool aligned = (q_s & 1023) == 0;    // (the swizzle needs the alignment that the declaration asks for)
+
+    if (warp == 4 * NQ)
+    {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    ta_fence_before();
+    __syncthreads();
+    ta_fence_after();
+    const uint32_t tmem = s_tmem;
+    if (S.pdl) pdl_launch_dependents();
+
+    bool ok = aligned;
+    if (!aligned && t == 0) atomicExch(&g_at_status, 2);
+    // (a warp agrees on whether a wait was lost: what follows is done by whole warps)
+    auto wait = [&](uint32_t bar, uint32_t parity)
+    {
+        if (ok && !__all_sync(0xffffffffu, ta_wait(bar, parity))) { ok = false; atomicExch(&g_at_status, 1); }
+        return ok;
+    };
+    // registers of the block's launch (168 for each of its three warpgroups), given to those that hold rows
+    if constexpr (NQ == 2)
+    {
+        if (warp < 4 * NQ) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
+    }
+
+    if (warp < 4 * NQ)
+    {
+        // ---- softmax: thread t has row t of the CTA's ROWS ------------------------------------------------------------------
+        const int i = warp >> 2;               // row tile
+        const int row = row0 + t, tok = row / group, head = h * group + row - tok * group;
+        const bool have = tok < seq.count;
+        const int p = seq.first + tok;
+        {
+            // its row of Q, with the sign of the scale (the rest counts with |scale|; scale 0: scores of 0)
+            const T* q = reinterpret_cast<const T*>(P.q) + (long long) (seq.row0 + tok) * P.q_token + (long long) head * P.q_head;
+            const uint32_t flip = P.scale < 0.0f ? 0x80008000u : 0u;
+            #pragma unroll 8
+            for (int c = 0; c < CH; ++c)
+            {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (have && P.scale != 0.0f) v = *reinterpret_cast<const uint4*>(q + c * 8);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                             :: "r"(q_s + i * Q_BYTES + (c >> 3) * (128 * 128) + (t & 127) * 128 + (((c & 7) ^ (t & 7)) << 4)),
+                                "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip) : "memory");
+            }
+            ta_fence_async();
+            ta_arrive(smem_u32(&q_full));
+        }
+        // keys of the compact list that the row sees: [0, n0) and [c1, c1 + len]
+        int n0 = 0, c1 = 0, c2 = p;
+        if (P.window)
+        {
+            n0 = min(p + 1, P.sinks);
+            c1 = max(p - P.window + 1, keys.lo) - keys.lo + keys.a;
+            c2 = p - keys.lo + keys.a;
+        }
+        if (!have) { n0 = 0; c2 = -1; }
+        const uint32_t len = c2 >= c1 ? (uint32_t) (c2 - c1) : 0u;
+        if (c2 < c1) c1 = 1 << 30;
+        // the same for the row tile's first and last token: tiles that all its rows see whole need no look at single keys
+        const int ta = seq.first + (row0 + 128 * i) / group, tb = seq.first + min((row0 + 128 * i + 127) / group, seq.count - 1);
+
+        const float sc = P.scale == 0.0f ? 1.0f : fabsf(S.scale2);
+        const uint32_t lane_base = tmem + ((uint32_t) (32 * (warp & 3)) << 16);
+        const uint32_t o_t = lane_base + O_COL + (NQ == 2 ? i * 128 : 0);
+        float m = -INFINITY;
+        f32x2 l2 = pack_f32x2(0.0f, 0.0f);
+        float l = 0.0f;
+        for (int j = 0; j < n; ++j)
+        {
+            const int buf = NQ == 2 ? i : (j & 1);
+            if (!wait(sf + 8 * buf, (NQ == 2 ? j : j >> 1) & 1)) break;
+            ta_fence_after();
+            const uint32_t s_t = lane_base + buf * S_STEP;
+            uint32_t s[KB];
+            #pragma unroll
+            for (int c = 0; c < KB; c += 32) ta_ld32(s_t + c, s + c);
+            ta_wait_ld();
+            const int k0 = (j0 + j) * KB, kl = k0 + KB - 1;
+            const bool whole = kl < keys.count() && keys.key(kl) <= ta && (!P.window || keys.key(k0) > tb - P.window || keys.key(kl) < P.sinks);
+            if (!whole)
+            {
+                #pragma unroll
+                for (int c = 0; c < KB; ++c)
+                {
+                    const int at = k0 + c;
+                    const bool see = at < n0 || (uint32_t) (at - c1) <= len;
+                    s[c] = see ? s[c] : 0xff800000u;
+                }
+            }
+            float top = -INFINITY, top2 = -INFINITY;
+            #pragma unroll
+            for (int c = 0; c < KB; c += 4)
+            {
+                top = fmaxf(fmaxf(top, __uint_as_float(s[c])), __uint_as_float(s[c + 1]));
+                top2 = fmaxf(fmaxf(top2, __uint_as_float(s[c + 2])), __uint_as_float(s[c + 3]));
+            }
+            top = fmaxf(top, top2);
+            const bool move = top > m && (m == -INFINITY || (top - m) * sc > TA_SLACK);
+            if (__any_sync(0xffffffffu, move))
+            {
+                const float f = move ? ta_exp2((m - top) * sc) : 1.0f;       // (m of -inf: 0)
+                if (move) m = top;
+                l2 = mul_f32x2(l2, pack_f32x2(f, f));
+                if (j > 0)
+                {
+                    if constexpr (NQ == 1) { if (!wait(smem_u32(&o_full), (j - 1) & 1)) break; ta_fence_after(); }
+                    #pragma unroll
+                    for (int c = 0; c < D; c += 32)
+                    {
+                        uint32_t o[32];
+                        ta_ld32(o_t + c, o);
+                        ta_wait_ld();
+                        #pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        ta_st32(o_t + c, o);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.0f : -m * sc;
+            const f32x2 sc2 = pack_f32x2(sc, sc), base2 = pack_f32x2(base, base);
+            #pragma unroll
+            for (int c = 0; c < KB; c += 64)
+            {
+                uint32_t w[32];
+                #pragma unroll
+                for (int e = 0; e < 64; e += 2)
+                {
+                    const float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[c + e]), __uint_as_float(s[c + e + 1])), sc2, base2));
+                    const float e0 = ta_exp2(y.x), e1 = ta_exp2(y.y);
+                    l2 = add_f32x2(l2, pack_f32x2(e0, e1));
+                    w[e / 2] = AtType<T>::pack(e0, e1);
+                }
+                ta_st32(s_t + c / 2, w);
+            }
+            ta_wait_st();
+            ta_fence_before();
+            ta_arrive(pf + 8 * buf);
+        }
+        const float2 ls = unpack_f32x2(l2);
+        l = ls.x + ls.y;
+        if (n > 0 && ok)
+        {
+            wait(smem_u32(&o_full), NQ == 2 ? 0 : (n - 1) & 1);
+            ta_fence_after();
+        }
+        const float m2 = m == -INFINITY ? m : m * sc;
+        if (S.slices > 1)
+        {
+            // a part: rows side by side, so that a warp writes whole lines; lost: NaN
+            float* const part = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(P.workspace) + S.part_offset)
+                                + (size_t) ((x * P.kv_heads + h) * S.slices + slice) * ta_part_floats(D);
+            if (n > 0)
+            {
+                #pragma unroll
+                for (int c = 0; c < D; c += 32)
+                {
+                    uint32_t o[32];
+                    ta_ld32(o_t + c, o);
+                    ta_wait_ld();
+                    if (have)
+                    {
+                        #pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            reinterpret_cast<uint4*>(part)[((c + e) / 4) * ROWS + t] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                }
+            }
+            if (have) reinterpret_cast<float2*>(part + ROWS * D)[t] = make_float2(m2, ok ? l : NAN);
+        }
+        else if (ok)
+        {
+            #pragma unroll
+            for (int c = 0; c < D; c += 32)
+            {
+                uint32_t o[32];
+                if (n > 0) { ta_ld32(o_t + c, o); ta_wait_ld(); }
+                if (have)
+                {
+                    #pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                    {
+                        const float4 a = n > 0 ? make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])) : make_float4(0, 0, 0, 0);
+                        const float4 b = n > 0 ? make_float4(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]), __uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])) : make_float4(0, 0, 0, 0);
+                        at_store8<T>(P, seq, tok, head, c + e, a, b, m2, l);
+                    }
+                }
+            }
+        }
+    }
+    else if (warp == 4 * NQ)
+    {
+        // ---- MMAs ------------------------------------------------------------------------------------------------------------
+        int stage = 0; uint32_t wrap = 0;      // of the next tile in the order K0, K1, V0, K2, V1, ...
+        auto next = [&]() { if (++stage == ST) { stage = 0; wrap ^= 1; } };
+        auto qk = [&](int buf, int tile, int at)
+        {
+            const uint64_t a = ta_desc(q_s + tile * Q_BYTES, 0), b = ta_desc(kv_s + at * KV_BYTES, 0);
+            if (ta_elect())
+            {
+                #pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    ta_mma_ss(tmem + buf * S_STEP, a + (kk >> 2) * (128 * 128 >> 4) + (kk & 3) * 2, b + (kk >> 2) * (KB * 128 >> 4) + (kk & 3) * 2, IDESC_QK, kk > 0);
+                ta_commit(sf + 8 * buf);
+            }
+            __syncwarp();
+        };
+        auto pv = [&](int buf, int tile, int at, bool first)
+        {
+            const uint64_t b = ta_desc(kv_s + at * KV_BYTES, KB * 128);
+            if (ta_elect())
+            {
+                #pragma unroll
+                for (int kk = 0; kk < KB / 16; ++kk)
+                    ta_mma_ts(tmem + O_COL + (NQ == 2 ? tile * 128 : 0), tmem + buf * S_STEP + 8 * kk, b + kk * (16 * 128 >> 4), IDESC_PV, !first || kk > 0);
+            }
+            __syncwarp();
+        };
+        auto commit = [&](uint32_t bar) { if (ta_elect()) ta_commit(bar); __syncwarp(); };
+        if (n > 0 && wait(smem_u32(&q_full), 0) && wait(full_s + 8 * stage, wrap))
+        {
+            ta_fence_after();
+            #pragma unroll
+            for (int i = 0; i < NQ; ++i) qk(i, i, stage);
+            commit(free_s + 8 * stage);
+            next();
+            for (int j = 0; j < n; ++j)
+            {
+                int kst = 0;
+                if (j + 1 < n)
+                {
+                    if (!wait(full_s + 8 * stage, wrap)) break;
+                    kst = stage;
+                    next();
+                }
+                if constexpr (NQ == 1)
+                {
+                    if (j + 1 < n) { ta_fence_after(); qk((j + 1) & 1, 0, kst); commit(free_s + 8 * kst); }
+                }
+                if (!wait(full_s + 8 * stage, wrap)) break;
+                const int vst = stage;
+                next();
+                #pragma unroll
+                for (int i = 0; i < NQ; ++i)
+                {
+                    const int buf = NQ == 2 ? i : (j & 1);
+                    if (!wait(pf + 8 * buf, (NQ == 2 ? j : j >> 1) & 1)) break;
+                    ta_fence_after();
+                    pv(buf, i, vst, j == 0);
+                    if (i == NQ - 1) commit(free_s + 8 * vst);
+                    if constexpr (NQ == 1) commit(smem_u32(&o_full));
+                    else if (j + 1 < n)
+                    {
+                        qk(i, i, kst);
+                        if (i == NQ - 1) commit(free_s + 8 * kst);
+                    }
+                }
+                if (!ok) break;
+            }
+            if (NQ == 2 && ok) commit(smem_u32(&o_full));
+        }
+        commit(smem_u32(&end));
+        ta_wait(smem_u32(&end), 0);            // (bounded; the accumulators are given back only then)
+    }
+    else if (warp <= 4 * NQ + 2)
+    {
+        // ---- keys and values: half of a tile's rows per warp ------------------------------------------------------------------
+        constexpr int RW = KB / 2, PER = CH >= 32 ? 1 : 32 / CH;
+        const int r_first = (warp - 4 * NQ - 1) * RW, tiles = 2 * n;
+        int issued = 0;
+        auto hand_over = [&](int tile)
+        {
+            ta_fence_async();
+            __syncwarp();
+            if (lane == 0) ta_arrive(full_s + 8 * (tile % ST));
+        };
+        for (; issued < tiles; ++issued)
+        {
+            // tile 0 is K0, then K1, V0, K2, V1, ..., the last one V(n - 1)
+            const bool is_v = issued > 0 && (issued % 2 == 0 || issued == tiles - 1);
+            const int j = issued == 0 ? 0 : issued == tiles - 1 ? n - 1 : is_v ? issued / 2 - 1 : (issued + 1) / 2;
+            const int stage = issued % ST;
+            if (issued >= ST && !wait(free_s + 8 * stage, (issued / ST - 1) & 1)) break;
+            if (!ok) break;
+            const T* const base = reinterpret_cast<const T*>(is_v ? P.v_cache : P.k_cache) + (long long) h * (is_v ? P.v_head : P.k_head);
+            const long long page_st = is_v ? P.v_page : P.k_page, row_st = is_v ? P.v_row : P.k_row;
+            long long off[RW / 32];
+            int state[RW / 32];                // 1: fetch, 0: beyond the keys, -1: on a page outside the pool
+            #pragma unroll
+            for (int g = 0; g < RW / 32; ++g)
+            {
+                const int c = (j0 + j) * KB + r_first + 32 * g + lane;
+                off[g] = 0; state[g] = 0;
+                if (c < keys.count())
+                {
+                    const int key = keys.key(c), pg = key / P.page_size, page = P.table[(long long) s_place[1] * P.table_row + pg];
+                    state[g] = page >= 0 && page < P.pages ? 1 : -1;
+                    if (state[g] > 0) off[g] = page * page_st + (key - pg * P.page_size) * row_st;
+                }
+            }
+            const uint32_t to = kv_s + stage * KV_BYTES;
+            #pragma unroll
+            for (int g = 0; g < RW / 32; ++g)
+            {
+                #pragma unroll 8
+                for (int r0 = 0; r0 < 32; r0 += PER)
+                {
+                    const int r = r0 + (CH >= 32 ? 0 : lane / CH), c = lane % CH, at = r_first + 32 * g + r;
+                    const long long o = __shfl_sync(0xffffffffu, off[g], r);
+                    const int st = __shfl_sync(0xffffffffu, state[g], r);
+                    const uint32_t dst = to + (c >> 3) * (KB * 128) + at * 128 + (((c & 7) ^ (at & 7)) << 4);
+                    if (st < 0 && !is_v)       // a key that cannot be found is NaN to the rows that see it
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" :: "r"(dst), "r"(0x7fff7fffu) : "memory");
+                    else
+                        at_copy16(dst, base + o + c * 8, st > 0);
+                }
+            }
+            cp_async_commit();
+            if (issued >= TA_AHEAD) { asm volatile("cp.async.wait_group %0;" :: "n"(TA_AHEAD) : "memory"); hand_over(issued - TA_AHEAD); }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (ok) for (int tile = max(0, issued - TA_AHEAD); tile < issued; ++tile) hand_over(tile);
+    }
+    ta_fence_before();
+    __syncthreads();
+    if (warp == 4 * NQ)
+    {
+        ta_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// Joins the slices of row tile x of key-value head h (blockIdx.x), 16 values of every row (blockIdx.y)
+template <typename T, int D>
+__global__ __launch_bounds__(128 * ta_nq<D>)
+void attention_tc_join_kernel(const TaPlan S)
+{
+    const amp_attention_args& P = S.P;
+    constexpr int NQ = ta_nq<D>, ROWS = 128 * NQ;
+    __shared__ int s_place[3];
+    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
+    const int t = threadIdx.x, h = blockIdx.x % P.kv_heads, x = blockIdx.x / P.kv_heads, group = P.heads / P.kv_heads;
+    if (t < 32)
+    {
+        int b = 0, tile = 0;
+        const bool have = ta_find<NQ>(S, x, b, tile);
+        if (t == 0) { s_place[0] = have; s_place[1] = b; s_place[2] = tile; }
+    }
+    __syncthreads();
+    if (!s_place[0]) return;
+    const AtSeq seq = at_seq(P, s_place[1]);
+    const int row = s_place[2] * ROWS + t, tok = row / group;
+    if (tok >= seq.count) return;
+    const float* const parts = reinterpret_cast<const float*>(reinterpret_cast<const unsigned char*>(P.workspace) + S.part_offset)
+                               + (size_t) blockIdx.x * S.slices * ta_part_floats(D);
+    auto ml = [&](int i) { return reinterpret_cast<const float2*>(parts + i * ta_part_floats(D) + ROWS * D)[t]; };
+    float m = -INFINITY, l = 0.0f;
+    for (int i = 0; i < S.slices; ++i) m = fmaxf(m, ml(i).x);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float4 o[4];
+    #pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    #pragma unroll 2
+    for (int i = 0; i < S.slices; ++i)
+    {
+        const float2 v = ml(i);
+        if (v.y == 0.0f) continue;             // (a slice without keys wrote nothing else)
+        const float f = ta_exp2(v.x - base);
+        l += v.y != v.y ? v.y : v.y * f;
+        const float4* p = reinterpret_cast<const float4*>(parts + i * ta_part_floats(D)) + (size_t) blockIdx.y * 4 * ROWS + t;
+        #pragma unroll
+        for (int c = 0; c < 4; ++c)
+        {
+            const float4 y = p[c * ROWS];
+            o[c].x += y.x * f; o[c].y += y.y * f; o[c].z += y.z * f; o[c].w += y.w * f;
+        }
+    }
+    const int head = h * group + row - tok * group;
+    at_store8<T>(P, seq, tok, head, blockIdx.y * 16, o[0], o[1], m, l);
+    at_store8<T>(P, seq, tok, head, blockIdx.y * 16 + 8, o[2], o[3], m, l);
+}
+
+template <typename T, int D>
+static int ta_launch(const TaPlan& S, cudaStream_t stream)
+{
+    const amp_attention_args& P = S.P;
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return cuda_rc(e, "attention device");
+    if (cudaError_t e = ensure_smem(attention_tc_kernel<T, D>, ta_smem<D>, dev)) return cuda_rc(e, "attention shared memory");
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(S.tiles * S.slices * P.kv_heads, 1, 1);
+    cfg.blockDim = dim3(ta_threads<D>, 1, 1);
+    cfg.dynamicSmemBytes = ta_smem<D>;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = S.pdl ? 1 : 0;
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, attention_tc_kernel<T, D>, S)) return cuda_rc(e, "attention launch");
+    if (S.slices == 1) return 0;
+    cfg.gridDim = dim3(S.tiles * P.kv_heads, D / 16, 1);
+    cfg.blockDim = dim3(128 * ta_nq<D>, 1, 1);
+    cfg.dynamicSmemBytes = 0;
+    return cuda_rc(cudaLaunchKernelEx(&cfg, attention_tc_join_kernel<T, D>, S), "attention join launch");
+}
+
+int attention_tc(const TaPlan& S, cudaStream_t stream)
+{
+    if (S.tiles == 0) return 0;
+    const int d = S.P.dim;
+    if (S.P.bf16) return d == 64 ? ta_launch<__nv_bfloat16, 64>(S, stream) : d == 128 ? ta_launch<__nv_bfloat16, 128>(S, stream) : ta_launch<__nv_bfloat16, 256>(S, stream);
+    return d == 64 ? ta_launch<__half, 64>(S, stream) : d == 128 ? ta_launch<__half, 128>(S, stream) : ta_launch<__half, 256>(S, stream);
+}
+
+}  // namespace amp
+
+AMP_API int amp_b200_attention_status(int* out)
+{
+    using namespace amp;
+    int v = 0, zero = 0;
+    if (cudaError_t e = cudaMemcpyFromSymbol(&v, g_at_status, sizeof(int))) return cuda_rc(e, "status read");
+    if (v) if (cudaError_t e = cudaMemcpyToSymbol(g_at_status, &zero, sizeof(int))) return cuda_rc(e, "status clear");
+    if (out) *out = v;
+    return 0;
+}

@@ -296,8 +296,10 @@ typedef struct amp_attention_args
     int tokens, seqs, heads, kv_heads, dim, pages, page_size, max_pages, window, sinks, bf16, pos64;
     float scale;
 } amp_attention_args;
-long amp_b200_attention_workspace(int tokens, int seqs, int heads, int kv_heads, int dim, int ragged, long max_keys);
+long amp_b200_attention_workspace(int tokens, int seqs, int heads, int kv_heads, int dim, int ragged, long max_keys, int window, int sinks);
 int amp_b200_attention(const amp_attention_args* args, cudaStream_t stream);
+/* 0, or 1: a bounded wait inside the prompt form ran out, and what depended on it was not stored, since the last call (which clears it) */
+int amp_b200_attention_status(int* out);
 
 /*
  * Copies whole pages inside caches: page dst[i] := page src[i] in every layer of every cache, for forks, defragmentation and
