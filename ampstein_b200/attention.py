@@ -29,6 +29,18 @@ _ROPE = struct.Struct("=10q15q12if4x")             # amp_rope_args
 _ATTENTION = struct.Struct("=10q11q12if4x")        # amp_attention_args
 
 
+_direct = None                         # the calls of csrc_py/tensor_call.h by name; {} where torch has no table for them
+
+
+def _calls():
+    global _direct
+    _lib.lib()
+    from . import _fast
+    names = ("rope_call", "attention_call", "copy_call")
+    _direct = {n: getattr(_fast, n) for n in names} if hasattr(_fast, "tensor_setup") and _fast.tensor_setup(torch.Tensor) else {}
+    return _direct
+
+
 def _cuda(name, what, t, dev=None):
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s: %s must be a torch tensor" % (name, what))
@@ -142,6 +154,12 @@ def rope_frequencies(rot, theta=10000.0, scaling=None, device="cuda"):
 
 
 def _rope(name, q, kv, pos, inv_freq, cu, interleaved, mscale, out):
+    call = (_calls() if _direct is None else _direct).get("rope_call")
+    if call is not None and type(q) is torch.Tensor:
+        k, v, kc, vc, table = kv or (None,) * 5
+        y = q.new_empty(q.shape) if out is None else out
+        if call(q, k, v, pos, inv_freq, kc, vc, table, cu, interleaved, mscale, y) is not None:
+            return y
     _cuda(name, "q", q)
     dev, dtype = q.get_device(), q.dtype
     if dtype not in _DTYPES:
@@ -225,6 +243,15 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
     anything; a token with a visible key on a page outside the pool, or beyond the table, gets NaN. Single tokens, a few drafted ones and
     prompt chunks may be mixed in one call with cu."""
     name = "paged_attention"
+    call = (_calls() if _direct is None else _direct).get("attention_call")
+    if call is not None and type(q) is torch.Tensor:
+        y = q.new_empty(q.shape) if out is None else out
+        s = q.shape[-1] ** -0.5 if scale is None and q.shape and q.shape[-1] else scale
+        n = call(q, k_cache, v_cache, table, pos, cu, window, sinks, s, y, lse, None)
+        if n:
+            n = call(q, k_cache, v_cache, table, pos, cu, window, sinks, s, y, lse, torch.empty(n, dtype=torch.uint8, device=q.device))
+        if n == 0:
+            return y
     _cuda(name, "q", q)
     dev, dtype = q.get_device(), q.dtype
     if dtype not in _DTYPES:
@@ -289,6 +316,9 @@ def copy_pages(caches, src, dst):
     page outside the pool, a page written twice and a page that is both read and written by different copies are refused. Returns
     caches."""
     name = "copy_pages"
+    call = (_calls() if _direct is None else _direct).get("copy_call")
+    if call is not None and call(caches, src, dst) == 0:
+        return caches
     src, dst = _page_list("src", src), _page_list("dst", dst)
     if len(src) != len(dst):
         raise ValueError("%s: %d sources for %d destinations" % (name, len(src), len(dst)))

@@ -67,17 +67,21 @@ def build(force=False, verbose=False):
 
 
 FAST_SRC = os.path.join(HERE, "csrc_py", "fast_call.c")
+FAST_TENSORS = os.path.join(HERE, "csrc_py", "tensor_call.h")
 FAST = os.path.join(HERE, "_fast.so")
 
 
 def build_fast_call(force=False):
     """Builds ampstein_b200/_fast.so: the per-token entries of the C ABI as builtins (plain gcc)."""
     header = os.path.join(HERE, "..", "include", "ampstein_b200.h")
-    if not force and os.path.exists(FAST) and os.path.getmtime(FAST) >= max(os.path.getmtime(FAST_SRC), os.path.getmtime(header)):
+    if not force and os.path.exists(FAST) and os.path.getmtime(FAST) >= max(os.path.getmtime(f) for f in (FAST_SRC, FAST_TENSORS, header)):
         return FAST
+    import importlib.util
     import sysconfig
+    torch_at = importlib.util.find_spec("torch")             # (for its dlpack.h; the calls that need it are left out without)
+    torch_inc = ["-I" + os.path.join(p, "include") for p in (torch_at.submodule_search_locations if torch_at else [])]
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
-    cmd = [os.environ.get("CC", "gcc"), "-O2", "-fPIC", "-shared", "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include"),
+    cmd = [os.environ.get("CC", "gcc"), "-O2", "-fPIC", "-shared", "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include")] + torch_inc + [
            FAST_SRC, "-o", FAST, "-L" + HERE, "-lampstein_b200", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

@@ -117,9 +117,15 @@ ENTRY(name) \
 STRUCT(amp_b200_rope, amp_rope_args)
 STRUCT(amp_b200_attention, amp_attention_args)
 
+#include "tensor_call.h"
+
 #define M(name) { #name, (PyCFunction) (void (*)(void)) py_##name, METH_FASTCALL, NULL }
 static PyMethodDef methods[] = { M(amp_exl3_gemm), M(amp_exl3_gemm_bf16), M(amp_exl3_mgemm), M(amp_exl3_mgemm_bf16), M(amp_exl3_moe_coop),
                                  M(amp_exl3_moe_sorted), M(amp_b200_rms_norm_res), M(amp_b200_silu_mul),
-                                 M(amp_b200_rope), M(amp_b200_attention), { NULL, NULL, 0, NULL } };
+                                 M(amp_b200_rope), M(amp_b200_attention),
+#ifdef TENSOR_CALLS
+                                 M(tensor_setup), M(rope_call), M(attention_call), M(copy_call),
+#endif
+                                 { NULL, NULL, 0, NULL } };
 static struct PyModuleDef module = { PyModuleDef_HEAD_INIT, "_fast", NULL, -1, methods, NULL, NULL, NULL, NULL };
 PyMODINIT_FUNC PyInit__fast(void) { return PyModule_Create(&module); }

@@ -283,3 +283,31 @@ def test_refusals(amp):
         with pytest.raises(kind):
             call()
             pytest.fail("call %d was taken" % i)
+
+
+def test_calls_without_the_tensor_table(amp, monkeypatch):
+    """The checks in Python and the ones on DLPack descriptions make the same calls"""
+    from ampstein_b200 import attention as at
+    assert at._calls()                                                  # this torch has the table
+    pos, counts = [40, 700], [3, 3]
+    q, k, v, table = make(pos, counts, 8, 2, 128, 16, B, window=100, sinks=3)
+    p, cu = torch.tensor(pos, device="cuda"), cu_of(counts)
+    inv_freq, m = amp.rope_frequencies(128, scaling=dict(kind="yarn", factor=4.0))
+    new = torch.randn((6, 4, 128), device="cuda").to(B)
+
+    def run():
+        a, b = k.clone(), v.clone()
+        lse = torch.zeros((6, 8), device="cuda")
+        r = amp.rope_append(q, new[:, :2], new[:, 2:], p, inv_freq, a, b, table, cu=cu, interleaved=True, mscale=m)
+        o = amp.paged_attention(r, a, b, table, p, cu=cu, window=100, sinks=3, scale=0.1, lse=lse)
+        w = amp.paged_attention(q, k, v, table, p, window=100, sinks=3)
+        amp.copy_pages([a, b], [0, 1], [2, 3])
+        return r, o, w, lse, a, b, amp.rope(q, p, inv_freq)
+
+    want = run()
+    monkeypatch.setattr(at, "_direct", {})
+    for x, y in zip(want, run()):
+        assert torch.equal(torch.nan_to_num(x), torch.nan_to_num(y))
+    monkeypatch.undo()
+    par = torch.nn.Parameter(q, requires_grad=False)                    # another type than a plain tensor
+    assert torch.equal(amp.paged_attention(par, k, v, table, p, window=100, sinks=3), want[2])
