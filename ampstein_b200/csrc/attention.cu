@@ -2,35 +2,39 @@
 // cache's length and joined.
 //
 // The query heads that share a key-value head, times the sequence's new tokens, are the rows of one problem (row = token * group +
-// head); 16 rows make a row tile, the M of mma.sync m16n8k16. The keys that a sequence's new tokens see, counted through (the
-// first tokens and the window's without what lies between), are cut into units of 64. All units of the call, ordered (sequence,
-// head, row tile, unit), are cut into equal contiguous ranges, one per CTA: the lengths stand on the device, so that a captured
-// graph replays with other lengths, and long and short sequences share the device evenly. What a CTA holds of a (sequence, head,
-// row tile) that other CTAs share goes to the workspace as partial result (o, m, l); a second kernel joins them in ascending key
-// order, so that the sums are the same in every run.
+// head). A row tile is 16 * WR rows, 16 being the M of mma.sync m16n8k16. The keys that a sequence's new tokens see, counted through
+// (the first tokens and the window's, without what lies between), are cut into units. All units of the call, ordered (sequence, head,
+// row tile, unit), are cut into equal contiguous ranges, one per CTA: the lengths stand on the device, so that a captured graph replays
+// with other lengths, and long and short sequences share the device evenly. What a CTA holds of a (sequence, head, row tile) that other
+// CTAs share, a part (o, m, l), goes to the workspace, and a second kernel joins the parts in ascending key order: the same sums in every
+// run.
 //
-// A warp owns 16 keys of every unit and a ring of stages of its own, filled with 16-byte asynchronous copies by its own lanes: the
-// loop has no barrier between warps, each keeps its own m, l and o, and the four meet when a segment ends. The rings run ahead over
-// the ends of segments.
+// The warps of a CTA are WK groups of WR: a group owns KW keys of every unit, its warps 16 rows each. A group has a ring of half
+// stages (KW keys, then their values), filled by its own lanes with 16-byte asynchronous copies, and meets nobody else until the segment
+// ends: every warp keeps m, l and o of its rows over its keys. The rings run ahead over the ends of segments.
 #include "attention_tc.cuh"
 
 namespace amp {
 
-constexpr int AT_ROWS = 16;                    // rows of a row tile
-constexpr int AT_UNIT = 64;                    // keys of a unit: 16 per warp
-constexpr int AT_DESC = 8;                     // ints of a CTA's description for the join
+constexpr int AT_MAX_PER_THREAD = 32;          // sequences counted by one warp; above, the block counts
 
-template <int D> constexpr int at_stages = D == 64 ? 4 : 3;
+template <int D> constexpr int at_warps = D == 256 ? 8 : 4;
+template <int D> constexpr int at_kw = D == 64 ? 32 : 16;      // keys of a group's step
 template <int D> constexpr int at_ctas = D == 64 ? 3 : (D == 128 ? 2 : 1);     // per SM
-template <int D> constexpr int at_stage_bytes = 64 * D;        // of one warp: 16 keys and 16 values; also 16 x D floats of o
-template <int D> constexpr int at_smem = 4 * at_stages<D> * at_stage_bytes<D>;
+template <int D> constexpr int at_half_bytes = at_kw<D> * D * 2;
+template <int D> constexpr int at_smem = (D == 64 ? 64 : D == 128 ? 96 : 192) * 1024;
+template <int D, int WR> constexpr int at_wk = at_warps<D> / WR;
+template <int D, int WR> constexpr int at_halves = at_smem<D> / (at_wk<D, WR> * at_half_bytes<D>);
+template <int D, int WR> constexpr int at_unit = at_wk<D, WR> * at_kw<D>;      // keys
 
 struct AtPlan
 {
     amp_attention_args P;
     int grid;                                  // CTAs of the split form
+    int unit, rows;                            // keys of a unit, rows of a row tile
     int split_rows;                            // with cu: sequences of more rows (tokens x group) are the prompt form's
     int whole;                                 // 1: every (sequence, head, row tile) belongs to one CTA, nothing to join
+    int by_segment;                            // join: blockIdx.x is a segment, else the CTA whose range begins inside it
     int pdl;
     float scale2;                              // scale * log2(e)
 };
@@ -58,14 +62,14 @@ __device__ __forceinline__ void at_mma(float (&c)[4], const uint32_t (&a)[4], ui
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Row tiles of a sequence, and units of each of them
+// Row tiles of a sequence, and units of each of them (one at least: a segment without keys stores its zeros)
 __device__ __forceinline__ int at_row_tiles(const AtPlan& S, const AtSeq& s)
 {
     const int rows = s.count * (S.P.heads / S.P.kv_heads);
-    return rows > S.split_rows ? 0 : (rows + AT_ROWS - 1) / AT_ROWS;
+    return rows > S.split_rows ? 0 : (rows + S.rows - 1) / S.rows;
 }
 
-__device__ __forceinline__ int at_units(const AtKeys& k) { return max(1, (k.count() + AT_UNIT - 1) / AT_UNIT); }
+__device__ __forceinline__ int at_units(const AtPlan& S, const AtKeys& k) { return max(1, (k.count() + S.unit - 1) / S.unit); }
 
 // A place in the order of units
 struct AtCursor
@@ -79,64 +83,51 @@ struct AtCursor
         s = at_seq(S.P, b);
         k = at_keys(S.P, s.first, s.count);
         tiles = at_row_tiles(S, s);
-        units = at_units(k);
+        units = at_units(S, k);
+    }
+    // the at-th unit of sequence b
+    __device__ __forceinline__ void place(const AtPlan& S, int seq, long long at)
+    {
+        b = seq;
+        load(S);
+        h = (int) (at / ((long long) tiles * units));
+        rt = (int) (at / units - (long long) h * tiles);
+        u = (int) (at % units);
     }
     // to the next unit; the caller knows that there is one
-    __device__ __forceinline__ bool advance(const AtPlan& S)
+    __device__ __forceinline__ void advance(const AtPlan& S)
     {
-        if (++u < units) return false;
+        if (++u < units) return;
         u = 0;
-        if (++rt < tiles) return true;
+        if (++rt < tiles) return;
         rt = 0;
-        if (++h < S.P.kv_heads) return true;
+        if (++h < S.P.kv_heads) return;
         h = 0;
         do { ++b; load(S); } while (!tiles && b + 1 < S.P.seqs);
-        return true;
     }
 };
 
-// Workspace: descriptions of the CTAs' first segments, then two partial results per CTA (16 rows of o, their m and l): of the
-// segment that began before the CTA, and of the one that it does not end
-__host__ __device__ constexpr size_t at_desc_bytes(int grid) { return ((size_t) grid * AT_DESC * 4 + 127) / 128 * 128; }
-__host__ __device__ constexpr size_t at_part_floats(int dim) { return (size_t) AT_ROWS * (dim + 2); }
-
-template <typename T, int D>
-__global__ __launch_bounds__(128, at_ctas<D>)
-void attention_split_kernel(const AtPlan S)
+// Units of the sequences, counted. Up to 32 sequences every warp does it by itself, one per lane; beyond, the block, a run per thread.
+// (all threads of the block call it)
+struct AtCount
 {
-    const amp_attention_args& P = S.P;
-    constexpr int NST = at_stages<D>, STAGE = at_stage_bytes<D>, CHUNKS = D / 8;
-    extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float s_ml[4][AT_ROWS][2];
-    __shared__ uint32_t s_flags[4][NST];       // per warp and stage: keys that count, keys on a page outside the pool (upper half)
-    __shared__ long long s_scan[128];
-    __shared__ int s_place[5];
+    int b0, b1;                                // this lane's, or thread's, sequences
+    long long before, mine, total;             // units in front of them, of them, of all
+    bool warp;                                 // counted by the warp
 
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, cta = blockIdx.x;
-    const int group = P.heads / P.kv_heads;
-    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
-    int* desc = reinterpret_cast<int*>(P.workspace) + (size_t) cta * AT_DESC;
-
-    // the CTA's range of units
-    AtCursor in;
-    long long left;
-    if (S.whole)
+    template <int NT>
+    __device__ __forceinline__ void count(const AtPlan& S, long long* s_scan)
     {
-        in.b = 0; in.load(S);                                // (all sequences have as many tokens)
-        const int per = P.kv_heads * in.tiles;
-        in.b = cta / per; in.h = cta % per / in.tiles; in.rt = cta % in.tiles; in.u = 0;
-        in.load(S);
-        left = in.units;
-    }
-    else
-    {
-        // prefix sums over the sequences: a thread counts a run of them
-        const int run = (P.seqs + 127) / 128, b0 = min(P.seqs, t * run), b1 = min(P.seqs, b0 + run);
-        long long mine = 0;
+        const int t = threadIdx.x, lane = t & 31;
+        warp = S.P.seqs <= AT_MAX_PER_THREAD;
+        const int run = warp ? 1 : (S.P.seqs + NT - 1) / NT;
+        b0 = min(S.P.seqs, (warp ? lane : t) * run);
+        b1 = min(S.P.seqs, b0 + run);
+        mine = 0;
         for (int b = b0; b < b1; ++b)
         {
-            const AtSeq s = at_seq(P, b);
-            mine += (long long) P.kv_heads * at_row_tiles(S, s) * at_units(at_keys(P, s.first, s.count));
+            const AtSeq s = at_seq(S.P, b);
+            mine += (long long) S.P.kv_heads * at_row_tiles(S, s) * at_units(S, at_keys(S.P, s.first, s.count));
         }
         long long sum = mine;
         #pragma unroll
@@ -145,64 +136,123 @@ void attention_split_kernel(const AtPlan S)
             const long long x = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += x;
         }
-        if (lane == 31) s_scan[warp] = sum;
-        __syncthreads();
-        long long total = 0;
-        for (int w = 0; w < 4; ++w) { if (w == warp) sum += total; total += s_scan[w]; }
-        const int ctas = (int) min((long long) S.grid, total);
-        if (cta >= ctas)
+        if (warp)
         {
-            if (t == 0) desc[0] = -1;
+            total = __shfl_sync(0xffffffffu, sum, 31);
+            before = sum - mine;
             return;
         }
-        const long long u0 = cta * total / ctas;
-        left = (cta + 1) * total / ctas - u0;
-        if (u0 >= sum - mine && u0 < sum)                    // in this thread's run of sequences
+        if (lane == 31) s_scan[t >> 5] = sum;
+        __syncthreads();
+        total = 0;
+        before = sum - mine;
+        for (int w = 0; w < NT / 32; ++w) { if (w == t >> 5) before += total; total += s_scan[w]; }
+    }
+
+    // sequence of unit u, and the units in front of the sequence. (u < total)
+    __device__ __forceinline__ void find(const AtPlan& S, long long u, int& b, long long& front, long long* s_found) const
+    {
+        const bool here = u >= before && u < before + mine;
+        if (warp)
         {
-            long long at = u0 - (sum - mine);
-            for (int b = b0; b < b1; ++b)
+            const int l = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+            b = l;
+            front = __shfl_sync(0xffffffffu, before, l);
+            return;
+        }
+        if (here)
+        {
+            long long at = before;
+            for (int i = b0; i < b1; ++i)
             {
-                AtCursor c;
-                c.b = b; c.load(S);
-                const long long n = (long long) P.kv_heads * c.tiles * c.units;
-                if (at < n)
-                {
-                    s_place[0] = b;
-                    s_place[1] = (int) (at / (c.tiles * c.units));
-                    s_place[2] = (int) (at / c.units) % c.tiles;
-                    s_place[3] = (int) (at % c.units);
-                    break;
-                }
-                at -= n;
+                const AtSeq s = at_seq(S.P, i);
+                const long long n = (long long) S.P.kv_heads * at_row_tiles(S, s) * at_units(S, at_keys(S.P, s.first, s.count));
+                if (u < at + n) { s_found[0] = i; s_found[1] = at; break; }
+                at += n;
             }
         }
         __syncthreads();
-        in.b = s_place[0]; in.h = s_place[1]; in.rt = s_place[2]; in.u = s_place[3];
-        in.load(S);
-        if (t == 0)
+        b = (int) s_found[0];
+        front = s_found[1];
+    }
+
+    // units in front of sequence b
+    __device__ __forceinline__ long long front_of(const AtPlan& S, int b, long long* s_found) const
+    {
+        if (warp) return __shfl_sync(0xffffffffu, before, b);
+        if (b >= b0 && b < b1)
         {
-            // a segment that began before this CTA: which CTAs hold parts of it
-            const long long g0 = u0 - in.u, g1 = g0 + in.units;
-            desc[0] = in.u ? in.b : -1;
-            desc[1] = in.h;
-            desc[2] = in.rt;
-            desc[3] = (int) (((g0 + 1) * ctas - 1) / total);
-            desc[4] = (int) ((g1 * ctas - 1) / total);
+            long long at = before;
+            for (int i = b0; i < b; ++i)
+            {
+                const AtSeq s = at_seq(S.P, i);
+                at += (long long) S.P.kv_heads * at_row_tiles(S, s) * at_units(S, at_keys(S.P, s.first, s.count));
+            }
+            s_found[0] = at;
         }
+        __syncthreads();
+        return s_found[0];
+    }
+
+    __device__ __forceinline__ int ctas(const AtPlan& S) const { return (int) min((long long) S.grid, total); }
+};
+
+// Workspace: two parts per CTA (o of the row tile, then m and l of its rows): of the segment that began before the CTA, and of the
+// one that it does not end
+__host__ __device__ constexpr size_t at_part_floats(int rows, int dim) { return (size_t) rows * (dim + 2); }
+
+template <typename T, int D, int WR>
+__global__ __launch_bounds__(32 * at_warps<D>, at_ctas<D>)
+void attention_split_kernel(const AtPlan S)
+{
+    const amp_attention_args& P = S.P;
+    constexpr int NW = at_warps<D>, NT = 32 * NW, WK = at_wk<D, WR>, KW = at_kw<D>, H = at_halves<D, WR>, HALF = at_half_bytes<D>;
+    constexpr int CH = D / 8, NK = KW / 8, ROWS = 16 * WR, UNIT = at_unit<D, WR>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float s_ml[WK][ROWS][2];
+    __shared__ long long s_scan[NW], s_found[2];
+
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, grp = warp / WR, wr = warp % WR, cta = blockIdx.x;
+    const int group = P.heads / P.kv_heads;
+    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
+
+    // the CTA's range of units
+    AtCursor in;
+    long long left;
+    if (S.whole)
+    {
+        in.b = 0; in.load(S);                                // (all sequences have as many tokens)
+        const int per = P.kv_heads * in.tiles;
+        in.place(S, cta / per, 0);
+        in.h = cta % per / in.tiles; in.rt = cta % in.tiles;
+        left = in.units;
+    }
+    else
+    {
+        AtCount C;
+        C.count<NT>(S, s_scan);
+        const int ctas = C.ctas(S);
+        if (cta >= ctas) return;
+        const long long u0 = cta * C.total / ctas;
+        left = (cta + 1) * C.total / ctas - u0;
+        int b;
+        long long front;
+        C.find(S, u0, b, front, s_found);
+        in.place(S, b, u0 - front);
     }
     const bool began_before = in.u > 0;
 
-    const uint32_t ring = smem_u32(smem) + warp * NST * STAGE;
-    const T* const kc = reinterpret_cast<const T*>(P.k_cache);
-    const T* const vc = reinterpret_cast<const T*>(P.v_cache);
+    const uint32_t ring = smem_u32(smem) + grp * H * HALF;
+    auto sync_group = [&]() { if constexpr (WR == 1) __syncwarp(); else asm volatile("bar.sync %0, %1;" :: "r"(1 + grp), "n"(32 * WR) : "memory"); };
 
-    // ---- loads: lane l < 16 looks up key l of the warp's sixteen, the table entry a unit ahead -----------------------------
+    // ---- loads: lane l looks up key l of the group's KW, the table entry a unit ahead; halves alternate keys, values -----------
     AtCursor ld = in;
-    long long to_load = left;
-    int pre_page = 0, pre_row = 0;
+    long long to_load = left;                                // units
+    bool values = false;
+    int pre_page = 0, pre_row = 0, fill_slot = 0;
     bool pre_live = false;
     auto look_up = [&]() {
-        const int i = ld.u * AT_UNIT + warp * 16 + (lane & 15);
+        const int i = ld.u * UNIT + grp * KW + (lane % KW);
         pre_live = i < ld.k.count();
         if (pre_live)
         {
@@ -211,42 +261,62 @@ void attention_split_kernel(const AtPlan S)
             pre_page = P.table[(long long) ld.b * P.table_row + pg];
         }
     };
-    auto issue = [&](int stage) {
+    auto issue = [&]() {
         if (to_load > 0)
         {
-            const bool bad = pre_live && (pre_page < 0 || pre_page >= P.pages);
-            const uint32_t live = __ballot_sync(0xffffffffu, pre_live) & 0xffffu, wrong = __ballot_sync(0xffffffffu, bad) & 0xffffu;
-            if (lane == 0) s_flags[warp][stage] = live | (wrong << 16);
-            const bool fetch = pre_live && !bad;
-            const long long ko = fetch ? pre_page * P.k_page + pre_row * P.k_row + ld.h * P.k_head : 0;
-            const long long vo = fetch ? pre_page * P.v_page + pre_row * P.v_row + ld.h * P.v_head : 0;
-            const uint32_t have = live & ~wrong;
-            const uint32_t at = ring + stage * STAGE;
-            constexpr int PER = 32 / CHUNKS > 0 ? 32 / CHUNKS : 1;          // rows per warp-wide copy
+            // 1: fetch, 0: behind the last key, -1: a key that cannot be found (NaN to the rows that see it; its value 0)
+            const int state = !pre_live ? 0 : (pre_page >= 0 && pre_page < P.pages ? 1 : -1);
+            const T* const base = reinterpret_cast<const T*>(values ? P.v_cache : P.k_cache);
+            const long long off = state <= 0 ? 0 : values ? pre_page * P.v_page + pre_row * P.v_row + ld.h * P.v_head
+                                                          : pre_page * P.k_page + pre_row * P.k_row + ld.h * P.k_head;
+            const uint32_t have = __ballot_sync(0xffffffffu, state > 0), lost = __ballot_sync(0xffffffffu, state < 0);
+            const uint32_t at = ring + fill_slot * HALF;
+            constexpr int PER = CH >= 32 ? 1 : 32 / CH;      // rows per warp-wide copy
             #pragma unroll
-            for (int r0 = 0; r0 < 16; r0 += PER)
+            for (int r0 = 0; r0 < KW / WR; r0 += PER)
             {
-                const int r = r0 + (CHUNKS >= 32 ? 0 : lane / CHUNKS), c = lane % CHUNKS;
-                const long long k = __shfl_sync(0xffffffffu, ko, r), v = __shfl_sync(0xffffffffu, vo, r);
-                const bool ok = (have >> r) & 1;
-                const uint32_t off = r * (2 * D) + ((c ^ (r & 7)) << 4);
-                at_copy16(at + off, kc + k + c * 8, ok);
-                at_copy16(at + STAGE / 2 + off, vc + v + c * 8, ok);
+                const int r = wr * (KW / WR) + r0 + (CH >= 32 ? 0 : lane / CH), c = lane % CH;
+                const long long o = __shfl_sync(0xffffffffu, off, r);
+                at_copy16(at + r * (2 * D) + ((c ^ (r & 7)) << 4), base + o + c * 8, (have >> r) & 1);
             }
-            if (--to_load > 0) { ld.advance(S); look_up(); }
+            if (KW == 16 ? (lost & 0xffffu) && !values : lost && !values)
+            {
+                // (behind the copies of zeros: they are waited for before the stores)
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                for (int i = lane; i < KW / WR * CH; i += 32)
+                {
+                    const int r = wr * (KW / WR) + i / CH;
+                    if ((lost >> r) & 1)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" :: "r"(at + r * (2 * D) + (i % CH) * 16), "r"(0x7fff7fffu) : "memory");
+                }
+            }
+            if (values && --to_load > 0) { ld.advance(S); look_up(); }
+            values = !values;
         }
         cp_async_commit();
+        fill_slot = fill_slot + 1 == H ? 0 : fill_slot + 1;
     };
     look_up();
-    #pragma unroll
-    for (int i = 0; i < NST; ++i) issue(i);
+    #pragma unroll 1
+    for (int i = 0; i < H; ++i) issue();
+    bool full = true;                                        // the half behind the one at hand has been requested H ahead
 
     // ---- the segments of the range -------------------------------------------------------------------------------------------
     uint32_t qf[D / 16][4];
     float o[D / 8][4], m[2], l[2];
-    int p_row[2];                                            // positions of the lane's two rows
+    int n0[2], c1[2], len[2];                                // keys that the lane's two rows see: [0, n0) and [c1, c1 + len]
+    int whole_from = 0, whole_to = 0;                        // units that all rows see whole: [from, to)
     bool fresh = true, first_segment = true;
-    int stage = 0;
+    int slot = 0;
+    // waits for the half at `slot` and refills the one in front of it
+    auto next_half = [&](bool refill) {
+        if (full) asm volatile("cp.async.wait_group %0;" :: "n"(H - 1) : "memory");
+        else asm volatile("cp.async.wait_group %0;" :: "n"(H - 2) : "memory");
+        sync_group();
+        if (!full && refill) issue();
+        else if (!full) return;
+        full = false;
+    };
     while (left > 0)
     {
         if (fresh)
@@ -254,9 +324,8 @@ void attention_split_kernel(const AtPlan S)
             #pragma unroll
             for (int i = 0; i < 2; ++i)
             {
-                const int r = in.rt * AT_ROWS + (lane >> 2) + 8 * i, tok = r / group;
+                const int r = in.rt * ROWS + wr * 16 + (lane >> 2) + 8 * i, tok = r / group, p = in.s.first + tok;
                 const bool have = tok < in.s.count;
-                p_row[i] = in.s.first + tok;
                 const T* q = reinterpret_cast<const T*>(P.q) + (long long) (in.s.row0 + tok) * P.q_token + (long long) (in.h * group + r - tok * group) * P.q_head + (lane & 3) * 2;
                 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
@@ -266,41 +335,58 @@ void attention_split_kernel(const AtPlan S)
                 }
                 m[i] = -INFINITY;
                 l[i] = 0.0f;
+                at_row_keys(P, in.k, p, n0[i], c1[i], len[i]);
             }
+            const int last = in.s.first + in.s.count - 1;
+            at_whole_keys(P, in.k, in.s.first, last, whole_from, whole_to);
             #pragma unroll
             for (int n = 0; n < D / 8; ++n) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f; }
             fresh = false;
         }
-        cp_async_wait(NST - 1);
-        __syncwarp();
-        const uint32_t flags = s_flags[warp][stage];
-        const uint32_t kb = ring + stage * STAGE, vb = kb + STAGE / 2;
-        if (flags & 0xffffu)
+        const int key0 = in.u * UNIT + grp * KW;
+        const bool some = key0 < in.k.count();
+        next_half(true);
+        const uint32_t kb = ring + slot * HALF;
+        float s[NK][4];
+        if (some)
         {
-            // s = q k^T: rows x 16 keys, two n tiles
-            float s[2][4] = {};
+            // s = q k^T: rows x KW keys
+            #pragma unroll
+            for (int n = 0; n < NK; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
             #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)
             {
-                const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * ks + ((lane >> 3) & 1);
-                uint32_t f[4];
-                at_ldsm4(kb + r * (2 * D) + ((c ^ (r & 7)) << 4), f);
-                at_mma<T>(s[0], qf[ks], f[0], f[1]);
-                at_mma<T>(s[1], qf[ks], f[2], f[3]);
+                #pragma unroll
+                for (int n = 0; n < NK; n += 2)
+                {
+                    const int r = n * 8 + (lane & 7) + ((lane >> 4) << 3), c = 2 * ks + ((lane >> 3) & 1);
+                    uint32_t f[4];
+                    at_ldsm4(kb + r * (2 * D) + ((c ^ (r & 7)) << 4), f);
+                    at_mma<T>(s[n], qf[ks], f[0], f[1]);
+                    at_mma<T>(s[n + 1], qf[ks], f[2], f[3]);
+                }
             }
+        }
+        const int key_slot = slot;
+        slot = slot + 1 == H ? 0 : slot + 1;
+        const bool ends = in.u + 1 == in.units, flush = ends || left == 1;
+        uint32_t pf[NK / 2][4];
+        if (some)
+        {
+            const bool all = key0 >= whole_from && key0 + KW <= whole_to;
             float top[2] = { m[0], m[1] };
-            const bool per_row = in.s.count > 1;
             #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NK; ++n)
             {
                 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                 {
-                    const int c = n * 8 + (lane & 3) * 2 + (e & 1);
-                    bool see = (flags >> c) & 1;
-                    if (per_row) see = see && at_sees(P, p_row[e >> 1], in.k.key(in.u * AT_UNIT + warp * 16 + c));
-                    const float x = (flags >> (16 + c)) & 1 ? NAN : s[n][e] * S.scale2;
-                    s[n][e] = see ? x : -INFINITY;
+                    s[n][e] *= S.scale2;
+                    if (!all)
+                    {
+                        const int c = key0 + n * 8 + (lane & 3) * 2 + (e & 1), i = e >> 1;
+                        if (!(c < n0[i] || (uint32_t) (c - c1[i]) <= (uint32_t) len[i])) s[n][e] = -INFINITY;
+                    }
                     top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
                 }
             }
@@ -315,7 +401,7 @@ void attention_split_kernel(const AtPlan S)
                 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                 {
-                    const float f = top[i] > m[i] ? exp2f(m[i] - top[i]) : 1.0f;
+                    const float f = top[i] > m[i] ? at_exp2(m[i] - top[i]) : 1.0f;
                     m[i] = top[i];
                     l[i] *= f;
                     #pragma unroll
@@ -324,145 +410,213 @@ void attention_split_kernel(const AtPlan S)
             }
             const float base0 = m[0] == -INFINITY ? 0.0f : m[0], base1 = m[1] == -INFINITY ? 0.0f : m[1];
             #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NK; ++n)
             {
-                s[n][0] = exp2f(s[n][0] - base0); s[n][1] = exp2f(s[n][1] - base0);
-                s[n][2] = exp2f(s[n][2] - base1); s[n][3] = exp2f(s[n][3] - base1);
+                s[n][0] = at_exp2(s[n][0] - base0); s[n][1] = at_exp2(s[n][1] - base0);
+                s[n][2] = at_exp2(s[n][2] - base1); s[n][3] = at_exp2(s[n][3] - base1);
                 l[0] += s[n][0] + s[n][1];
                 l[1] += s[n][2] + s[n][3];
-            }
-            const uint32_t pf[4] = { AtType<T>::pack(s[0][0], s[0][1]), AtType<T>::pack(s[0][2], s[0][3]),
-                                     AtType<T>::pack(s[1][0], s[1][1]), AtType<T>::pack(s[1][2], s[1][3]) };
-            #pragma unroll
-            for (int n = 0; n < D / 16; ++n)
-            {
-                const int r = lane & 15, c = 2 * n + (lane >> 4);
-                uint32_t f[4];
-                at_ldsm4_trans(vb + r * (2 * D) + ((c ^ (r & 7)) << 4), f);
-                at_mma<T>(o[2 * n], pf, f[0], f[1]);
-                at_mma<T>(o[2 * n + 1], pf, f[2], f[3]);
+                pf[n / 2][2 * (n & 1)] = AtType<T>::pack(s[n][0], s[n][1]);
+                pf[n / 2][2 * (n & 1) + 1] = AtType<T>::pack(s[n][2], s[n][3]);
             }
         }
-        __syncwarp();
-        --left;
-        const bool ends = in.u + 1 == in.units;
-        if (ends || left == 0)
+        next_half(!flush);                                   // (a flush uses both halves)
+        const uint32_t vb = ring + slot * HALF;
+        if (some)
         {
-            // the four warps' parts meet in the stage each has just read
+            #pragma unroll
+            for (int kk = 0; kk < NK / 2; ++kk)
+            {
+                #pragma unroll
+                for (int n = 0; n < D / 16; ++n)
+                {
+                    const int r = kk * 16 + (lane & 15), c = 2 * n + (lane >> 4);
+                    uint32_t f[4];
+                    at_ldsm4_trans(vb + r * (2 * D) + ((c ^ (r & 7)) << 4), f);
+                    at_mma<T>(o[2 * n], pf[kk], f[0], f[1]);
+                    at_mma<T>(o[2 * n + 1], pf[kk], f[2], f[3]);
+                }
+            }
+        }
+        --left;
+        if (flush)
+        {
+            const bool shared = !S.whole && ((first_segment && began_before) || !ends);
+            float* const part = reinterpret_cast<float*>(P.workspace) + (size_t) (2 * cta + (first_segment && began_before ? 0 : 1)) * at_part_floats(ROWS, D);
             #pragma unroll
             for (int i = 0; i < 2; ++i)
             {
                 l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
                 l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-                if ((lane & 3) == 0) { s_ml[warp][(lane >> 2) + 8 * i][0] = m[i]; s_ml[warp][(lane >> 2) + 8 * i][1] = l[i]; }
+                if ((lane & 3) == 0) { s_ml[grp][wr * 16 + (lane >> 2) + 8 * i][0] = m[i]; s_ml[grp][wr * 16 + (lane >> 2) + 8 * i][1] = l[i]; }
             }
             __syncthreads();
+            float f[2];
             #pragma unroll
             for (int i = 0; i < 2; ++i)
             {
-                const int r = (lane >> 2) + 8 * i;
-                const float top = fmaxf(fmaxf(s_ml[0][r][0], s_ml[1][r][0]), fmaxf(s_ml[2][r][0], s_ml[3][r][0]));
-                const float f = m[i] == -INFINITY ? 0.0f : exp2f(m[i] - top);
+                float top = s_ml[0][wr * 16 + (lane >> 2) + 8 * i][0];
                 #pragma unroll
-                for (int n = 0; n < D / 8; ++n)
-                {
-                    const int col = (n * 8 + (lane & 3) * 2) ^ ((r & 3) << 3);
-                    asm volatile("st.shared.v2.f32 [%0], {%1, %2};" :: "r"(kb + (r * D + col) * 4), "f"(o[n][2 * i] * f), "f"(o[n][2 * i + 1] * f) : "memory");
-                }
+                for (int g = 1; g < WK; ++g) top = fmaxf(top, s_ml[g][wr * 16 + (lane >> 2) + 8 * i][0]);
+                f[i] = m[i] == -INFINITY ? 0.0f : at_exp2(m[i] - top);
             }
-            __syncthreads();
-            const bool shared = !S.whole && ((first_segment && began_before) || !ends);
-            const int slot = 2 * cta + (first_segment && began_before ? 0 : 1);
-            float* const part = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(P.workspace) + at_desc_bytes(S.grid)) + slot * at_part_floats(D);
-            for (int i = t; i < AT_ROWS * D / 4; i += 128)
+            // the groups' parts meet in the two half stages that each has just read, D / WR columns at a time: the
+            // columns of a row are turned round by 8 for every row (mod 4), so that eight rows meet all banks
+            constexpr int COLS = D / WR, PIECE = 16 * COLS * 4, TURN = COLS >= 32 ? 3 : COLS / 8 - 1;
+            auto place = [&](int g, int w, int r, int c) {   // byte offset in the group's ring
+                const int at = w * PIECE + (r * COLS + (c ^ ((r & TURN) << 3))) * 4;
+                return g * H * HALF + (at < HALF ? key_slot * HALF + at : slot * HALF + at - HALF);
+            };
+            #pragma unroll
+            for (int pass = 0; pass < WR; ++pass)
             {
-                const int r = i / (D / 4), c = (i % (D / 4)) * 4;
-                const int row = in.rt * AT_ROWS + r, tok = row / group;
-                if (tok >= in.s.count) break;                // (rows ascend with i)
-                float top = -INFINITY, sum = 0.0f;
                 #pragma unroll
-                for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ml[w][r][0]);
-                #pragma unroll
-                for (int w = 0; w < 4; ++w) sum += s_ml[w][r][0] == -INFINITY ? s_ml[w][r][1] : s_ml[w][r][1] * exp2f(s_ml[w][r][0] - top);
-                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                #pragma unroll
-                for (int w = 0; w < 4; ++w)
+                for (int i = 0; i < 2; ++i)
                 {
-                    const float4 y = *reinterpret_cast<const float4*>(smem + (w * NST + stage) * STAGE + (r * D + (c ^ ((r & 3) << 3))) * 4);
-                    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+                    const int r = (lane >> 2) + 8 * i;
+                    #pragma unroll
+                    for (int n = 0; n < COLS / 8; ++n)
+                        *reinterpret_cast<float2*>(smem + place(grp, wr, r, n * 8 + (lane & 3) * 2)) =
+                            make_float2(o[pass * (COLS / 8) + n][2 * i] * f[i], o[pass * (COLS / 8) + n][2 * i + 1] * f[i]);
                 }
-                if (shared)
+                __syncthreads();
+                for (int i = t; i < ROWS * COLS / 4; i += NT)
                 {
-                    *reinterpret_cast<float4*>(part + r * D + c) = x;
-                    if (c == 0) *reinterpret_cast<float2*>(part + AT_ROWS * D + 2 * r) = make_float2(top, sum);
+                    const int r = i / (COLS / 4), c = (i % (COLS / 4)) * 4;
+                    const int row = in.rt * ROWS + r, tok = row / group;
+                    if (tok >= in.s.count) break;            // (rows ascend with i)
+                    float top = s_ml[0][r][0], sum = 0.0f;
+                    #pragma unroll
+                    for (int g = 1; g < WK; ++g) top = fmaxf(top, s_ml[g][r][0]);
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    #pragma unroll
+                    for (int g = 0; g < WK; ++g)
+                    {
+                        sum += s_ml[g][r][0] == -INFINITY ? s_ml[g][r][1] : s_ml[g][r][1] * at_exp2(s_ml[g][r][0] - top);      // (an l of NaN stays one)
+                        const float4 y = *reinterpret_cast<const float4*>(smem + place(g, r >> 4, r & 15, c));
+                        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+                    }
+                    const int col = pass * COLS + c;
+                    if (shared)
+                    {
+                        *reinterpret_cast<float4*>(part + r * D + col) = x;
+                        if (col == 0) *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(top, sum);
+                    }
+                    else
+                        at_store<T>(P, in.s, tok, in.h * group + row - tok * group, col, x, top, sum);
                 }
-                else
-                    at_store<T>(P, in.s, tok, in.h * group + row - tok * group, c, x, top, sum);
+                __syncthreads();
             }
-            __syncthreads();
             fresh = true;
             first_segment = false;
+            issue();                                         // both halves
+            issue();
+            full = true;
         }
-        issue(stage);
-        stage = stage + 1 == NST ? 0 : stage + 1;
+        slot = slot + 1 == H ? 0 : slot + 1;
         if (left > 0) in.advance(S);
     }
 }
 
-// One CTA per CTA of the split form (x) and row of a row tile (y): joins the parts of the segment whose second part that CTA holds
+// Joins the parts of a segment, one row of it (blockIdx.y) per CTA: of segment blockIdx.x, or of the one that the range of CTA
+// blockIdx.x is the second to hold. Which parts those are is found while the split kernel's last CTAs still run.
 template <typename T, int D>
 __global__ __launch_bounds__(128)
 void attention_join_kernel(const AtPlan S)
 {
     const amp_attention_args& P = S.P;
-    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
     __shared__ float s_red[4], s_sum[4];
     __shared__ float4 s_o[4][D / 4];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, cta = blockIdx.x + 1, r = blockIdx.y;
-    const int* desc = reinterpret_cast<const int*>(P.workspace) + (size_t) cta * AT_DESC;
-    const int4 d = *reinterpret_cast<const int4*>(desc);
-    if (d.x < 0 || d.w != cta - 1) return;
-    const int last = desc[4], group = P.heads / P.kv_heads;
-    const AtSeq s = at_seq(P, d.x);
-    const int row = d.z * AT_ROWS + r, tok = row / group;
-    if (tok >= s.count) return;
-    const float* const parts = reinterpret_cast<const float*>(reinterpret_cast<const unsigned char*>(P.workspace) + at_desc_bytes(S.grid));
-    // part i of the segment: the first is the end of its CTA's range, the others are the beginning of theirs
-    const int n = last - d.w + 1;
-    auto part = [&](int i) { return parts + (size_t) (2 * (d.w + i) + (i ? 0 : 1)) * at_part_floats(D); };
+    __shared__ long long s_scan[4], s_found[2];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, r = blockIdx.y, group = P.heads / P.kv_heads;
+    AtCount C;
+    C.count<128>(S, s_scan);
+    const int ctas = C.ctas(S);
+    AtCursor in;
+    long long g0;                                            // first unit of the segment
+    int first, last;                                         // CTAs that hold it
+    bool join = false;
+    if (S.by_segment)
+    {
+        in.b = 0; in.load(S);                                // (all sequences have as many tokens)
+        const int per = P.kv_heads * in.tiles, b = blockIdx.x / per;
+        in.b = b; in.h = blockIdx.x % per / in.tiles; in.rt = blockIdx.x % in.tiles;
+        in.load(S);
+        g0 = C.front_of(S, b, s_found) + ((long long) in.h * in.tiles + in.rt) * in.units;
+        join = true;
+    }
+    else if ((int) blockIdx.x < ctas)
+    {
+        const long long u0 = blockIdx.x * C.total / ctas;
+        int b;
+        long long front;
+        C.find(S, u0, b, front, s_found);
+        in.place(S, b, u0 - front);
+        g0 = u0 - in.u;
+        join = in.u > 0;
+    }
+    if (join)
+    {
+        first = (int) (((g0 + 1) * ctas - 1) / C.total);
+        last = (int) (((g0 + in.units) * ctas - 1) / C.total);
+        join = first < last && (S.by_segment || first == (int) blockIdx.x - 1);
+    }
+    const int row = join ? in.rt * S.rows + r : 0, tok = row / group;
+    if (S.pdl) pdl_wait();
+    if (S.pdl) pdl_launch_dependents();
+    if (!join || tok >= in.s.count) return;
 
+    // part i of the segment: the first is the end of its CTA's range, the others are the beginning of theirs
+    const size_t size = at_part_floats(S.rows, D);
+    const float* const parts = reinterpret_cast<const float*>(P.workspace);
+    const int n = last - first + 1;
+    auto part = [&](int i) { return parts + (size_t) (2 * (first + i) + (i ? 0 : 1)) * size; };
     float m = -INFINITY;
-    for (int i = t; i < n; i += 128) m = fmaxf(m, part(i)[AT_ROWS * D + 2 * r]);
+    for (int i = t; i < n; i += 128) m = fmaxf(m, part(i)[(size_t) S.rows * D + 2 * r]);
+    // a warp adds every fourth part up, a lane D / 32 values of the row (in pieces of four); the first parts are on their way while m is found
+    constexpr int PIECES = D / 4, EACH = (PIECES + 31) / 32, AHEAD = D == 256 ? 4 : 8;
+    float4 x[AHEAD][EACH];
+    float2 ml[AHEAD];
+    auto fetch = [&](int i0) {
+        #pragma unroll
+        for (int a = 0; a < AHEAD; ++a)
+        {
+            const int i = i0 + 4 * a;
+            ml[a] = make_float2(-INFINITY, 0.0f);
+            if (i >= n) continue;
+            const float* p = part(i);
+            ml[a] = *reinterpret_cast<const float2*>(p + (size_t) S.rows * D + 2 * r);
+            #pragma unroll
+            for (int e = 0; e < EACH; ++e)
+                if (PIECES % 32 == 0 || lane + 32 * e < PIECES) x[a][e] = reinterpret_cast<const float4*>(p + r * D)[lane + 32 * e];
+        }
+    };
+    fetch(warp);
     #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) s_red[warp] = m;
     __syncthreads();
     m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
     const float base = m == -INFINITY ? 0.0f : m;
-
-    // a warp adds every fourth part up, a lane D / 32 values of the row (in pieces of four)
-    constexpr int PIECES = D / 4, EACH = (PIECES + 31) / 32;
     float4 acc[EACH];
     #pragma unroll
     for (int e = 0; e < EACH; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float l = 0.0f;
-    #pragma unroll 4
-    for (int i = warp; i < n; i += 4)
+    for (int i0 = warp; i0 < n; i0 += 4 * AHEAD)
     {
-        const float* p = part(i);
-        const float2 ml = *reinterpret_cast<const float2*>(p + AT_ROWS * D + 2 * r);
-        const float f = exp2f(ml.x - base);
-        l += ml.x == -INFINITY ? ml.y : ml.y * f;            // (an l of NaN stays one)
         #pragma unroll
-        for (int e = 0; e < EACH; ++e)
+        for (int a = 0; a < AHEAD; ++a)
         {
-            const int c = lane + 32 * e;
-            if (PIECES % 32 == 0 || c < PIECES)
+            if (i0 + 4 * a >= n) continue;
+            const float f = at_exp2(ml[a].x - base);
+            l += ml[a].x == -INFINITY ? ml[a].y : ml[a].y * f;
+            #pragma unroll
+            for (int e = 0; e < EACH; ++e)
             {
-                const float4 x = reinterpret_cast<const float4*>(p + r * D)[c];
-                acc[e].x += x.x * f; acc[e].y += x.y * f; acc[e].z += x.z * f; acc[e].w += x.w * f;
+                acc[e].x += x[a][e].x * f; acc[e].y += x[a][e].y * f; acc[e].z += x[a][e].z * f; acc[e].w += x[a][e].w * f;
             }
         }
+        if (i0 + 4 * AHEAD < n) fetch(i0 + 4 * AHEAD);
     }
     if (lane == 0) s_sum[warp] = l;
     #pragma unroll
@@ -471,10 +625,10 @@ void attention_join_kernel(const AtPlan S)
     l = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
     for (int c = t; c < PIECES; c += 128)
     {
-        float4 x = s_o[0][c];
+        float4 y = s_o[0][c];
         #pragma unroll
-        for (int w = 1; w < 4; ++w) { const float4 y = s_o[w][c]; x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w; }
-        at_store<T>(P, s, tok, d.y * group + row - tok * group, c * 4, x, m, l);
+        for (int w = 1; w < 4; ++w) { const float4 z = s_o[w][c]; y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w; }
+        at_store<T>(P, in.s, tok, in.h * group + row - tok * group, c * 4, y, m, l);
     }
 }
 
@@ -498,7 +652,7 @@ static const AtDevice* at_device(int* rc)
 // Sequences that fit into this many keys are not split: nothing is joined then
 constexpr int AT_WHOLE_KEYS = 256;
 // Rows (tokens x group) up to which a sequence takes the split form; beyond, the prompt form
-constexpr int AT_SPLIT_ROWS = 32;
+constexpr int AT_SPLIT_ROWS = 64;
 
 static int at_grid(int dim, int sms) { return sms * (dim == 64 ? at_ctas<64> : dim == 128 ? at_ctas<128> : at_ctas<256>); }
 
@@ -506,7 +660,7 @@ static int at_grid(int dim, int sms) { return sms * (dim == 64 ? at_ctas<64> : d
 struct AtCut
 {
     bool split, tc;                            // forms that are launched
-    int whole, grid;                           // split form
+    int whole, grid, wr;                       // split form: 16 * wr rows per row tile
     int tiles, slices;                         // prompt form
     size_t tc_offset, bytes;                   // of the workspace
 };
@@ -533,45 +687,64 @@ static AtCut at_cut(int tokens, int seqs, int heads, int kv_heads, int dim, bool
     C.tc = ragged ? all > AT_SPLIT_ROWS : !C.split;
     C.whole = C.split && !ragged && max_keys <= AT_WHOLE_KEYS;
     C.grid = at_grid(dim, sms);
-    if (C.split && !C.whole) C.bytes = (at_desc_bytes(C.grid) + 2 * C.grid * at_part_floats(dim) * 4 + 127) / 128 * 128;
+    const long rows = ragged ? group : each;   // (ragged: single tokens are the rule)
+    C.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    if (C.split && !C.whole) C.bytes = (2 * C.grid * at_part_floats(16 * C.wr, dim) * 4 + 127) / 128 * 128;
     C.tc_offset = C.bytes;
     C.slices = 1;
     if (C.tc)
     {
-        const int rows = ta_rows(dim), kb = dim <= 128 ? 128 : 64;
-        C.tiles = (int) (ragged ? all / rows + min((long) seqs, all / (AT_SPLIT_ROWS + 1)) : seqs * ((each + rows - 1) / rows));
-        const long keys = window ? min(max_keys, (long) window + sinks + rows / group + 1) : max_keys;
+        const int tile = ta_rows(dim), kb = dim <= 128 ? 128 : 64;
+        C.tiles = (int) (ragged ? all / tile + min((long) seqs, all / (AT_SPLIT_ROWS + 1)) : seqs * ((each + tile - 1) / tile));
+        const long keys = window ? min(max_keys, (long) window + sinks + tile / group + 1) : max_keys;
         C.slices = ta_slices((long) C.tiles * kv_heads, (keys + kb - 1) / kb, sms);
         if (C.slices > 1) C.bytes += (size_t) C.tiles * kv_heads * C.slices * ta_part_floats(dim) * 4;
     }
     return C;
 }
 
-template <typename T, int D>
+template <typename T, int D, int WR>
 static int at_launch(AtPlan& S, cudaStream_t stream)
 {
     const amp_attention_args& P = S.P;
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return cuda_rc(e, "attention device");
-    if (cudaError_t e = ensure_smem(attention_split_kernel<T, D>, at_smem<D>, dev)) return cuda_rc(e, "attention shared memory");
-    const int group = P.heads / P.kv_heads;
-    int grid = S.grid;
-    if (S.whole) grid = P.seqs * P.kv_heads * ((P.tokens / P.seqs * group + AT_ROWS - 1) / AT_ROWS);
+    if (cudaError_t e = ensure_smem(attention_split_kernel<T, D, WR>, at_smem<D>, dev)) return cuda_rc(e, "attention shared memory");
+    S.unit = at_unit<D, WR>;
+    S.rows = 16 * WR;
+    // (segments of the call, where the host knows them)
+    const long rows = (long) (P.tokens / P.seqs) * (P.heads / P.kv_heads), segments = (long) P.seqs * P.kv_heads * ((rows + S.rows - 1) / S.rows);
+    const long grid = S.whole ? segments : S.grid;
+    AMP_REQUIRE(grid < (1l << 31), "attention: too many sequences");
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid, 1, 1);
-    cfg.blockDim = dim3(128, 1, 1);
+    cfg.gridDim = dim3((unsigned) grid, 1, 1);
+    cfg.blockDim = dim3(32 * at_warps<D>, 1, 1);
     cfg.dynamicSmemBytes = at_smem<D>;
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = S.pdl ? 1 : 0;
-    if (cudaError_t e = cudaLaunchKernelEx(&cfg, attention_split_kernel<T, D>, (const AtPlan) S)) return cuda_rc(e, "attention launch");
-    if (S.whole || grid < 2) return 0;
-    cfg.gridDim = dim3(grid - 1, P.cu ? AT_ROWS : min(AT_ROWS, P.tokens / P.seqs * group), 1);
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, attention_split_kernel<T, D, WR>, (const AtPlan) S)) return cuda_rc(e, "attention launch");
+    if (S.whole) return 0;
+    S.by_segment = !P.cu && segments < S.grid;
+    cfg.gridDim = dim3(S.by_segment ? (unsigned) segments : S.grid, P.cu ? S.rows : (int) min((long) S.rows, rows), 1);
+    cfg.blockDim = dim3(128, 1, 1);
     cfg.dynamicSmemBytes = 0;
     return cuda_rc(cudaLaunchKernelEx(&cfg, attention_join_kernel<T, D>, (const AtPlan) S), "attention join launch");
+}
+
+template <typename T, int D>
+static int at_launch_rows(AtPlan& S, int wr, cudaStream_t stream)
+{
+    return wr == 1 ? at_launch<T, D, 1>(S, stream) : wr == 2 ? at_launch<T, D, 2>(S, stream) : at_launch<T, D, 4>(S, stream);
+}
+
+template <typename T>
+static int at_launch_dim(AtPlan& S, int wr, cudaStream_t stream)
+{
+    return S.P.dim == 64 ? at_launch_rows<T, 64>(S, wr, stream) : S.P.dim == 128 ? at_launch_rows<T, 128>(S, wr, stream) : at_launch_rows<T, 256>(S, wr, stream);
 }
 
 }  // namespace amp
@@ -618,10 +791,7 @@ AMP_API int amp_b200_attention(const amp_attention_args* args, cudaStream_t stre
     {
         S.grid = C.grid; S.whole = C.whole; S.pdl = g_pdl; S.split_rows = P.cu ? AT_SPLIT_ROWS : 1 << 30;
         S.scale2 = P.scale * 1.4426950408889634f;
-        if (P.bf16)
-            rc = P.dim == 64 ? at_launch<__nv_bfloat16, 64>(S, stream) : P.dim == 128 ? at_launch<__nv_bfloat16, 128>(S, stream) : at_launch<__nv_bfloat16, 256>(S, stream);
-        else
-            rc = P.dim == 64 ? at_launch<__half, 64>(S, stream) : P.dim == 128 ? at_launch<__half, 128>(S, stream) : at_launch<__half, 256>(S, stream);
+        rc = P.bf16 ? at_launch_dim<__nv_bfloat16>(S, C.wr, stream) : at_launch_dim<__half>(S, C.wr, stream);
         if (rc) return rc;
     }
     if (!C.tc) return 0;

@@ -58,10 +58,27 @@ __device__ __forceinline__ AtKeys at_keys(const amp_attention_args& P, int first
     return k;
 }
 
-// Does the token at p see key j?
-__device__ __forceinline__ bool at_sees(const amp_attention_args& P, int p, int j)
+// Of the keys counted through, the ones that the token at p sees: [0, n0) and [c1, c1 + len] (c1 out of reach: none)
+__device__ __forceinline__ void at_row_keys(const amp_attention_args& P, const AtKeys& k, int p, int& n0, int& c1, int& len)
 {
-    return j <= p && (!P.window || j > p - P.window || j < P.sinks);
+    n0 = P.window ? min(p + 1, P.sinks) : 0;
+    c1 = P.window ? max(p - P.window + 1, k.lo) - k.lo + k.a : 0;
+    len = p - k.lo + k.a - c1;
+    if (len < 0) { c1 = 1 << 30; len = 0; }
+}
+
+// ... and a run of them, [from, to), that every token from p0 to p1 sees
+__device__ __forceinline__ void at_whole_keys(const amp_attention_args& P, const AtKeys& k, int p0, int p1, int& from, int& to)
+{
+    to = min(k.count(), p0 - k.lo + k.a + 1);
+    from = P.window ? k.a + max(0, p1 - P.window + 1 - k.lo) : 0;
+}
+
+__device__ __forceinline__ float at_exp2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 template <typename T> struct AtType;

@@ -111,22 +111,6 @@ __device__ __forceinline__ void ta_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void ta_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void ta_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ float ta_exp2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Of row tile `tile` (NQ * 128 rows) of sequence s: tokens [tok0, tok1]
-template <int NQ>
-struct TaTile
-{
-    int b, tile, tok0, tok1;
-    AtSeq s;
-    AtKeys k;
-};
-
 // Sequence and row tile of the x-th tile of the call; false: there is none. By one warp.
 template <int NQ>
 __device__ __forceinline__ bool ta_find(const TaPlan& S, int x, int& b, int& tile)
@@ -258,19 +242,10 @@ void attention_tc_kernel(const TaPlan S)
             ta_fence_async();
             ta_arrive(smem_u32(&q_full));
         }
-        // keys of the compact list that the row sees: [0, n0) and [c1, c1 + len]
-        int n0 = 0, c1 = 0, c2 = p;
-        if (P.window)
-        {
-            n0 = min(p + 1, P.sinks);
-            c1 = max(p - P.window + 1, keys.lo) - keys.lo + keys.a;
-            c2 = p - keys.lo + keys.a;
-        }
-        if (!have) { n0 = 0; c2 = -1; }
-        const uint32_t len = c2 >= c1 ? (uint32_t) (c2 - c1) : 0u;
-        if (c2 < c1) c1 = 1 << 30;
-        // the same for the row tile's first and last token: tiles that all its rows see whole need no look at single keys
-        const int ta = seq.first + (row0 + 128 * i) / group, tb = seq.first + min((row0 + 128 * i + 127) / group, seq.count - 1);
+        // what its row sees of the keys, and a run of them that all rows of the row tile see: there no single key is looked at
+        int n0, c1, len, from, to;
+        at_row_keys(P, keys, p, n0, c1, len);
+        at_whole_keys(P, keys, seq.first + (row0 + 128 * i) / group, seq.first + min((row0 + 128 * i + 127) / group, seq.count - 1), from, to);
 
         const float sc = P.scale == 0.0f ? 1.0f : fabsf(S.scale2);
         const uint32_t lane_base = tmem + ((uint32_t) (32 * (warp & 3)) << 16);
@@ -288,15 +263,14 @@ void attention_tc_kernel(const TaPlan S)
             #pragma unroll
             for (int c = 0; c < KB; c += 32) ta_ld32(s_t + c, s + c);
             ta_wait_ld();
-            const int k0 = (j0 + j) * KB, kl = k0 + KB - 1;
-            const bool whole = kl < keys.count() && keys.key(kl) <= ta && (!P.window || keys.key(k0) > tb - P.window || keys.key(kl) < P.sinks);
-            if (!whole)
+            const int k0 = (j0 + j) * KB;
+            if (k0 < from || k0 + KB > to)
             {
                 #pragma unroll
                 for (int c = 0; c < KB; ++c)
                 {
                     const int at = k0 + c;
-                    const bool see = at < n0 || (uint32_t) (at - c1) <= len;
+                    const bool see = at < n0 || (uint32_t) (at - c1) <= (uint32_t) len;
                     s[c] = see ? s[c] : 0xff800000u;
                 }
             }
@@ -311,7 +285,7 @@ void attention_tc_kernel(const TaPlan S)
             const bool move = top > m && (m == -INFINITY || (top - m) * sc > TA_SLACK);
             if (__any_sync(0xffffffffu, move))
             {
-                const float f = move ? ta_exp2((m - top) * sc) : 1.0f;       // (m of -inf: 0)
+                const float f = move ? at_exp2((m - top) * sc) : 1.0f;       // (m of -inf: 0)
                 if (move) m = top;
                 l2 = mul_f32x2(l2, pack_f32x2(f, f));
                 if (j > 0)
@@ -339,7 +313,7 @@ void attention_tc_kernel(const TaPlan S)
                 for (int e = 0; e < 64; e += 2)
                 {
                     const float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[c + e]), __uint_as_float(s[c + e + 1])), sc2, base2));
-                    const float e0 = ta_exp2(y.x), e1 = ta_exp2(y.y);
+                    const float e0 = at_exp2(y.x), e1 = at_exp2(y.y);
                     l2 = add_f32x2(l2, pack_f32x2(e0, e1));
                     w[e / 2] = AtType<T>::pack(e0, e1);
                 }
@@ -577,7 +551,7 @@ void attention_tc_join_kernel(const TaPlan S)
     {
         const float2 v = ml(i);
         if (v.y == 0.0f) continue;             // (a slice without keys wrote nothing else)
-        const float f = ta_exp2(v.x - base);
+        const float f = at_exp2(v.x - base);
         l += v.y != v.y ? v.y : v.y * f;
         const float4* p = reinterpret_cast<const float4*>(parts + i * ta_part_floats(D)) + (size_t) blockIdx.y * 4 * ROWS + t;
         #pragma unroll
