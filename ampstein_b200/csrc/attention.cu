@@ -16,10 +16,10 @@
 
 namespace amp {
 
-constexpr int AT_MAX_PER_THREAD = 32;          // sequences counted by one warp; above, the block counts
+constexpr int AT_WARP_SEQS = 32;               // sequences that a warp counts by itself
 
 template <int D> constexpr int at_warps = D == 256 ? 8 : 4;
-template <int D> constexpr int at_kw = D == 64 ? 32 : 16;      // keys of a group's step
+template <int D> constexpr int at_kw = D == 256 ? 16 : 32;     // keys of a group's step
 template <int D> constexpr int at_ctas = D == 64 ? 3 : (D == 128 ? 2 : 1);     // per SM
 template <int D> constexpr int at_half_bytes = at_kw<D> * D * 2;
 template <int D> constexpr int at_smem = (D == 64 ? 64 : D == 128 ? 96 : 192) * 1024;
@@ -37,6 +37,7 @@ struct AtPlan
     int by_segment;                            // join: blockIdx.x is a segment, else the CTA whose range begins inside it
     int pdl;
     float scale2;                              // scale * log2(e)
+    AtPages g;
 };
 
 __device__ __forceinline__ void at_ldsm4(uint32_t addr, uint32_t (&r)[4])
@@ -86,13 +87,14 @@ struct AtCursor
         units = at_units(S, k);
     }
     // the at-th unit of sequence b
-    __device__ __forceinline__ void place(const AtPlan& S, int seq, long long at)
+    __device__ __forceinline__ void place(const AtPlan& S, int seq, int at)
     {
         b = seq;
         load(S);
-        h = (int) (at / ((long long) tiles * units));
-        rt = (int) (at / units - (long long) h * tiles);
-        u = (int) (at % units);
+        const int row_tile = at / units;
+        u = at - row_tile * units;
+        h = row_tile / tiles;
+        rt = row_tile - h * tiles;
     }
     // to the next unit; the caller knows that there is one
     __device__ __forceinline__ void advance(const AtPlan& S)
@@ -107,94 +109,99 @@ struct AtCursor
     }
 };
 
-// Units of the sequences, counted. Up to 32 sequences every warp does it by itself, one per lane; beyond, the block, a run per thread.
-// (all threads of the block call it)
+// Units of the sequences, counted (there are fewer than 2^31, the host sees to it). Up to 32 sequences every warp does it by itself,
+// one per lane; beyond, the block, a run per thread. All threads of the block call these.
 struct AtCount
 {
     int b0, b1;                                // this lane's, or thread's, sequences
-    long long before, mine, total;             // units in front of them, of them, of all
+    int before, mine, total;                   // units in front of them, of them, of all
     bool warp;                                 // counted by the warp
+    int ctas, each, more;                      // CTAs with units: the first `more` have each + 1, the others each
+
+    static __device__ __forceinline__ int units_of(const AtPlan& S, int b)
+    {
+        const AtSeq s = at_seq(S.P, b);
+        return S.P.kv_heads * at_row_tiles(S, s) * at_units(S, at_keys(S.P, s.first, s.count));
+    }
 
     template <int NT>
-    __device__ __forceinline__ void count(const AtPlan& S, long long* s_scan)
+    __device__ __forceinline__ void count(const AtPlan& S, int* s_scan)
     {
         const int t = threadIdx.x, lane = t & 31;
-        warp = S.P.seqs <= AT_MAX_PER_THREAD;
+        warp = S.P.seqs <= AT_WARP_SEQS;
         const int run = warp ? 1 : (S.P.seqs + NT - 1) / NT;
         b0 = min(S.P.seqs, (warp ? lane : t) * run);
         b1 = min(S.P.seqs, b0 + run);
         mine = 0;
-        for (int b = b0; b < b1; ++b)
-        {
-            const AtSeq s = at_seq(S.P, b);
-            mine += (long long) S.P.kv_heads * at_row_tiles(S, s) * at_units(S, at_keys(S.P, s.first, s.count));
-        }
-        long long sum = mine;
+        for (int b = b0; b < b1; ++b) mine += units_of(S, b);
+        int sum = mine;
         #pragma unroll
         for (int o = 1; o < 32; o <<= 1)
         {
-            const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += x;
         }
-        if (warp)
-        {
-            total = __shfl_sync(0xffffffffu, sum, 31);
-            before = sum - mine;
-            return;
-        }
-        if (lane == 31) s_scan[t >> 5] = sum;
-        __syncthreads();
-        total = 0;
         before = sum - mine;
-        for (int w = 0; w < NT / 32; ++w) { if (w == t >> 5) before += total; total += s_scan[w]; }
+        if (warp) total = __shfl_sync(0xffffffffu, sum, 31);
+        else
+        {
+            if (lane == 31) s_scan[t >> 5] = sum;
+            __syncthreads();
+            total = 0;
+            for (int w = 0; w < NT / 32; ++w) { if (w == t >> 5) before += total; total += s_scan[w]; }
+        }
+        ctas = min(S.grid, total);
+        each = ctas ? total / ctas : 0;
+        more = total - each * ctas;
     }
 
-    // sequence of unit u, and the units in front of the sequence. (u < total)
-    __device__ __forceinline__ void find(const AtPlan& S, long long u, int& b, long long& front, long long* s_found) const
+    __device__ __forceinline__ int begin(int cta) const { return cta * each + min(cta, more); }
+
+    // the CTA that has unit u
+    __device__ __forceinline__ int cta_of(int u) const
+    {
+        const int low = more * (each + 1);
+        return u < low ? u / (each + 1) : more + (u - low) / each;
+    }
+
+    // sequence of unit u (u < total), and the units in front of the sequence
+    __device__ __forceinline__ void find(const AtPlan& S, int u, int& b, int& front, int* s_found) const
     {
         const bool here = u >= before && u < before + mine;
         if (warp)
         {
-            const int l = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-            b = l;
-            front = __shfl_sync(0xffffffffu, before, l);
+            b = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+            front = __shfl_sync(0xffffffffu, before, b);
             return;
         }
         if (here)
         {
-            long long at = before;
+            int at = before;
             for (int i = b0; i < b1; ++i)
             {
-                const AtSeq s = at_seq(S.P, i);
-                const long long n = (long long) S.P.kv_heads * at_row_tiles(S, s) * at_units(S, at_keys(S.P, s.first, s.count));
+                const int n = units_of(S, i);
                 if (u < at + n) { s_found[0] = i; s_found[1] = at; break; }
                 at += n;
             }
         }
         __syncthreads();
-        b = (int) s_found[0];
+        b = s_found[0];
         front = s_found[1];
     }
 
     // units in front of sequence b
-    __device__ __forceinline__ long long front_of(const AtPlan& S, int b, long long* s_found) const
+    __device__ __forceinline__ int front_of(const AtPlan& S, int b, int* s_found) const
     {
         if (warp) return __shfl_sync(0xffffffffu, before, b);
         if (b >= b0 && b < b1)
         {
-            long long at = before;
-            for (int i = b0; i < b; ++i)
-            {
-                const AtSeq s = at_seq(S.P, i);
-                at += (long long) S.P.kv_heads * at_row_tiles(S, s) * at_units(S, at_keys(S.P, s.first, s.count));
-            }
+            int at = before;
+            for (int i = b0; i < b; ++i) at += units_of(S, i);
             s_found[0] = at;
         }
         __syncthreads();
         return s_found[0];
     }
-
-    __device__ __forceinline__ int ctas(const AtPlan& S) const { return (int) min((long long) S.grid, total); }
 };
 
 // Workspace: two parts per CTA (o of the row tile, then m and l of its rows): of the segment that began before the CTA, and of the
@@ -210,7 +217,7 @@ void attention_split_kernel(const AtPlan S)
     constexpr int CH = D / 8, NK = KW / 8, ROWS = 16 * WR, UNIT = at_unit<D, WR>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_ml[WK][ROWS][2];
-    __shared__ long long s_scan[NW], s_found[2];
+    __shared__ int s_scan[NW], s_found[2];
 
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, grp = warp / WR, wr = warp % WR, cta = blockIdx.x;
     const int group = P.heads / P.kv_heads;
@@ -218,7 +225,7 @@ void attention_split_kernel(const AtPlan S)
 
     // the CTA's range of units
     AtCursor in;
-    long long left;
+    int left;
     if (S.whole)
     {
         in.b = 0; in.load(S);                                // (all sequences have as many tokens)
@@ -231,12 +238,10 @@ void attention_split_kernel(const AtPlan S)
     {
         AtCount C;
         C.count<NT>(S, s_scan);
-        const int ctas = C.ctas(S);
-        if (cta >= ctas) return;
-        const long long u0 = cta * C.total / ctas;
-        left = (cta + 1) * C.total / ctas - u0;
-        int b;
-        long long front;
+        if (cta >= C.ctas) return;
+        const int u0 = C.begin(cta);
+        left = C.begin(cta + 1) - u0;
+        int b, front;
         C.find(S, u0, b, front, s_found);
         in.place(S, b, u0 - front);
     }
@@ -247,16 +252,17 @@ void attention_split_kernel(const AtPlan S)
 
     // ---- loads: lane l looks up key l of the group's KW, the table entry a unit ahead; halves alternate keys, values -----------
     AtCursor ld = in;
-    long long to_load = left;                                // units
-    bool values = false;
+    int to_load = left;                                      // units
+    bool values = false, pre_live = false;
     int pre_page = 0, pre_row = 0, fill_slot = 0;
-    bool pre_live = false;
+    const unsigned char* const k_lane = reinterpret_cast<const unsigned char*>(P.k_cache) + lane % CH * 16;
+    const unsigned char* const v_lane = reinterpret_cast<const unsigned char*>(P.v_cache) + lane % CH * 16;
     auto look_up = [&]() {
         const int i = ld.u * UNIT + grp * KW + (lane % KW);
         pre_live = i < ld.k.count();
         if (pre_live)
         {
-            const int j = ld.k.key(i), pg = j / P.page_size;
+            const int j = ld.k.key(i), pg = S.g.page_of(j);
             pre_row = j - pg * P.page_size;
             pre_page = P.table[(long long) ld.b * P.table_row + pg];
         }
@@ -264,30 +270,43 @@ void attention_split_kernel(const AtPlan S)
     auto issue = [&]() {
         if (to_load > 0)
         {
-            // 1: fetch, 0: behind the last key, -1: a key that cannot be found (NaN to the rows that see it; its value 0)
-            const int state = !pre_live ? 0 : (pre_page >= 0 && pre_page < P.pages ? 1 : -1);
-            const T* const base = reinterpret_cast<const T*>(values ? P.v_cache : P.k_cache);
-            const long long off = state <= 0 ? 0 : values ? pre_page * P.v_page + pre_row * P.v_row + ld.h * P.v_head
-                                                          : pre_page * P.k_page + pre_row * P.k_row + ld.h * P.k_head;
-            const uint32_t have = __ballot_sync(0xffffffffu, state > 0), lost = __ballot_sync(0xffffffffu, state < 0);
-            const uint32_t at = ring + fill_slot * HALF;
+            const bool found = (unsigned) pre_page < (unsigned) P.pages;
+            const uint32_t off = values ? pre_page * S.g.v_page + pre_row * S.g.v_row : pre_page * S.g.k_page + pre_row * S.g.k_row;
+            const unsigned char* const from = values ? v_lane + ld.h * P.v_head * 2 : k_lane + ld.h * P.k_head * 2;
+            const uint32_t have = __ballot_sync(0xffffffffu, pre_live && found), at = ring + fill_slot * HALF;
             constexpr int PER = CH >= 32 ? 1 : 32 / CH;      // rows per warp-wide copy
-            #pragma unroll
-            for (int r0 = 0; r0 < KW / WR; r0 += PER)
+            const int r_lane = wr * (KW / WR) + (CH >= 32 ? 0 : lane / CH);
+            if (have == 0xffffffffu)
             {
-                const int r = wr * (KW / WR) + r0 + (CH >= 32 ? 0 : lane / CH), c = lane % CH;
-                const long long o = __shfl_sync(0xffffffffu, off, r);
-                at_copy16(at + r * (2 * D) + ((c ^ (r & 7)) << 4), base + o + c * 8, (have >> r) & 1);
-            }
-            if (KW == 16 ? (lost & 0xffffu) && !values : lost && !values)
-            {
-                // (behind the copies of zeros: they are waited for before the stores)
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                for (int i = lane; i < KW / WR * CH; i += 32)
+                #pragma unroll
+                for (int r0 = 0; r0 < KW / WR; r0 += PER)
                 {
-                    const int r = wr * (KW / WR) + i / CH;
-                    if ((lost >> r) & 1)
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" :: "r"(at + r * (2 * D) + (i % CH) * 16), "r"(0x7fff7fffu) : "memory");
+                    const int r = r_lane + r0;
+                    cp_async16_s(at + r * (2 * D) + (((lane % CH) ^ (r & 7)) << 4), from + (unsigned long long) __shfl_sync(0xffffffffu, off, r) * 16);
+                }
+            }
+            else
+            {
+                // behind the last key, and on pages outside the pool: zeros
+                #pragma unroll
+                for (int r0 = 0; r0 < KW / WR; r0 += PER)
+                {
+                    const int r = r_lane + r0;
+                    const uint32_t o = __shfl_sync(0xffffffffu, off, r);
+                    const bool get = (have >> r) & 1;
+                    at_copy16(at + r * (2 * D) + (((lane % CH) ^ (r & 7)) << 4), get ? from + (unsigned long long) o * 16 : from, get);
+                }
+                const uint32_t lost = __ballot_sync(0xffffffffu, pre_live && !found);
+                if (lost && !values)
+                {
+                    // a key that cannot be found is NaN to the rows that see it, its value 0 (the copies of zeros are in front)
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    for (int i = lane; i < KW / WR * CH; i += 32)
+                    {
+                        const int r = wr * (KW / WR) + i / CH;
+                        if ((lost >> r) & 1)
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" :: "r"(at + r * (2 * D) + (i % CH) * 16), "r"(0x7fff7fffu) : "memory");
+                    }
                 }
             }
             if (values && --to_load > 0) { ld.advance(S); look_up(); }
@@ -527,13 +546,12 @@ void attention_join_kernel(const AtPlan S)
     const amp_attention_args& P = S.P;
     __shared__ float s_red[4], s_sum[4];
     __shared__ float4 s_o[4][D / 4];
-    __shared__ long long s_scan[4], s_found[2];
+    __shared__ int s_scan[4], s_found[2];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, r = blockIdx.y, group = P.heads / P.kv_heads;
     AtCount C;
     C.count<128>(S, s_scan);
-    const int ctas = C.ctas(S);
     AtCursor in;
-    long long g0;                                            // first unit of the segment
+    int g0;                                                  // first unit of the segment
     int first, last;                                         // CTAs that hold it
     bool join = false;
     if (S.by_segment)
@@ -542,14 +560,13 @@ void attention_join_kernel(const AtPlan S)
         const int per = P.kv_heads * in.tiles, b = blockIdx.x / per;
         in.b = b; in.h = blockIdx.x % per / in.tiles; in.rt = blockIdx.x % in.tiles;
         in.load(S);
-        g0 = C.front_of(S, b, s_found) + ((long long) in.h * in.tiles + in.rt) * in.units;
+        g0 = C.front_of(S, b, s_found) + (in.h * in.tiles + in.rt) * in.units;
         join = true;
     }
-    else if ((int) blockIdx.x < ctas)
+    else if ((int) blockIdx.x < C.ctas)
     {
-        const long long u0 = blockIdx.x * C.total / ctas;
-        int b;
-        long long front;
+        const int u0 = C.begin(blockIdx.x);
+        int b, front;
         C.find(S, u0, b, front, s_found);
         in.place(S, b, u0 - front);
         g0 = u0 - in.u;
@@ -557,8 +574,8 @@ void attention_join_kernel(const AtPlan S)
     }
     if (join)
     {
-        first = (int) (((g0 + 1) * ctas - 1) / C.total);
-        last = (int) (((g0 + in.units) * ctas - 1) / C.total);
+        first = C.cta_of(g0);
+        last = C.cta_of(g0 + in.units - 1);
         join = first < last && (S.by_segment || first == (int) blockIdx.x - 1);
     }
     const int row = join ? in.rt * S.rows + r : 0, tok = row / group;
@@ -712,8 +729,11 @@ static int at_launch(AtPlan& S, cudaStream_t stream)
     if (cudaError_t e = ensure_smem(attention_split_kernel<T, D, WR>, at_smem<D>, dev)) return cuda_rc(e, "attention shared memory");
     S.unit = at_unit<D, WR>;
     S.rows = 16 * WR;
+    const long group = P.heads / P.kv_heads;
+    AMP_REQUIRE((double) P.kv_heads * (P.tokens * group / S.rows + P.seqs) * (P.max_pages * (double) P.page_size / S.unit + 1) < 2147483648.0,
+                "attention: more keys than one call takes (%d sequences of up to %ld)", P.seqs, (long) P.max_pages * P.page_size);
     // (segments of the call, where the host knows them)
-    const long rows = (long) (P.tokens / P.seqs) * (P.heads / P.kv_heads), segments = (long) P.seqs * P.kv_heads * ((rows + S.rows - 1) / S.rows);
+    const long rows = (long) (P.tokens / P.seqs) * group, segments = (long) P.seqs * P.kv_heads * ((rows + S.rows - 1) / S.rows);
     const long grid = S.whole ? segments : S.grid;
     AMP_REQUIRE(grid < (1l << 31), "attention: too many sequences");
     cudaLaunchAttribute attr[1];
@@ -784,19 +804,21 @@ AMP_API int amp_b200_attention(const amp_attention_args* args, cudaStream_t stre
     int rc = 0;
     const AtDevice* d = at_device(&rc);
     if (!d) return rc;
+    AtPages g;
+    AMP_REQUIRE(at_pages(P, g), "attention: a cache of more than 64 GB, or negative strides");
     const AtCut C = at_cut(P.tokens, P.seqs, P.heads, P.kv_heads, P.dim, P.cu != nullptr, (long) P.max_pages * P.page_size, P.window, P.sinks, d->sms);
     if (C.bytes)
         AMP_REQUIRE(P.workspace && ((uintptr_t) P.workspace & 15) == 0 && P.workspace_bytes >= (long) C.bytes, "attention: workspace too small or misaligned");
     if (C.split)
     {
         S.grid = C.grid; S.whole = C.whole; S.pdl = g_pdl; S.split_rows = P.cu ? AT_SPLIT_ROWS : 1 << 30;
-        S.scale2 = P.scale * 1.4426950408889634f;
+        S.scale2 = P.scale * 1.4426950408889634f; S.g = g;
         rc = P.bf16 ? at_launch_dim<__nv_bfloat16>(S, C.wr, stream) : at_launch_dim<__half>(S, C.wr, stream);
         if (rc) return rc;
     }
     if (!C.tc) return 0;
     TaPlan A;
     A.P = P; A.tiles = C.tiles; A.slices = C.slices; A.split_rows = P.cu ? AT_SPLIT_ROWS : 0; A.pdl = g_pdl;
-    A.scale2 = P.scale * 1.4426950408889634f; A.part_offset = C.tc_offset;
+    A.scale2 = P.scale * 1.4426950408889634f; A.part_offset = C.tc_offset; A.g = g;
     return attention_tc(A, stream);
 }

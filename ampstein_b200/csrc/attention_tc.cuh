@@ -23,6 +23,7 @@ struct TaPlan
     int pdl;
     float scale2;                              // scale * log2(e)
     size_t part_offset;                        // of the parts in the workspace
+    AtPages g;
 };
 
 int attention_tc(const TaPlan& S, cudaStream_t stream);
