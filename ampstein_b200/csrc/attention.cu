@@ -72,7 +72,8 @@ __device__ __forceinline__ int at_row_tiles(const AtPlan& S, const AtSeq& s)
 
 __device__ __forceinline__ int at_units(const AtPlan& S, const AtKeys& k) { return max(1, (k.count() + S.unit - 1) / S.unit); }
 
-// A place in the order of units
+// A place in the order of units. The end of a segment, where its parts meet and the next rows are fetched, counts as one more unit
+// (u == units): it takes a CTA about as long, and the many ends of short sequences would come on top of a full range.
 struct AtCursor
 {
     int b, h, rt, u, tiles, units;
@@ -91,12 +92,12 @@ struct AtCursor
     {
         b = seq;
         load(S);
-        const int row_tile = at / units;
-        u = at - row_tile * units;
+        const int row_tile = at / (units + 1);
+        u = at - row_tile * (units + 1);
         h = row_tile / tiles;
         rt = row_tile - h * tiles;
     }
-    // to the next unit; the caller knows that there is one
+    // to the next unit with keys, or segment; the caller knows that there is one
     __device__ __forceinline__ void advance(const AtPlan& S)
     {
         if (++u < units) return;
@@ -121,7 +122,7 @@ struct AtCount
     static __device__ __forceinline__ int units_of(const AtPlan& S, int b)
     {
         const AtSeq s = at_seq(S.P, b);
-        return S.P.kv_heads * at_row_tiles(S, s) * at_units(S, at_keys(S.P, s.first, s.count));
+        return S.P.kv_heads * at_row_tiles(S, s) * (at_units(S, at_keys(S.P, s.first, s.count)) + 1);
     }
 
     template <int NT>
@@ -244,6 +245,11 @@ void attention_split_kernel(const AtPlan S)
         int b, front;
         C.find(S, u0, b, front, s_found);
         in.place(S, b, u0 - front);
+        if (in.u == in.units)                                // (the CTA in front ends that segment)
+        {
+            if (--left == 0) return;
+            in.advance(S);
+        }
     }
     const bool began_before = in.u > 0;
 
@@ -309,7 +315,11 @@ void attention_split_kernel(const AtPlan S)
                     }
                 }
             }
-            if (values && --to_load > 0) { ld.advance(S); look_up(); }
+            if (values)
+            {
+                to_load -= ld.u + 1 == ld.units ? 2 : 1;
+                if (to_load > 0) { ld.advance(S); look_up(); }
+            }
             values = !values;
         }
         cp_async_commit();
@@ -457,7 +467,7 @@ void attention_split_kernel(const AtPlan S)
                 }
             }
         }
-        --left;
+        left -= ends ? 2 : 1;
         if (flush)
         {
             const bool shared = !S.whole && ((first_segment && began_before) || !ends);
@@ -560,7 +570,7 @@ void attention_join_kernel(const AtPlan S)
         const int per = P.kv_heads * in.tiles, b = blockIdx.x / per;
         in.b = b; in.h = blockIdx.x % per / in.tiles; in.rt = blockIdx.x % in.tiles;
         in.load(S);
-        g0 = C.front_of(S, b, s_found) + (in.h * in.tiles + in.rt) * in.units;
+        g0 = C.front_of(S, b, s_found) + (in.h * in.tiles + in.rt) * (in.units + 1);
         join = true;
     }
     else if ((int) blockIdx.x < C.ctas)
@@ -570,7 +580,7 @@ void attention_join_kernel(const AtPlan S)
         C.find(S, u0, b, front, s_found);
         in.place(S, b, u0 - front);
         g0 = u0 - in.u;
-        join = in.u > 0;
+        join = in.u > 0 && in.u < in.units;
     }
     if (join)
     {
@@ -730,7 +740,7 @@ static int at_launch(AtPlan& S, cudaStream_t stream)
     S.unit = at_unit<D, WR>;
     S.rows = 16 * WR;
     const long group = P.heads / P.kv_heads;
-    AMP_REQUIRE((double) P.kv_heads * (P.tokens * group / S.rows + P.seqs) * (P.max_pages * (double) P.page_size / S.unit + 1) < 2147483648.0,
+    AMP_REQUIRE((double) P.kv_heads * (P.tokens * group / S.rows + P.seqs) * (P.max_pages * (double) P.page_size / S.unit + 2) < 2147483648.0,
                 "attention: more keys than one call takes (%d sequences of up to %ld)", P.seqs, (long) P.max_pages * P.page_size);
     // (segments of the call, where the host knows them)
     const long rows = (long) (P.tokens / P.seqs) * group, segments = (long) P.seqs * P.kv_heads * ((rows + S.rows - 1) / S.rows);
