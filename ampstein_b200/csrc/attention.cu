@@ -18,14 +18,17 @@ namespace amp {
 
 constexpr int AT_WARP_SEQS = 32;               // sequences that a warp counts by itself
 
-template <int D> constexpr int at_warps = D == 256 ? 8 : 4;
+constexpr int AT_WARPS = 4, AT_THREADS = 32 * AT_WARPS;
 template <int D> constexpr int at_kw = D == 256 ? 16 : 32;     // keys of a group's step
-template <int D> constexpr int at_ctas = D == 64 ? 3 : (D == 128 ? 2 : 1);     // per SM
+template <int D> constexpr int at_ctas = D == 64 ? 3 : 2;      // per SM
 template <int D> constexpr int at_half_bytes = at_kw<D> * D * 2;
-template <int D> constexpr int at_smem = (D == 64 ? 64 : D == 128 ? 96 : 192) * 1024;
-template <int D, int WR> constexpr int at_wk = at_warps<D> / WR;
-template <int D, int WR> constexpr int at_halves = at_smem<D> / (at_wk<D, WR> * at_half_bytes<D>);
-template <int D, int WR> constexpr int at_unit = at_wk<D, WR> * at_kw<D>;      // keys
+template <int WR> constexpr int at_wk = AT_WARPS / WR;
+template <int WR> constexpr int at_rows = 16 * WR;             // of a row tile
+template <int D, int WR> constexpr int at_unit = at_wk<WR> * at_kw<D>;         // keys
+// shared memory: rings, then the rows of q
+template <int D, int WR> constexpr int at_halves = (D == 64 ? 64 : D == 128 ? (WR == 4 ? 80 : 96) : (WR == 1 ? 96 : WR == 2 ? 80 : 64)) * 1024 / (at_wk<WR> * at_half_bytes<D>);
+template <int D, int WR> constexpr int at_ring_bytes = at_halves<D, WR> * at_wk<WR> * at_half_bytes<D>;
+template <int D, int WR> constexpr int at_smem = at_ring_bytes<D, WR> + at_rows<WR> * D * 2;
 
 struct AtPlan
 {
@@ -210,15 +213,17 @@ struct AtCount
 __host__ __device__ constexpr size_t at_part_floats(int rows, int dim) { return (size_t) rows * (dim + 2); }
 
 template <typename T, int D, int WR>
-__global__ __launch_bounds__(32 * at_warps<D>, at_ctas<D>)
+__global__ __launch_bounds__(AT_THREADS, at_ctas<D>)
 void attention_split_kernel(const AtPlan S)
 {
     const amp_attention_args& P = S.P;
-    constexpr int NW = at_warps<D>, NT = 32 * NW, WK = at_wk<D, WR>, KW = at_kw<D>, H = at_halves<D, WR>, HALF = at_half_bytes<D>;
-    constexpr int CH = D / 8, NK = KW / 8, ROWS = 16 * WR, UNIT = at_unit<D, WR>;
+    constexpr int NT = AT_THREADS, WK = at_wk<WR>, KW = at_kw<D>, H = at_halves<D, WR>, HALF = at_half_bytes<D>;
+    constexpr int CH = D / 8, NK = KW / 8, ROWS = at_rows<WR>, UNIT = at_unit<D, WR>;
+    constexpr bool KEEP_Q = D <= 128;          // q's fragments stay in registers (256: they are read for every step)
+    static_assert(H >= 3, "ring");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_ml[WK][ROWS][2];
-    __shared__ int s_scan[NW], s_found[2];
+    __shared__ int s_scan[AT_WARPS], s_found[2];
 
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, grp = warp / WR, wr = warp % WR, cta = blockIdx.x;
     const int group = P.heads / P.kv_heads;
@@ -253,7 +258,7 @@ void attention_split_kernel(const AtPlan S)
     }
     const bool began_before = in.u > 0;
 
-    const uint32_t ring = smem_u32(smem) + grp * H * HALF;
+    const uint32_t ring = smem_u32(smem) + grp * H * HALF, q_s = smem_u32(smem) + at_ring_bytes<D, WR>;
     auto sync_group = [&]() { if constexpr (WR == 1) __syncwarp(); else asm volatile("bar.sync %0, %1;" :: "r"(1 + grp), "n"(32 * WR) : "memory"); };
 
     // ---- loads: lane l looks up key l of the group's KW, the table entry a unit ahead; halves alternate keys, values -----------
@@ -326,224 +331,232 @@ void attention_split_kernel(const AtPlan S)
         fill_slot = fill_slot + 1 == H ? 0 : fill_slot + 1;
     };
     look_up();
-    #pragma unroll 1
-    for (int i = 0; i < H; ++i) issue();
-    bool full = true;                                        // the half behind the one at hand has been requested H ahead
 
-    // ---- the segments of the range -------------------------------------------------------------------------------------------
-    uint32_t qf[D / 16][4];
+    // ---- the segments of the range, a half stage per turn ---------------------------------------------------------------------
+    uint32_t qf[KEEP_Q ? D / 16 : 1][4], pf[NK / 2][4];
     float o[D / 8][4], m[2], l[2];
     int n0[2], c1[2], len[2];                                // keys that the lane's two rows see: [0, n0) and [c1, c1 + len]
-    int whole_from = 0, whole_to = 0;                        // units that all rows see whole: [from, to)
-    bool fresh = true, first_segment = true;
-    int slot = 0;
-    // waits for the half at `slot` and refills the one in front of it
-    auto next_half = [&](bool refill) {
-        if (full) asm volatile("cp.async.wait_group %0;" :: "n"(H - 1) : "memory");
-        else asm volatile("cp.async.wait_group %0;" :: "n"(H - 2) : "memory");
-        sync_group();
-        if (!full && refill) issue();
-        else if (!full) return;
-        full = false;
+    int whole_from = 0, whole_to = 0;                        // keys that all rows see
+    bool fresh = true, first_segment = true, hold = false;
+    int slot = 0, key_slot = 0, ahead = 0;                   // ahead: half stages requested from the one at hand on
+    // fragment of q for a step of 16 values: rows of the warp
+    auto q_fragment = [&](int ks, uint32_t (&f)[4]) {
+        const int r = wr * 16 + (lane & 15), c = 2 * ks + (lane >> 4);
+        at_ldsm4(q_s + r * (2 * D) + ((c ^ (r & 7)) << 4), f);
     };
-    while (left > 0)
+    for (int turn = -1; left > 0; ++turn)
     {
-        if (fresh)
+        // the half at hand has landed, for all lanes of the group; the ones in front of it are read: their slots are filled again
+        if (turn >= 0)
         {
-            #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            if (ahead == H) asm volatile("cp.async.wait_group %0;" :: "n"(H - 1) : "memory");
+            else if (ahead == H - 1) asm volatile("cp.async.wait_group %0;" :: "n"(H - 2) : "memory");
+            else asm volatile("cp.async.wait_group %0;" :: "n"(H - 3) : "memory");
+            sync_group();
+        }
+        const bool is_key = (turn & 1) == 0, ends = in.u + 1 == in.units;
+        hold = !is_key && turn >= 0 && (ends || left == 1);  // (the end of a segment uses both halves at hand)
+        #pragma unroll 1
+        while (ahead < H && !hold) { issue(); ++ahead; }
+        if (turn < 0) continue;
+        const int key0 = in.u * UNIT + grp * KW;
+        const bool some = key0 < in.k.count();
+        const uint32_t at = ring + slot * HALF;
+        if (is_key)
+        {
+            if (fresh)
             {
-                const int r = in.rt * ROWS + wr * 16 + (lane >> 2) + 8 * i, tok = r / group, p = in.s.first + tok;
-                const bool have = tok < in.s.count;
-                const T* q = reinterpret_cast<const T*>(P.q) + (long long) (in.s.row0 + tok) * P.q_token + (long long) (in.h * group + r - tok * group) * P.q_head + (lane & 3) * 2;
+                for (int i = t; i < ROWS * CH; i += NT)
+                {
+                    const int r = i / CH, c = i % CH, row = in.rt * ROWS + r, tok = row / group;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (tok < in.s.count)
+                        v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(P.q) + (long long) (in.s.row0 + tok) * P.q_token
+                                                            + (long long) (in.h * group + row - tok * group) * P.q_head + c * 8);
+                    *reinterpret_cast<uint4*>(smem + at_ring_bytes<D, WR> + r * (2 * D) + ((c ^ (r & 7)) << 4)) = v;
+                }
+                #pragma unroll
+                for (int i = 0; i < 2; ++i)
+                {
+                    m[i] = -INFINITY;
+                    l[i] = 0.0f;
+                    at_row_keys(P, in.k, in.s.first + (in.rt * ROWS + wr * 16 + (lane >> 2) + 8 * i) / group, n0[i], c1[i], len[i]);
+                }
+                at_whole_keys(P, in.k, in.s.first, in.s.first + in.s.count - 1, whole_from, whole_to);
+                #pragma unroll
+                for (int n = 0; n < D / 8; ++n) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f; }
+                __syncthreads();
+                if constexpr (KEEP_Q)
+                {
+                    #pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) q_fragment(ks, qf[ks]);
+                }
+                fresh = false;
+            }
+            key_slot = slot;
+            if (some)
+            {
+                // s = q k^T: rows x KW keys
+                float s[NK][4];
+                #pragma unroll
+                for (int n = 0; n < NK; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
                 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
                 {
-                    qf[ks][i] = have ? *reinterpret_cast<const uint32_t*>(q + ks * 16) : 0u;
-                    qf[ks][i + 2] = have ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8) : 0u;
-                }
-                m[i] = -INFINITY;
-                l[i] = 0.0f;
-                at_row_keys(P, in.k, p, n0[i], c1[i], len[i]);
-            }
-            const int last = in.s.first + in.s.count - 1;
-            at_whole_keys(P, in.k, in.s.first, last, whole_from, whole_to);
-            #pragma unroll
-            for (int n = 0; n < D / 8; ++n) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f; }
-            fresh = false;
-        }
-        const int key0 = in.u * UNIT + grp * KW;
-        const bool some = key0 < in.k.count();
-        next_half(true);
-        const uint32_t kb = ring + slot * HALF;
-        float s[NK][4];
-        if (some)
-        {
-            // s = q k^T: rows x KW keys
-            #pragma unroll
-            for (int n = 0; n < NK; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-            #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
-            {
-                #pragma unroll
-                for (int n = 0; n < NK; n += 2)
-                {
-                    const int r = n * 8 + (lane & 7) + ((lane >> 4) << 3), c = 2 * ks + ((lane >> 3) & 1);
-                    uint32_t f[4];
-                    at_ldsm4(kb + r * (2 * D) + ((c ^ (r & 7)) << 4), f);
-                    at_mma<T>(s[n], qf[ks], f[0], f[1]);
-                    at_mma<T>(s[n + 1], qf[ks], f[2], f[3]);
-                }
-            }
-        }
-        const int key_slot = slot;
-        slot = slot + 1 == H ? 0 : slot + 1;
-        const bool ends = in.u + 1 == in.units, flush = ends || left == 1;
-        uint32_t pf[NK / 2][4];
-        if (some)
-        {
-            const bool all = key0 >= whole_from && key0 + KW <= whole_to;
-            float top[2] = { m[0], m[1] };
-            #pragma unroll
-            for (int n = 0; n < NK; ++n)
-            {
-                #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                {
-                    s[n][e] *= S.scale2;
-                    if (!all)
+                    if constexpr (!KEEP_Q) q_fragment(ks, qf[0]);
+                    #pragma unroll
+                    for (int n = 0; n < NK; n += 2)
                     {
-                        const int c = key0 + n * 8 + (lane & 3) * 2 + (e & 1), i = e >> 1;
-                        if (!(c < n0[i] || (uint32_t) (c - c1[i]) <= (uint32_t) len[i])) s[n][e] = -INFINITY;
+                        const int r = n * 8 + (lane & 7) + ((lane >> 4) << 3), c = 2 * ks + ((lane >> 3) & 1);
+                        uint32_t f[4];
+                        at_ldsm4(at + r * (2 * D) + ((c ^ (r & 7)) << 4), f);
+                        at_mma<T>(s[n], qf[KEEP_Q ? ks : 0], f[0], f[1]);
+                        at_mma<T>(s[n + 1], qf[KEEP_Q ? ks : 0], f[2], f[3]);
                     }
-                    top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
                 }
-            }
-            #pragma unroll
-            for (int i = 0; i < 2; ++i)
-            {
-                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-            }
-            if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1]))
-            {
+                const bool all = key0 >= whole_from && key0 + KW <= whole_to;
+                float top[2] = { m[0], m[1] };
+                #pragma unroll
+                for (int n = 0; n < NK; ++n)
+                {
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        s[n][e] *= S.scale2;
+                        if (!all)
+                        {
+                            const int c = key0 + n * 8 + (lane & 3) * 2 + (e & 1), i = e >> 1;
+                            if (!(c < n0[i] || (uint32_t) (c - c1[i]) <= (uint32_t) len[i])) s[n][e] = -INFINITY;
+                        }
+                        top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+                    }
+                }
                 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                 {
-                    const float f = top[i] > m[i] ? at_exp2(m[i] - top[i]) : 1.0f;
-                    m[i] = top[i];
-                    l[i] *= f;
-                    #pragma unroll
-                    for (int n = 0; n < D / 8; ++n) { o[n][2 * i] *= f; o[n][2 * i + 1] *= f; }
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
                 }
-            }
-            const float base0 = m[0] == -INFINITY ? 0.0f : m[0], base1 = m[1] == -INFINITY ? 0.0f : m[1];
-            #pragma unroll
-            for (int n = 0; n < NK; ++n)
-            {
-                s[n][0] = at_exp2(s[n][0] - base0); s[n][1] = at_exp2(s[n][1] - base0);
-                s[n][2] = at_exp2(s[n][2] - base1); s[n][3] = at_exp2(s[n][3] - base1);
-                l[0] += s[n][0] + s[n][1];
-                l[1] += s[n][2] + s[n][3];
-                pf[n / 2][2 * (n & 1)] = AtType<T>::pack(s[n][0], s[n][1]);
-                pf[n / 2][2 * (n & 1) + 1] = AtType<T>::pack(s[n][2], s[n][3]);
-            }
-        }
-        next_half(!flush);                                   // (a flush uses both halves)
-        const uint32_t vb = ring + slot * HALF;
-        if (some)
-        {
-            #pragma unroll
-            for (int kk = 0; kk < NK / 2; ++kk)
-            {
-                #pragma unroll
-                for (int n = 0; n < D / 16; ++n)
+                if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1]))
                 {
-                    const int r = kk * 16 + (lane & 15), c = 2 * n + (lane >> 4);
-                    uint32_t f[4];
-                    at_ldsm4_trans(vb + r * (2 * D) + ((c ^ (r & 7)) << 4), f);
-                    at_mma<T>(o[2 * n], pf[kk], f[0], f[1]);
-                    at_mma<T>(o[2 * n + 1], pf[kk], f[2], f[3]);
+                    #pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                    {
+                        const float f = top[i] > m[i] ? at_exp2(m[i] - top[i]) : 1.0f;
+                        m[i] = top[i];
+                        l[i] *= f;
+                        #pragma unroll
+                        for (int n = 0; n < D / 8; ++n) { o[n][2 * i] *= f; o[n][2 * i + 1] *= f; }
+                    }
+                }
+                const float base0 = m[0] == -INFINITY ? 0.0f : m[0], base1 = m[1] == -INFINITY ? 0.0f : m[1];
+                #pragma unroll
+                for (int n = 0; n < NK; ++n)
+                {
+                    s[n][0] = at_exp2(s[n][0] - base0); s[n][1] = at_exp2(s[n][1] - base0);
+                    s[n][2] = at_exp2(s[n][2] - base1); s[n][3] = at_exp2(s[n][3] - base1);
+                    l[0] += s[n][0] + s[n][1];
+                    l[1] += s[n][2] + s[n][3];
+                    pf[n / 2][2 * (n & 1)] = AtType<T>::pack(s[n][0], s[n][1]);
+                    pf[n / 2][2 * (n & 1) + 1] = AtType<T>::pack(s[n][2], s[n][3]);
                 }
             }
         }
-        left -= ends ? 2 : 1;
-        if (flush)
+        else
         {
-            const bool shared = !S.whole && ((first_segment && began_before) || !ends);
-            float* const part = reinterpret_cast<float*>(P.workspace) + (size_t) (2 * cta + (first_segment && began_before ? 0 : 1)) * at_part_floats(ROWS, D);
-            #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            if (some)
             {
-                l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-                l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-                if ((lane & 3) == 0) { s_ml[grp][wr * 16 + (lane >> 2) + 8 * i][0] = m[i]; s_ml[grp][wr * 16 + (lane >> 2) + 8 * i][1] = l[i]; }
-            }
-            __syncthreads();
-            float f[2];
-            #pragma unroll
-            for (int i = 0; i < 2; ++i)
-            {
-                float top = s_ml[0][wr * 16 + (lane >> 2) + 8 * i][0];
                 #pragma unroll
-                for (int g = 1; g < WK; ++g) top = fmaxf(top, s_ml[g][wr * 16 + (lane >> 2) + 8 * i][0]);
-                f[i] = m[i] == -INFINITY ? 0.0f : at_exp2(m[i] - top);
+                for (int kk = 0; kk < NK / 2; ++kk)
+                {
+                    #pragma unroll
+                    for (int n = 0; n < D / 16; ++n)
+                    {
+                        const int r = kk * 16 + (lane & 15), c = 2 * n + (lane >> 4);
+                        uint32_t f[4];
+                        at_ldsm4_trans(at + r * (2 * D) + ((c ^ (r & 7)) << 4), f);
+                        at_mma<T>(o[2 * n], pf[kk], f[0], f[1]);
+                        at_mma<T>(o[2 * n + 1], pf[kk], f[2], f[3]);
+                    }
+                }
             }
-            // the groups' parts meet in the two half stages that each has just read, D / WR columns at a time: the
-            // columns of a row are turned round by 8 for every row (mod 4), so that eight rows meet all banks
-            constexpr int COLS = D / WR, PIECE = 16 * COLS * 4, TURN = COLS >= 32 ? 3 : COLS / 8 - 1;
-            auto place = [&](int g, int w, int r, int c) {   // byte offset in the group's ring
-                const int at = w * PIECE + (r * COLS + (c ^ ((r & TURN) << 3))) * 4;
-                return g * H * HALF + (at < HALF ? key_slot * HALF + at : slot * HALF + at - HALF);
-            };
-            #pragma unroll
-            for (int pass = 0; pass < WR; ++pass)
+            left -= ends ? 2 : 1;
+            if (hold)
             {
+                const bool before = first_segment && began_before, shared = !S.whole && (before || !ends);
+                float* const part = reinterpret_cast<float*>(P.workspace) + (size_t) (2 * cta + (before ? 0 : 1)) * at_part_floats(ROWS, D);
                 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                 {
-                    const int r = (lane >> 2) + 8 * i;
-                    #pragma unroll
-                    for (int n = 0; n < COLS / 8; ++n)
-                        *reinterpret_cast<float2*>(smem + place(grp, wr, r, n * 8 + (lane & 3) * 2)) =
-                            make_float2(o[pass * (COLS / 8) + n][2 * i] * f[i], o[pass * (COLS / 8) + n][2 * i + 1] * f[i]);
+                    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+                    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+                    if ((lane & 3) == 0) { s_ml[grp][wr * 16 + (lane >> 2) + 8 * i][0] = m[i]; s_ml[grp][wr * 16 + (lane >> 2) + 8 * i][1] = l[i]; }
                 }
                 __syncthreads();
-                for (int i = t; i < ROWS * COLS / 4; i += NT)
+                float f[2];
+                #pragma unroll
+                for (int i = 0; i < 2; ++i)
                 {
-                    const int r = i / (COLS / 4), c = (i % (COLS / 4)) * 4;
-                    const int row = in.rt * ROWS + r, tok = row / group;
-                    if (tok >= in.s.count) break;            // (rows ascend with i)
-                    float top = s_ml[0][r][0], sum = 0.0f;
+                    float top = s_ml[0][wr * 16 + (lane >> 2) + 8 * i][0];
                     #pragma unroll
-                    for (int g = 1; g < WK; ++g) top = fmaxf(top, s_ml[g][r][0]);
-                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    #pragma unroll
-                    for (int g = 0; g < WK; ++g)
-                    {
-                        sum += s_ml[g][r][0] == -INFINITY ? s_ml[g][r][1] : s_ml[g][r][1] * at_exp2(s_ml[g][r][0] - top);      // (an l of NaN stays one)
-                        const float4 y = *reinterpret_cast<const float4*>(smem + place(g, r >> 4, r & 15, c));
-                        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-                    }
-                    const int col = pass * COLS + c;
-                    if (shared)
-                    {
-                        *reinterpret_cast<float4*>(part + r * D + col) = x;
-                        if (col == 0) *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(top, sum);
-                    }
-                    else
-                        at_store<T>(P, in.s, tok, in.h * group + row - tok * group, col, x, top, sum);
+                    for (int g = 1; g < WK; ++g) top = fmaxf(top, s_ml[g][wr * 16 + (lane >> 2) + 8 * i][0]);
+                    f[i] = m[i] == -INFINITY ? 0.0f : at_exp2(m[i] - top);
                 }
-                __syncthreads();
+                // the groups' parts meet in the two half stages that each has just read, D / WR columns at a time: the columns of a row
+                // are turned round by 8 for every row (mod 4), so that eight rows meet all banks
+                constexpr int COLS = D / WR, PIECE = 16 * COLS * 4, TURN = COLS >= 32 ? 3 : COLS / 8 - 1;
+                auto place = [&](int g, int w, int r, int c) {           // byte offset in the group's ring
+                    const int x = w * PIECE + (r * COLS + (c ^ ((r & TURN) << 3))) * 4;
+                    return g * H * HALF + (x < HALF ? key_slot * HALF + x : slot * HALF + x - HALF);
+                };
+                #pragma unroll
+                for (int pass = 0; pass < WR; ++pass)
+                {
+                    #pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                    {
+                        const int r = (lane >> 2) + 8 * i;
+                        #pragma unroll
+                        for (int n = 0; n < COLS / 8; ++n)
+                            *reinterpret_cast<float2*>(smem + place(grp, wr, r, n * 8 + (lane & 3) * 2)) =
+                                make_float2(o[pass * (COLS / 8) + n][2 * i] * f[i], o[pass * (COLS / 8) + n][2 * i + 1] * f[i]);
+                    }
+                    __syncthreads();
+                    #pragma unroll 1
+                    for (int i = t; i < ROWS * COLS / 4; i += NT)
+                    {
+                        const int r = i / (COLS / 4), c = (i % (COLS / 4)) * 4;
+                        const int row = in.rt * ROWS + r, tok = row / group;
+                        if (tok >= in.s.count) break;        // (rows ascend with i)
+                        float top = s_ml[0][r][0], sum = 0.0f;
+                        #pragma unroll
+                        for (int g = 1; g < WK; ++g) top = fmaxf(top, s_ml[g][r][0]);
+                        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        #pragma unroll
+                        for (int g = 0; g < WK; ++g)
+                        {
+                            sum += s_ml[g][r][0] == -INFINITY ? s_ml[g][r][1] : s_ml[g][r][1] * at_exp2(s_ml[g][r][0] - top);      // (an l of NaN stays one)
+                            const float4 y = *reinterpret_cast<const float4*>(smem + place(g, r >> 4, r & 15, c));
+                            x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+                        }
+                        const int col = pass * COLS + c;
+                        if (shared)
+                        {
+                            *reinterpret_cast<float4*>(part + r * D + col) = x;
+                            if (col == 0) *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(top, sum);
+                        }
+                        else
+                            at_store<T>(P, in.s, tok, in.h * group + row - tok * group, col, x, top, sum);
+                    }
+                    __syncthreads();
+                }
+                fresh = true;
+                first_segment = false;
             }
-            fresh = true;
-            first_segment = false;
-            issue();                                         // both halves
-            issue();
-            full = true;
+            if (left > 0) in.advance(S);
         }
         slot = slot + 1 == H ? 0 : slot + 1;
-        if (left > 0) in.advance(S);
+        --ahead;
     }
 }
 
@@ -736,7 +749,7 @@ static int at_launch(AtPlan& S, cudaStream_t stream)
     const amp_attention_args& P = S.P;
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return cuda_rc(e, "attention device");
-    if (cudaError_t e = ensure_smem(attention_split_kernel<T, D, WR>, at_smem<D>, dev)) return cuda_rc(e, "attention shared memory");
+    if (cudaError_t e = ensure_smem(attention_split_kernel<T, D, WR>, at_smem<D, WR>, dev)) return cuda_rc(e, "attention shared memory");
     S.unit = at_unit<D, WR>;
     S.rows = 16 * WR;
     const long group = P.heads / P.kv_heads;
@@ -751,8 +764,8 @@ static int at_launch(AtPlan& S, cudaStream_t stream)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) grid, 1, 1);
-    cfg.blockDim = dim3(32 * at_warps<D>, 1, 1);
-    cfg.dynamicSmemBytes = at_smem<D>;
+    cfg.blockDim = dim3(AT_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = at_smem<D, WR>;
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = S.pdl ? 1 : 0;
