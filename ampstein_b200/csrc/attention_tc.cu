@@ -11,8 +11,8 @@
 // weights from fp16's range), so that O is rarely scaled again. Where the grid leaves SMs idle the keys of a tile are cut into
 // slices, whose parts a second kernel joins in order.
 //
-// Warps: four per row tile do the softmax (a thread a row, the warp's quarter of tensor memory), then one issues the MMAs, two load
-// keys and values by 16-byte asynchronous copies (a page of any size, strides of any kind), one rests.
+// Warps: four per row tile do the softmax (a thread a row, the warp's quarter of tensor memory), then one issues the MMAs, three load
+// keys and values by 16-byte asynchronous copies (a page of any size, strides of any kind).
 //
 // Every mbarrier wait is bounded: a role whose wait ran out hands nothing over any more, whatever depends on it runs out too, nothing
 // is stored (slices: their rows become NaN), the status word is set, and the CTA leaves when its copies and MMAs are done.
@@ -23,6 +23,7 @@ namespace amp {
 __device__ int g_at_status;
 
 constexpr unsigned AT_SPIN_LIMIT = 1u << 21;   // looks at a barrier before a wait is declared lost (a look lasts up to 4 us)
+constexpr int TA_LOADERS = 3;                  // warps that load keys and values
 constexpr int TA_AHEAD = 2;                    // tiles on their way when the next is requested
 constexpr float TA_SLACK = 8.0f;               // powers of two that a row's maximum may grow before O is scaled again
 
@@ -176,7 +177,7 @@ void attention_tc_kernel(const TaPlan S)
     if (t == 0)
     {
         mbar_init(&q_full, 128 * NQ);
-        for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], 2); mbar_init(&kv_free[i], 1); }
+        for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], TA_LOADERS); mbar_init(&kv_free[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); }
         mbar_init(&o_full, 1);
         mbar_init(&end, 1);
@@ -448,11 +449,14 @@ void attention_tc_kernel(const TaPlan S)
         commit(smem_u32(&end));
         ta_wait(smem_u32(&end), 0);            // (bounded; the accumulators are given back only then)
     }
-    else if (warp <= 4 * NQ + 2)
+    else
     {
-        // ---- keys and values: half of a tile's rows per warp ------------------------------------------------------------------
-        constexpr int RW = KB / 2, PER = CH >= 32 ? 1 : 32 / CH;
-        const int r_first = (warp - 4 * NQ - 1) * RW, tiles = 2 * n;
+        // ---- keys and values, three warps: warp w makes every third of the copies of 32 x 16 bytes that a tile takes ---------------
+        constexpr int PER = CH >= 32 ? 1 : 32 / CH, COPIES = KB / PER, MINE = (COPIES + TA_LOADERS - 1) / TA_LOADERS, LOOKS = (MINE * PER + 31) / 32;
+        const int w = warp - 4 * NQ - 1, tiles = 2 * n, r_lane = CH >= 32 ? 0 : lane / CH, c_lane = lane % CH, count = keys.count();
+        const unsigned char* const k_base = reinterpret_cast<const unsigned char*>(P.k_cache) + h * P.k_head * 2 + c_lane * 16;
+        const unsigned char* const v_base = reinterpret_cast<const unsigned char*>(P.v_cache) + h * P.v_head * 2 + c_lane * 16;
+        const int* const table = P.table + (long long) s_place[1] * P.table_row;
         int issued = 0;
         auto hand_over = [&](int tile)
         {
@@ -460,45 +464,67 @@ void attention_tc_kernel(const TaPlan S)
             __syncwarp();
             if (lane == 0) ta_arrive(full_s + 8 * (tile % ST));
         };
+        #pragma unroll 1
         for (; issued < tiles; ++issued)
         {
             // tile 0 is K0, then K1, V0, K2, V1, ..., the last one V(n - 1)
             const bool is_v = issued > 0 && (issued % 2 == 0 || issued == tiles - 1);
             const int j = issued == 0 ? 0 : issued == tiles - 1 ? n - 1 : is_v ? issued / 2 - 1 : (issued + 1) / 2;
-            const int stage = issued % ST;
-            if (issued >= ST && !wait(free_s + 8 * stage, (issued / ST - 1) & 1)) break;
-            if (!ok) break;
-            const T* const base = reinterpret_cast<const T*>(is_v ? P.v_cache : P.k_cache) + (long long) h * (is_v ? P.v_head : P.k_head);
-            const long long page_st = is_v ? P.v_page : P.k_page, row_st = is_v ? P.v_row : P.k_row;
-            long long off[RW / 32];
-            int state[RW / 32];                // 1: fetch, 0: beyond the keys, -1: on a page outside the pool
+            // lane l looks up the l-th, (l + 32)-th ... of the warp's rows: offsets in pieces of 16 bytes
+            uint32_t off[LOOKS];
+            uint32_t have = 0xffffffffu;                     // lanes whose rows are all there
+            int state[LOOKS];                                // 1: there, 0: behind the last key, -1: on a page outside the pool
             #pragma unroll
-            for (int g = 0; g < RW / 32; ++g)
+            for (int g = 0; g < LOOKS; ++g)
             {
-                const int c = (j0 + j) * KB + r_first + 32 * g + lane;
-                off[g] = 0; state[g] = 0;
-                if (c < keys.count())
+                const int q = lane + 32 * g, r = (w + TA_LOADERS * (q / PER)) * PER + q % PER, c = (j0 + j) * KB + r;
+                off[g] = 0; state[g] = q < MINE * PER && r < KB ? 0 : 1;
+                if (state[g] == 0 && c < count)
                 {
-                    const int key = keys.key(c), pg = key / P.page_size, page = P.table[(long long) s_place[1] * P.table_row + pg];
-                    state[g] = page >= 0 && page < P.pages ? 1 : -1;
-                    if (state[g] > 0) off[g] = page * page_st + (key - pg * P.page_size) * row_st;
+                    const int key = keys.key(c), pg = S.g.page_of(key), page = table[pg], row = key - pg * P.page_size;
+                    state[g] = (unsigned) page < (unsigned) P.pages ? 1 : -1;
+                    off[g] = is_v ? page * S.g.v_page + row * S.g.v_row : page * S.g.k_page + row * S.g.k_row;
+                }
+                have &= __ballot_sync(0xffffffffu, state[g] > 0);
+            }
+            const int stage = issued % ST;
+            if (issued >= ST) wait(free_s + 8 * stage, (issued / ST - 1) & 1);
+            if (!ok) break;
+            const unsigned char* const base = is_v ? v_base : k_base;
+            const uint32_t to = kv_s + stage * KV_BYTES + (c_lane >> 3) * (KB * 128);
+            if (have == 0xffffffffu)
+            {
+                #pragma unroll
+                for (int i = 0; i < MINE; ++i)
+                {
+                    const int r = (w + TA_LOADERS * i) * PER + r_lane;
+                    const uint32_t o = __shfl_sync(0xffffffffu, off[i * PER / 32], i * PER % 32 + r_lane);
+                    if (COPIES % TA_LOADERS == 0 || i + 1 < MINE || w + TA_LOADERS * i < COPIES)
+                        cp_async16_s(to + r * 128 + (((c_lane & 7) ^ (r & 7)) << 4), base + (unsigned long long) o * 16);
                 }
             }
-            const uint32_t to = kv_s + stage * KV_BYTES;
-            #pragma unroll
-            for (int g = 0; g < RW / 32; ++g)
+            else
             {
-                #pragma unroll 8
-                for (int r0 = 0; r0 < 32; r0 += PER)
+                #pragma unroll 4
+                for (int i = 0; i < MINE; ++i)
                 {
-                    const int r = r0 + (CH >= 32 ? 0 : lane / CH), c = lane % CH, at = r_first + 32 * g + r;
-                    const long long o = __shfl_sync(0xffffffffu, off[g], r);
-                    const int st = __shfl_sync(0xffffffffu, state[g], r);
-                    const uint32_t dst = to + (c >> 3) * (KB * 128) + at * 128 + (((c & 7) ^ (at & 7)) << 4);
-                    if (st < 0 && !is_v)       // a key that cannot be found is NaN to the rows that see it
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" :: "r"(dst), "r"(0x7fff7fffu) : "memory");
-                    else
-                        at_copy16(dst, base + o + c * 8, st > 0);
+                    const int r = (w + TA_LOADERS * i) * PER + r_lane, from = (i * PER) % 32 + r_lane;
+                    uint32_t o = 0;
+                    int st = 0;
+                    #pragma unroll
+                    for (int g = 0; g < LOOKS; ++g)
+                    {
+                        const uint32_t x = __shfl_sync(0xffffffffu, off[g], from);
+                        const int y = __shfl_sync(0xffffffffu, state[g], from);
+                        if (g == i * PER / 32) { o = x; st = y; }
+                    }
+                    const uint32_t dst = to + r * 128 + (((c_lane & 7) ^ (r & 7)) << 4);
+                    if (w + TA_LOADERS * i < COPIES)
+                    {
+                        // a key that cannot be found is NaN to the rows that see it, its value 0; zeros behind the last key
+                        if (st < 0 && !is_v) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" :: "r"(dst), "r"(0x7fff7fffu) : "memory");
+                        else at_copy16(dst, st > 0 ? base + (unsigned long long) o * 16 : base, st > 0);
+                    }
                 }
             }
             cp_async_commit();
