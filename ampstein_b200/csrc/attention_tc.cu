@@ -25,6 +25,7 @@ __device__ int g_at_status;
 constexpr unsigned AT_SPIN_LIMIT = 1u << 21;   // looks at a barrier before a wait is declared lost (a look lasts up to 4 us)
 constexpr int TA_LOADERS = 3;                  // warps that load keys and values
 constexpr int TA_AHEAD = 2;                    // tiles on their way when the next is requested
+constexpr int TA_POLY = 0;                     // pairs of four whose exponentials are a polynomial's
 constexpr float TA_SLACK = 8.0f;               // powers of two that a row's maximum may grow before O is scaled again
 
 __device__ __forceinline__ bool ta_wait(uint32_t bar, uint32_t parity)
@@ -103,6 +104,11 @@ __device__ __forceinline__ void ta_st32(uint32_t addr, const uint32_t* r)
                  "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
                  :: "r"(addr), TA_W8(r, 0), TA_W8(r, 8), TA_W8(r, 16), TA_W8(r, 24) : "memory");
 }
+__device__ __forceinline__ void ta_st16(uint32_t addr, const uint32_t* r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 :: "r"(addr), TA_W8(r, 0), TA_W8(r, 8) : "memory");
+}
 #undef TA_R8
 #undef TA_W8
 
@@ -111,6 +117,28 @@ __device__ __forceinline__ void ta_wait_st() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ void ta_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void ta_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void ta_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 2^y of two values without the exponential unit, which has 16 results a clock for the SM and would be busy as long as the tensor
+// cores: y = i + f with i the nearest whole number, 2^f on [-1/2, 1/2] by a polynomial of degree 5 (minimax in the relative error, by
+// Remez exchange: 7.5e-8), 2^i through the exponent field. Below 2^-126.5: 0 (the field is 0); a NaN stays one. y <= 127.
+__device__ __forceinline__ float2 ta_exp2_pair(f32x2 y2)
+{
+    float2 y = unpack_f32x2(y2);
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(y.x));      // -127
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(y.y));
+    y2 = pack_f32x2(y.x, y.y);
+    constexpr float MAGIC = 12582912.0f + 127.0f;            // 1.5 2^23: the sum's last bits are i + 127
+    const f32x2 t = add_f32x2(y2, pack_f32x2(MAGIC, MAGIC));
+    const f32x2 f = fma_f32x2(add_f32x2(t, pack_f32x2(-MAGIC, -MAGIC)), pack_f32x2(-1.0f, -1.0f), y2);
+    f32x2 p = pack_f32x2(0x1.5c08e6p-10f, 0x1.5c08e6p-10f);
+    p = fma_f32x2(p, f, pack_f32x2(0x1.3d0c52p-7f, 0x1.3d0c52p-7f));
+    p = fma_f32x2(p, f, pack_f32x2(0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f));
+    p = fma_f32x2(p, f, pack_f32x2(0x1.ebf918p-3f, 0x1.ebf918p-3f));
+    p = fma_f32x2(p, f, pack_f32x2(0x1.62e428p-1f, 0x1.62e428p-1f));
+    p = fma_f32x2(p, f, pack_f32x2(0x1.000002p+0f, 0x1.000002p+0f));
+    const float2 u = unpack_f32x2(t);
+    return unpack_f32x2(mul_f32x2(p, pack_f32x2(__uint_as_float(__float_as_uint(u.x) << 23), __uint_as_float(__float_as_uint(u.y) << 23))));
+}
 
 // Sequence and row tile of the x-th tile of the call; false: there is none. By one warp.
 template <int NQ>
@@ -158,7 +186,7 @@ void attention_tc_kernel(const TaPlan S)
     constexpr int S_STEP = NQ == 2 ? 128 : KB;
     constexpr uint32_t IDESC_QK = ta_idesc(KB, BF, false), IDESC_PV = ta_idesc(D, BF, true);
     extern __shared__ __align__(1024) unsigned char ta_mem[];
-    __shared__ uint64_t q_full, kv_full[ST], kv_free[ST], s_full[2], p_full[2], o_full, end;
+    __shared__ uint64_t q_full, kv_full[ST], kv_free[ST], s_full[2], p_full[4], o_full, end;
     __shared__ uint32_t s_tmem;
     __shared__ int s_place[3];
 
@@ -178,7 +206,8 @@ void attention_tc_kernel(const TaPlan S)
     {
         mbar_init(&q_full, 128 * NQ);
         for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], TA_LOADERS); mbar_init(&kv_free[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); }
+        for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 128);
         mbar_init(&o_full, 1);
         mbar_init(&end, 1);
         fence_mbar_init();
@@ -261,28 +290,40 @@ void attention_tc_kernel(const TaPlan S)
             ta_fence_after();
             const uint32_t s_t = lane_base + buf * S_STEP;
             uint32_t s[KB];
-            #pragma unroll
-            for (int c = 0; c < KB; c += 32) ta_ld32(s_t + c, s + c);
-            ta_wait_ld();
             const int k0 = (j0 + j) * KB;
-            if (k0 < from || k0 + KB > to)
+            const bool look = k0 < from || k0 + KB > to;
+            float top4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
+            #pragma unroll
+            for (int c = 0; c < KB / 2; c += 32) ta_ld32(s_t + c, s + c);
+            ta_wait_ld();
+            #pragma unroll
+            for (int half = 0; half < 2; ++half)
             {
-                #pragma unroll
-                for (int c = 0; c < KB; ++c)
+                // (the second half is on its way while the first one's maximum is taken)
+                if (half == 0)
                 {
-                    const int at = k0 + c;
-                    const bool see = at < n0 || (uint32_t) (at - c1) <= (uint32_t) len;
-                    s[c] = see ? s[c] : 0xff800000u;
+                    #pragma unroll
+                    for (int c = KB / 2; c < KB; c += 32) ta_ld32(s_t + c, s + c);
+                }
+                else ta_wait_ld();
+                if (look)
+                {
+                    #pragma unroll
+                    for (int c = half * (KB / 2); c < (half + 1) * (KB / 2); ++c)
+                    {
+                        const int at = k0 + c;
+                        const bool see = at < n0 || (uint32_t) (at - c1) <= (uint32_t) len;
+                        s[c] = see ? s[c] : 0xff800000u;
+                    }
+                }
+                #pragma unroll
+                for (int c = half * (KB / 2); c < (half + 1) * (KB / 2); c += 8)
+                {
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) top4[e] = fmaxf(fmaxf(top4[e], __uint_as_float(s[c + e])), __uint_as_float(s[c + 4 + e]));
                 }
             }
-            float top = -INFINITY, top2 = -INFINITY;
-            #pragma unroll
-            for (int c = 0; c < KB; c += 4)
-            {
-                top = fmaxf(fmaxf(top, __uint_as_float(s[c])), __uint_as_float(s[c + 1]));
-                top2 = fmaxf(fmaxf(top2, __uint_as_float(s[c + 2])), __uint_as_float(s[c + 3]));
-            }
-            top = fmaxf(top, top2);
+            const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
             const bool move = top > m && (m == -INFINITY || (top - m) * sc > TA_SLACK);
             if (__any_sync(0xffffffffu, move))
             {
@@ -307,22 +348,27 @@ void attention_tc_kernel(const TaPlan S)
             const float base = m == -INFINITY ? 0.0f : -m * sc;
             const f32x2 sc2 = pack_f32x2(sc, sc), base2 = pack_f32x2(base, base);
             #pragma unroll
-            for (int c = 0; c < KB; c += 64)
+            for (int half = 0; half < 2; ++half)
             {
-                uint32_t w[32];
+                // (the MMAs over the first half's keys run while the second half is made)
+                uint32_t w[KB / 4];
                 #pragma unroll
-                for (int e = 0; e < 64; e += 2)
+                for (int e = 0; e < KB / 2; e += 2)
                 {
-                    const float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[c + e]), __uint_as_float(s[c + e + 1])), sc2, base2));
-                    const float e0 = at_exp2(y.x), e1 = at_exp2(y.y);
-                    l2 = add_f32x2(l2, pack_f32x2(e0, e1));
-                    w[e / 2] = AtType<T>::pack(e0, e1);
+                    const int c = half * (KB / 2) + e;
+                    const f32x2 y = fma_f32x2(pack_f32x2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, base2);
+                    float2 x;
+                    if ((e / 2) % 4 < TA_POLY) x = ta_exp2_pair(y);
+                    else { x = unpack_f32x2(y); x.x = at_exp2(x.x); x.y = at_exp2(x.y); }
+                    l2 = add_f32x2(l2, pack_f32x2(x.x, x.y));
+                    w[e / 2] = AtType<T>::pack(x.x, x.y);
                 }
-                ta_st32(s_t + c / 2, w);
+                if constexpr (KB == 128) ta_st32(s_t + half * 32, w);
+                else ta_st16(s_t + half * 16, w);
+                ta_wait_st();
+                ta_fence_before();
+                ta_arrive(pf + 8 * (2 * buf + half));
             }
-            ta_wait_st();
-            ta_fence_before();
-            ta_arrive(pf + 8 * buf);
         }
         const float2 ls = unpack_f32x2(l2);
         l = ls.x + ls.y;
@@ -392,13 +438,13 @@ void attention_tc_kernel(const TaPlan S)
             }
             __syncwarp();
         };
-        auto pv = [&](int buf, int tile, int at, bool first)
+        auto pv = [&](int buf, int tile, int at, int half, bool first)
         {
             const uint64_t b = ta_desc(kv_s + at * KV_BYTES, KB * 128);
             if (ta_elect())
             {
                 #pragma unroll
-                for (int kk = 0; kk < KB / 16; ++kk)
+                for (int kk = half * (KB / 32); kk < (half + 1) * (KB / 32); ++kk)
                     ta_mma_ts(tmem + O_COL + (NQ == 2 ? tile * 128 : 0), tmem + buf * S_STEP + 8 * kk, b + kk * (16 * 128 >> 4), IDESC_PV, !first || kk > 0);
             }
             __syncwarp();
@@ -431,9 +477,14 @@ void attention_tc_kernel(const TaPlan S)
                 for (int i = 0; i < NQ; ++i)
                 {
                     const int buf = NQ == 2 ? i : (j & 1);
-                    if (!wait(pf + 8 * buf, (NQ == 2 ? j : j >> 1) & 1)) break;
-                    ta_fence_after();
-                    pv(buf, i, vst, j == 0);
+                    #pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                    {
+                        if (!wait(pf + 8 * (2 * buf + half), (NQ == 2 ? j : j >> 1) & 1)) break;
+                        ta_fence_after();
+                        pv(buf, i, vst, half, j == 0);
+                    }
+                    if (!ok) break;
                     if (i == NQ - 1) commit(free_s + 8 * vst);
                     if constexpr (NQ == 1) commit(smem_u32(&o_full));
                     else if (j + 1 < n)
@@ -453,43 +504,47 @@ void attention_tc_kernel(const TaPlan S)
     {
         // ---- keys and values, three warps: warp w makes every third of the copies of 32 x 16 bytes that a tile takes ---------------
         constexpr int PER = CH >= 32 ? 1 : 32 / CH, COPIES = KB / PER, MINE = (COPIES + TA_LOADERS - 1) / TA_LOADERS, LOOKS = (MINE * PER + 31) / 32;
-        const int w = warp - 4 * NQ - 1, tiles = 2 * n, r_lane = CH >= 32 ? 0 : lane / CH, c_lane = lane % CH, count = keys.count();
+        const int w = warp - 4 * NQ - 1, r_lane = CH >= 32 ? 0 : lane / CH, c_lane = lane % CH, count = keys.count();
         const unsigned char* const k_base = reinterpret_cast<const unsigned char*>(P.k_cache) + h * P.k_head * 2 + c_lane * 16;
         const unsigned char* const v_base = reinterpret_cast<const unsigned char*>(P.v_cache) + h * P.v_head * 2 + c_lane * 16;
         const int* const table = P.table + (long long) s_place[1] * P.table_row;
-        int issued = 0;
+        // lane l looks up the l-th, (l + 32)-th ... of the warp's rows: page and row in it
+        struct Rows { int page[LOOKS], row[LOOKS]; };        // (row -1: behind the last key, -2: no row of this warp)
+        auto look_up = [&](int j, Rows& x)
+        {
+            #pragma unroll
+            for (int g = 0; g < LOOKS; ++g)
+            {
+                const int q = lane + 32 * g, r = (w + TA_LOADERS * (q / PER)) * PER + q % PER, c = (j0 + j) * KB + r;
+                x.page[g] = -1;
+                x.row[g] = q < MINE * PER && r < KB ? (c < count ? 0 : -1) : -2;
+                if (x.row[g] == 0)
+                {
+                    const int key = keys.key(c), pg = S.g.page_of(key);
+                    x.page[g] = table[pg];
+                    x.row[g] = key - pg * P.page_size;
+                }
+            }
+        };
+        int issued = 0, stage = 0;
         auto hand_over = [&](int tile)
         {
             ta_fence_async();
             __syncwarp();
             if (lane == 0) ta_arrive(full_s + 8 * (tile % ST));
         };
-        #pragma unroll 1
-        for (; issued < tiles; ++issued)
+        auto copy_tile = [&](const Rows& x, bool is_v)
         {
-            // tile 0 is K0, then K1, V0, K2, V1, ..., the last one V(n - 1)
-            const bool is_v = issued > 0 && (issued % 2 == 0 || issued == tiles - 1);
-            const int j = issued == 0 ? 0 : issued == tiles - 1 ? n - 1 : is_v ? issued / 2 - 1 : (issued + 1) / 2;
-            // lane l looks up the l-th, (l + 32)-th ... of the warp's rows: offsets in pieces of 16 bytes
-            uint32_t off[LOOKS];
-            uint32_t have = 0xffffffffu;                     // lanes whose rows are all there
+            uint32_t off[LOOKS], have = 0xffffffffu;         // offsets in pieces of 16 bytes; lanes whose rows are all there
             int state[LOOKS];                                // 1: there, 0: behind the last key, -1: on a page outside the pool
             #pragma unroll
             for (int g = 0; g < LOOKS; ++g)
             {
-                const int q = lane + 32 * g, r = (w + TA_LOADERS * (q / PER)) * PER + q % PER, c = (j0 + j) * KB + r;
-                off[g] = 0; state[g] = q < MINE * PER && r < KB ? 0 : 1;
-                if (state[g] == 0 && c < count)
-                {
-                    const int key = keys.key(c), pg = S.g.page_of(key), page = table[pg], row = key - pg * P.page_size;
-                    state[g] = (unsigned) page < (unsigned) P.pages ? 1 : -1;
-                    off[g] = is_v ? page * S.g.v_page + row * S.g.v_row : page * S.g.k_page + row * S.g.k_row;
-                }
+                state[g] = x.row[g] == -2 ? 1 : x.row[g] == -1 ? 0 : (unsigned) x.page[g] < (unsigned) P.pages ? 1 : -1;
+                off[g] = x.row[g] < 0 || state[g] < 0 ? 0 : is_v ? x.page[g] * S.g.v_page + x.row[g] * S.g.v_row : x.page[g] * S.g.k_page + x.row[g] * S.g.k_row;
                 have &= __ballot_sync(0xffffffffu, state[g] > 0);
             }
-            const int stage = issued % ST;
-            if (issued >= ST) wait(free_s + 8 * stage, (issued / ST - 1) & 1);
-            if (!ok) break;
+            if (issued >= ST && !wait(free_s + 8 * stage, (issued / ST - 1) & 1)) return;
             const unsigned char* const base = is_v ? v_base : k_base;
             const uint32_t to = kv_s + stage * KV_BYTES + (c_lane >> 3) * (KB * 128);
             if (have == 0xffffffffu)
@@ -505,7 +560,7 @@ void attention_tc_kernel(const TaPlan S)
             }
             else
             {
-                #pragma unroll 4
+                #pragma unroll 1
                 for (int i = 0; i < MINE; ++i)
                 {
                     const int r = (w + TA_LOADERS * i) * PER + r_lane, from = (i * PER) % 32 + r_lane;
@@ -514,9 +569,9 @@ void attention_tc_kernel(const TaPlan S)
                     #pragma unroll
                     for (int g = 0; g < LOOKS; ++g)
                     {
-                        const uint32_t x = __shfl_sync(0xffffffffu, off[g], from);
-                        const int y = __shfl_sync(0xffffffffu, state[g], from);
-                        if (g == i * PER / 32) { o = x; st = y; }
+                        const uint32_t y = __shfl_sync(0xffffffffu, off[g], from);
+                        const int z = __shfl_sync(0xffffffffu, state[g], from);
+                        if (g == i * PER / 32) { o = y; st = z; }
                     }
                     const uint32_t dst = to + r * 128 + (((c_lane & 7) ^ (r & 7)) << 4);
                     if (w + TA_LOADERS * i < COPIES)
@@ -529,6 +584,26 @@ void attention_tc_kernel(const TaPlan S)
             }
             cp_async_commit();
             if (issued >= TA_AHEAD) { asm volatile("cp.async.wait_group %0;" :: "n"(TA_AHEAD) : "memory"); hand_over(issued - TA_AHEAD); }
+            ++issued;
+            stage = stage + 1 == ST ? 0 : stage + 1;
+        };
+        // K0, then K1, V0, K2, V1, ...: a tile's rows are looked up two tiles ahead, and kept from its keys to its values
+        Rows now, next, then;
+        if (n > 0)
+        {
+            look_up(0, now);
+            if (n > 1) look_up(1, next);
+            copy_tile(now, false);
+            #pragma unroll 1
+            for (int j = 0; j < n && ok; ++j)
+            {
+                if (j + 1 < n) copy_tile(next, false);
+                if (!ok) break;
+                if (j + 2 < n) look_up(j + 2, then);
+                copy_tile(now, true);
+                now = next;
+                next = then;
+            }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         if (ok) for (int tile = max(0, issued - TA_AHEAD); tile < issued; ++tile) hand_over(tile);
