@@ -701,19 +701,19 @@ struct AtCut
 {
     bool split, tc;                            // forms that are launched
     int whole, grid, wr;                       // split form: 16 * wr rows per row tile
-    int tiles, slices;                         // prompt form
+    int nq, tiles, slices;                     // prompt form
     size_t tc_offset, bytes;                   // of the workspace
 };
 
 // Slices of the keys of each of `items` row tiles, `kt` key tiles long at most: waves of CTAs, each its share of the key tiles and a
 // set-up of about two, and a join worth four
-static int ta_slices(long items, long kt, int sms)
+static int ta_slices(long items, long kt, int places)
 {
     int best = 1;
     double cost = 1e30;
-    for (int s = 1; s <= kt && s * items <= 4l * sms && s <= 256; ++s)
+    for (int s = 1; s <= kt && s * items <= 4l * places && s <= 256; ++s)
     {
-        const double c = (double) ((items * s + sms - 1) / sms) * ((double) ((kt + s - 1) / s) + 2) + (s > 1 ? 4 : 0);
+        const double c = (double) ((items * s + places - 1) / places) * ((double) ((kt + s - 1) / s) + 2) + (s > 1 ? 4 : 0);
         if (c < cost * 0.97) { cost = c; best = s; }
     }
     return best;
@@ -734,11 +734,17 @@ static AtCut at_cut(int tokens, int seqs, int heads, int kv_heads, int dim, bool
     C.slices = 1;
     if (C.tc)
     {
-        const int tile = ta_rows(dim), kb = dim <= 128 ? 128 : 64;
+        // One row tile per CTA and two CTAs per SM where a tile has few keys: set-up and ends of one run under the other's keys. Two row tiles
+        // per CTA share every key otherwise (us, one tile / two; 4 query heads per key-value head at 128 values, 8 at 64: windows of 128,
+        // 512, 1024, 2048 keys 34.0 / 52.4, 52.6 / 69.6, 76.7 / 91.3, 93.2 / 91.8 at 128; 45.5 / 64.1, 75.1 / 85.3, 113 / 113, 153 / 136 at 64;
+        // a prompt of 2048 tokens 53.6 / 56.6 and 88 / 79, of 8192 567 / 509 and 1017 / 747)
+        const long few = dim == 128 ? 1536 : 768;
+        C.nq = dim == 256 || (window ? min(max_keys, (long) window + sinks + 128 / group) : max_keys) <= few ? 1 : 2;
+        const int tile = 128 * C.nq, kb = 64 * C.nq;
         C.tiles = (int) (ragged ? all / tile + min((long) seqs, all / (AT_SPLIT_ROWS + 1)) : seqs * ((each + tile - 1) / tile));
         const long keys = window ? min(max_keys, (long) window + sinks + tile / group + 1) : max_keys;
-        C.slices = ta_slices((long) C.tiles * kv_heads, (keys + kb - 1) / kb, sms);
-        if (C.slices > 1) C.bytes += (size_t) C.tiles * kv_heads * C.slices * ta_part_floats(dim) * 4;
+        C.slices = ta_slices((long) C.tiles * kv_heads, (keys + kb - 1) / kb, C.nq == 1 && dim <= 128 ? 2 * sms : sms);
+        if (C.slices > 1) C.bytes += (size_t) C.tiles * kv_heads * C.slices * ta_part_floats(tile, dim) * 4;
     }
     return C;
 }
@@ -841,7 +847,7 @@ AMP_API int amp_b200_attention(const amp_attention_args* args, cudaStream_t stre
     }
     if (!C.tc) return 0;
     TaPlan A;
-    A.P = P; A.tiles = C.tiles; A.slices = C.slices; A.split_rows = P.cu ? AT_SPLIT_ROWS : 0; A.pdl = g_pdl;
+    A.P = P; A.nq = C.nq; A.tiles = C.tiles; A.slices = C.slices; A.split_rows = P.cu ? AT_SPLIT_ROWS : 0; A.pdl = g_pdl;
     A.scale2 = P.scale * 1.4426950408889634f; A.part_offset = C.tc_offset; A.g = g;
     return attention_tc(A, stream);
 }

@@ -25,7 +25,7 @@ __device__ int g_at_status;
 constexpr unsigned AT_SPIN_LIMIT = 1u << 21;   // looks at a barrier before a wait is declared lost (a look lasts up to 4 us)
 constexpr int TA_LOADERS = 3;                  // warps that load keys and values
 constexpr int TA_AHEAD = 2;                    // tiles on their way when the next is requested
-constexpr int TA_POLY = 0;                     // pairs of four whose exponentials are a polynomial's
+template <int D> constexpr int ta_poly = D == 64 ? 1 : 0;     // pairs of four whose exponentials are a polynomial's
 constexpr float TA_SLACK = 8.0f;               // powers of two that a row's maximum may grow before O is scaled again
 
 __device__ __forceinline__ bool ta_wait(uint32_t bar, uint32_t parity)
@@ -104,6 +104,12 @@ __device__ __forceinline__ void ta_st32(uint32_t addr, const uint32_t* r)
                  "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
                  :: "r"(addr), TA_W8(r, 0), TA_W8(r, 8), TA_W8(r, 16), TA_W8(r, 24) : "memory");
 }
+__device__ __forceinline__ void ta_ld16(uint32_t addr, uint32_t* r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : TA_R8(r, 0), TA_R8(r, 8) : "r"(addr) : "memory");
+}
+
 __device__ __forceinline__ void ta_st16(uint32_t addr, const uint32_t* r)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
@@ -174,19 +180,20 @@ __device__ __forceinline__ bool ta_find(const TaPlan& S, int x, int& b, int& til
     return false;
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(ta_threads<D>, 1)
+template <typename T, int D, int NQ>
+__global__ __launch_bounds__(ta_threads<NQ>, (ta_ctas<D, NQ>))
 void attention_tc_kernel(const TaPlan S)
 {
     const amp_attention_args& P = S.P;
-    constexpr int NQ = ta_nq<D>, KB = ta_kb<D>, ST = ta_stages<D>, ROWS = NQ * 128;
+    constexpr int KB = ta_kb<NQ>, ST = ta_stages<D, NQ>, ROWS = ta_rows<NQ>;
     constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = KB * D * 2, CH = D / 8;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
-    constexpr int O_COL = 256;                 // tensor memory: S at 0 (two tiles or two buffers), O at 256
-    constexpr int S_STEP = NQ == 2 ? 128 : KB;
+    // tensor memory: S (two tiles or two buffers), then O
+    constexpr int S_STEP = KB, O_COL = 2 * KB, TMEM = O_COL + NQ * (NQ == 2 ? 128 : D) <= 256 ? 256 : 512;
+    static_assert(O_COL + (NQ == 2 ? 128 + D : D) <= TMEM && TMEM * ta_ctas<D, NQ> <= 512, "tensor memory");
     constexpr uint32_t IDESC_QK = ta_idesc(KB, BF, false), IDESC_PV = ta_idesc(D, BF, true);
     extern __shared__ __align__(1024) unsigned char ta_mem[];
-    __shared__ uint64_t q_full, kv_full[ST], kv_free[ST], s_full[2], p_full[4], o_full, end;
+    __shared__ uint64_t q_full, kv_full[ST], kv_free[ST], s_full[2], p_full[4], pv_done, o_full, end;
     __shared__ uint32_t s_tmem;
     __shared__ int s_place[3];
 
@@ -208,6 +215,7 @@ void attention_tc_kernel(const TaPlan S)
         for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], TA_LOADERS); mbar_init(&kv_free[i], 1); }
         for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
         for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 128);
+        mbar_init(&pv_done, 1);
         mbar_init(&o_full, 1);
         mbar_init(&end, 1);
         fence_mbar_init();
@@ -225,7 +233,7 @@ void attention_tc_kernel(const TaPlan S)
 
     if (warp == 4 * NQ)
     {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&s_tmem)), "r"((uint32_t) TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     ta_fence_before();
@@ -332,16 +340,20 @@ void attention_tc_kernel(const TaPlan S)
                 l2 = mul_f32x2(l2, pack_f32x2(f, f));
                 if (j > 0)
                 {
-                    if constexpr (NQ == 1) { if (!wait(smem_u32(&o_full), (j - 1) & 1)) break; ta_fence_after(); }
+                    constexpr int PIECE = NQ == 2 ? 32 : 16;             // columns at a time: 16 where two CTAs share the registers
+                    // (one tile: S(j) was made before P V(j - 1), behind P V(j - 2): the phase is this one or the one in front)
+                    if constexpr (NQ == 1) { if (!wait(smem_u32(&pv_done), (j - 1) & 1)) break; ta_fence_after(); }
                     #pragma unroll
-                    for (int c = 0; c < D; c += 32)
+                    for (int c = 0; c < D; c += PIECE)
                     {
-                        uint32_t o[32];
-                        ta_ld32(o_t + c, o);
+                        uint32_t o[PIECE];
+                        if constexpr (PIECE == 32) ta_ld32(o_t + c, o);
+                        else ta_ld16(o_t + c, o);
                         ta_wait_ld();
                         #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        ta_st32(o_t + c, o);
+                        for (int e = 0; e < PIECE; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        if constexpr (PIECE == 32) ta_st32(o_t + c, o);
+                        else ta_st16(o_t + c, o);
                     }
                 }
             }
@@ -358,7 +370,7 @@ void attention_tc_kernel(const TaPlan S)
                     const int c = half * (KB / 2) + e;
                     const f32x2 y = fma_f32x2(pack_f32x2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, base2);
                     float2 x;
-                    if ((e / 2) % 4 < TA_POLY) x = ta_exp2_pair(y);
+                    if ((e / 2) % 4 < ta_poly<D>) x = ta_exp2_pair(y);
                     else { x = unpack_f32x2(y); x.x = at_exp2(x.x); x.y = at_exp2(x.y); }
                     l2 = add_f32x2(l2, pack_f32x2(x.x, x.y));
                     w[e / 2] = AtType<T>::pack(x.x, x.y);
@@ -374,7 +386,7 @@ void attention_tc_kernel(const TaPlan S)
         l = ls.x + ls.y;
         if (n > 0 && ok)
         {
-            wait(smem_u32(&o_full), NQ == 2 ? 0 : (n - 1) & 1);
+            wait(smem_u32(&o_full), 0);
             ta_fence_after();
         }
         const float m2 = m == -INFINITY ? m : m * sc;
@@ -382,7 +394,7 @@ void attention_tc_kernel(const TaPlan S)
         {
             // a part: rows side by side, so that a warp writes whole lines; lost: NaN
             float* const part = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(P.workspace) + S.part_offset)
-                                + (size_t) ((x * P.kv_heads + h) * S.slices + slice) * ta_part_floats(D);
+                                + (size_t) ((x * P.kv_heads + h) * S.slices + slice) * ta_part_floats(ROWS, D);
             if (n > 0)
             {
                 #pragma unroll
@@ -486,7 +498,7 @@ void attention_tc_kernel(const TaPlan S)
                     }
                     if (!ok) break;
                     if (i == NQ - 1) commit(free_s + 8 * vst);
-                    if constexpr (NQ == 1) commit(smem_u32(&o_full));
+                    if constexpr (NQ == 1) commit(smem_u32(&pv_done));
                     else if (j + 1 < n)
                     {
                         qk(i, i, kst);
@@ -495,7 +507,7 @@ void attention_tc_kernel(const TaPlan S)
                 }
                 if (!ok) break;
             }
-            if (NQ == 2 && ok) commit(smem_u32(&o_full));
+            if (ok) commit(smem_u32(&o_full));
         }
         commit(smem_u32(&end));
         ta_wait(smem_u32(&end), 0);            // (bounded; the accumulators are given back only then)
@@ -613,17 +625,17 @@ void attention_tc_kernel(const TaPlan S)
     if (warp == 4 * NQ)
     {
         ta_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((uint32_t) TMEM) : "memory");
     }
 }
 
 // Joins the slices of row tile x of key-value head h (blockIdx.x), 16 values of every row (blockIdx.y)
-template <typename T, int D>
-__global__ __launch_bounds__(128 * ta_nq<D>)
+template <typename T, int D, int NQ>
+__global__ __launch_bounds__(128 * NQ)
 void attention_tc_join_kernel(const TaPlan S)
 {
     const amp_attention_args& P = S.P;
-    constexpr int NQ = ta_nq<D>, ROWS = 128 * NQ;
+    constexpr int ROWS = ta_rows<NQ>;
     __shared__ int s_place[3];
     if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
     const int t = threadIdx.x, h = blockIdx.x % P.kv_heads, x = blockIdx.x / P.kv_heads, group = P.heads / P.kv_heads;
@@ -639,8 +651,8 @@ void attention_tc_join_kernel(const TaPlan S)
     const int row = s_place[2] * ROWS + t, tok = row / group;
     if (tok >= seq.count) return;
     const float* const parts = reinterpret_cast<const float*>(reinterpret_cast<const unsigned char*>(P.workspace) + S.part_offset)
-                               + (size_t) blockIdx.x * S.slices * ta_part_floats(D);
-    auto ml = [&](int i) { return reinterpret_cast<const float2*>(parts + i * ta_part_floats(D) + ROWS * D)[t]; };
+                               + (size_t) blockIdx.x * S.slices * ta_part_floats(ROWS, D);
+    auto ml = [&](int i) { return reinterpret_cast<const float2*>(parts + i * ta_part_floats(ROWS, D) + ROWS * D)[t]; };
     float m = -INFINITY, l = 0.0f;
     for (int i = 0; i < S.slices; ++i) m = fmaxf(m, ml(i).x);
     const float base = m == -INFINITY ? 0.0f : m;
@@ -654,7 +666,7 @@ void attention_tc_join_kernel(const TaPlan S)
         if (v.y == 0.0f) continue;             // (a slice without keys wrote nothing else)
         const float f = at_exp2(v.x - base);
         l += v.y != v.y ? v.y : v.y * f;
-        const float4* p = reinterpret_cast<const float4*>(parts + i * ta_part_floats(D)) + (size_t) blockIdx.y * 4 * ROWS + t;
+        const float4* p = reinterpret_cast<const float4*>(parts + i * ta_part_floats(ROWS, D)) + (size_t) blockIdx.y * 4 * ROWS + t;
         #pragma unroll
         for (int c = 0; c < 4; ++c)
         {
@@ -667,37 +679,43 @@ void attention_tc_join_kernel(const TaPlan S)
     at_store8<T>(P, seq, tok, head, blockIdx.y * 16 + 8, o[2], o[3], m, l);
 }
 
-template <typename T, int D>
+template <typename T, int D, int NQ>
 static int ta_launch(const TaPlan& S, cudaStream_t stream)
 {
     const amp_attention_args& P = S.P;
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return cuda_rc(e, "attention device");
-    if (cudaError_t e = ensure_smem(attention_tc_kernel<T, D>, ta_smem<D>, dev)) return cuda_rc(e, "attention shared memory");
+    if (cudaError_t e = ensure_smem(attention_tc_kernel<T, D, NQ>, ta_smem<D, NQ>, dev)) return cuda_rc(e, "attention shared memory");
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(S.tiles * S.slices * P.kv_heads, 1, 1);
-    cfg.blockDim = dim3(ta_threads<D>, 1, 1);
-    cfg.dynamicSmemBytes = ta_smem<D>;
+    cfg.blockDim = dim3(ta_threads<NQ>, 1, 1);
+    cfg.dynamicSmemBytes = ta_smem<D, NQ>;
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = S.pdl ? 1 : 0;
-    if (cudaError_t e = cudaLaunchKernelEx(&cfg, attention_tc_kernel<T, D>, S)) return cuda_rc(e, "attention launch");
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, attention_tc_kernel<T, D, NQ>, S)) return cuda_rc(e, "attention launch");
     if (S.slices == 1) return 0;
     cfg.gridDim = dim3(S.tiles * P.kv_heads, D / 16, 1);
-    cfg.blockDim = dim3(128 * ta_nq<D>, 1, 1);
+    cfg.blockDim = dim3(128 * NQ, 1, 1);
     cfg.dynamicSmemBytes = 0;
-    return cuda_rc(cudaLaunchKernelEx(&cfg, attention_tc_join_kernel<T, D>, S), "attention join launch");
+    return cuda_rc(cudaLaunchKernelEx(&cfg, attention_tc_join_kernel<T, D, NQ>, S), "attention join launch");
+}
+
+template <typename T>
+static int ta_launch_dim(const TaPlan& S, cudaStream_t stream)
+{
+    if (S.P.dim == 256) return ta_launch<T, 256, 1>(S, stream);
+    if (S.P.dim == 128) return S.nq == 1 ? ta_launch<T, 128, 1>(S, stream) : ta_launch<T, 128, 2>(S, stream);
+    return S.nq == 1 ? ta_launch<T, 64, 1>(S, stream) : ta_launch<T, 64, 2>(S, stream);
 }
 
 int attention_tc(const TaPlan& S, cudaStream_t stream)
 {
     if (S.tiles == 0) return 0;
-    const int d = S.P.dim;
-    if (S.P.bf16) return d == 64 ? ta_launch<__nv_bfloat16, 64>(S, stream) : d == 128 ? ta_launch<__nv_bfloat16, 128>(S, stream) : ta_launch<__nv_bfloat16, 256>(S, stream);
-    return d == 64 ? ta_launch<__half, 64>(S, stream) : d == 128 ? ta_launch<__half, 128>(S, stream) : ta_launch<__half, 256>(S, stream);
+    return S.P.bf16 ? ta_launch_dim<__nv_bfloat16>(S, stream) : ta_launch_dim<__half>(S, stream);
 }
 
 }  // namespace amp

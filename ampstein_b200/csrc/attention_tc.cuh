@@ -4,19 +4,21 @@
 
 namespace amp {
 
-template <int D> constexpr int ta_nq = D <= 128 ? 2 : 1;       // tiles of 128 rows per CTA
-template <int D> constexpr int ta_kb = D <= 128 ? 128 : 64;    // keys per tile
-template <int D> constexpr int ta_stages = D == 64 ? 8 : 5;    // tiles of keys or values in shared memory
-template <int D> constexpr int ta_threads = 128 * (ta_nq<D> + 1);
-template <int D> constexpr int ta_smem = ta_nq<D> * 128 * D * 2 + ta_stages<D> * ta_kb<D> * D * 2;
+// A CTA has NQ tiles of 128 rows: two, one CTA per SM, or one; then two CTAs share an SM, up to 128 values per head
+template <int NQ> constexpr int ta_rows = 128 * NQ;
+template <int NQ> constexpr int ta_kb = 64 * NQ;               // keys per tile
+template <int NQ> constexpr int ta_threads = 128 * (NQ + 1);
+template <int D, int NQ> constexpr int ta_ctas = NQ == 1 && D <= 128 ? 2 : 1;
+template <int D, int NQ> constexpr int ta_stages = D == 64 && NQ == 2 ? 8 : 5;         // tiles of keys or values in shared memory
+template <int D, int NQ> constexpr int ta_smem = ta_rows<NQ> * D * 2 + ta_stages<D, NQ> * ta_kb<NQ> * D * 2;
 
-// Tiles of rows that cover `rows` rows; floats of a part (one slice of one tile)
-__host__ __device__ constexpr int ta_rows(int dim) { return dim <= 128 ? 256 : 128; }
-__host__ __device__ constexpr size_t ta_part_floats(int dim) { return (size_t) ta_rows(dim) * (dim + 2); }
+// floats of a part (one slice of one tile)
+__host__ __device__ constexpr size_t ta_part_floats(int rows, int dim) { return (size_t) rows * (dim + 2); }
 
 struct TaPlan
 {
     amp_attention_args P;
+    int nq;                                    // row tiles of 128 per CTA
     int tiles;                                 // row tiles per key-value head (an upper bound with cu)
     int slices;                                // of every tile's keys
     int split_rows;                            // sequences of up to so many rows (tokens x group) are the split form's
