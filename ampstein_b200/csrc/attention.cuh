@@ -129,7 +129,7 @@ __device__ __forceinline__ float at_factor(const amp_attention_args& P, int p, f
     return p >= P.max_pages * P.page_size ? NAN : (l == 0.0f ? 0.0f : 1.0f / l);
 }
 
-// Stores four or eight values of a finished row, and with the first of them its lse. m counts in powers of two.
+// Stores four or eight values of a finished row (f: at_factor), and with the first of them its lse. m counts in powers of two.
 template <typename T>
 __device__ __forceinline__ T* at_out(const amp_attention_args& P, const AtSeq& s, int tok, int head, int c, float f, float m, float l)
 {
@@ -146,9 +146,8 @@ __device__ __forceinline__ void at_store(const amp_attention_args& P, const AtSe
 }
 
 template <typename T>
-__device__ __forceinline__ void at_store8(const amp_attention_args& P, const AtSeq& s, int tok, int head, int c, float4 x, float4 y, float m, float l)
+__device__ __forceinline__ void at_store8(const amp_attention_args& P, const AtSeq& s, int tok, int head, int c, float4 x, float4 y, float f, float m, float l)
 {
-    const float f = at_factor(P, s.first + tok, l);
     *reinterpret_cast<uint4*>(at_out<T>(P, s, tok, head, c, f, m, l)) =
         make_uint4(AtType<T>::pack(x.x * f, x.y * f), AtType<T>::pack(x.z * f, x.w * f), AtType<T>::pack(y.x * f, y.y * f), AtType<T>::pack(y.z * f, y.w * f));
 }

@@ -146,24 +146,34 @@ __device__ __forceinline__ float2 ta_exp2_pair(f32x2 y2)
     return unpack_f32x2(mul_f32x2(p, pack_f32x2(__uint_as_float(__float_as_uint(u.x) << 23), __uint_as_float(__float_as_uint(u.y) << 23))));
 }
 
-// Sequence and row tile of the x-th tile of the call; false: there is none. By one warp.
+// Sequence of the x-th row tile of the call, and the tile in it; false: there is none. By one warp.
+struct TaPlace
+{
+    AtSeq s;
+    int have, b, tile;
+};
+
 template <int NQ>
-__device__ __forceinline__ bool ta_find(const TaPlan& S, int x, int& b, int& tile)
+__device__ __forceinline__ TaPlace ta_find(const TaPlan& S, int x)
 {
     const amp_attention_args& P = S.P;
     const int group = P.heads / P.kv_heads, lane = threadIdx.x & 31;
-    auto tiles = [&](int rows) { return rows <= S.split_rows ? 0 : (rows + NQ * 128 - 1) / (NQ * 128); };
+    auto tiles = [&](int rows) { return rows <= S.split_rows ? 0 : (rows + ta_rows<NQ> - 1) / ta_rows<NQ>; };
+    TaPlace f = {};
     if (!P.cu)
     {
         const int each = tiles(P.tokens / P.seqs * group);
-        b = each ? x / each : P.seqs;
-        tile = x - b * each;
-        return b < P.seqs;
+        f.b = each ? x / each : P.seqs;
+        f.tile = x - f.b * each;
+        f.have = f.b < P.seqs;
+        if (f.have) f.s = at_seq(P, f.b);
+        return f;
     }
     for (int b0 = 0; b0 < P.seqs; b0 += 32)
     {
-        int n = 0;
-        if (b0 + lane < P.seqs) n = tiles(at_seq(P, b0 + lane).count * group);
+        AtSeq s = {};
+        if (b0 + lane < P.seqs) s = at_seq(P, b0 + lane);
+        const int n = tiles(s.count * group);
         int sum = n;
         #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += y; }
@@ -171,13 +181,17 @@ __device__ __forceinline__ bool ta_find(const TaPlan& S, int x, int& b, int& til
         if (hit)
         {
             const int l = __ffs(hit) - 1;
-            b = b0 + l;
-            tile = x - (__shfl_sync(0xffffffffu, sum, l) - __shfl_sync(0xffffffffu, n, l));
-            return true;
+            f.have = 1;
+            f.b = b0 + l;
+            f.tile = x - (__shfl_sync(0xffffffffu, sum, l) - __shfl_sync(0xffffffffu, n, l));
+            f.s.first = __shfl_sync(0xffffffffu, s.first, l);
+            f.s.count = __shfl_sync(0xffffffffu, s.count, l);
+            f.s.row0 = __shfl_sync(0xffffffffu, s.row0, l);
+            return f;
         }
         x -= __shfl_sync(0xffffffffu, sum, 31);
     }
-    return false;
+    return f;
 }
 
 template <typename T, int D, int NQ>
@@ -195,21 +209,25 @@ void attention_tc_kernel(const TaPlan S)
     extern __shared__ __align__(1024) unsigned char ta_mem[];
     __shared__ uint64_t q_full, kv_full[ST], kv_free[ST], s_full[2], p_full[4], pv_done, o_full, end;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_place[3];
+    __shared__ TaPlace s_place;
 
     const int t = threadIdx.x, lane = t & 31, warp = __shfl_sync(0xffffffffu, t >> 5, 0);
     const int group = P.heads / P.kv_heads;
-    // (before tensor memory is taken: a CTA in front may still have to take its own here)
+    // (before tensor memory is taken: a CTA in front may still have to take its own here; those behind are let in when it is taken)
     if (S.pdl) pdl_wait();
     const int h = blockIdx.x % P.kv_heads, slice = blockIdx.x / P.kv_heads % S.slices;
     const int x = S.tiles - 1 - (int) (blockIdx.x / P.kv_heads / S.slices);      // (the last tiles see most keys: first)
     if (warp == 0)
     {
-        int b = 0, tile = 0;
-        const bool have = ta_find<NQ>(S, x, b, tile);
-        if (lane == 0) { s_place[0] = have; s_place[1] = b; s_place[2] = tile; }
+        const TaPlace f = ta_find<NQ>(S, x);
+        if (lane == 0) s_place = f;
     }
-    if (t == 0)
+    else if (warp == 4 * NQ)
+    {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&s_tmem)), "r"((uint32_t) TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    else if (warp == 1 && lane == 0)
     {
         mbar_init(&q_full, 128 * NQ);
         for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], TA_LOADERS); mbar_init(&kv_free[i], 1); }
@@ -220,27 +238,24 @@ void attention_tc_kernel(const TaPlan S)
         mbar_init(&end, 1);
         fence_mbar_init();
     }
+    ta_fence_before();
     __syncthreads();
-    if (!s_place[0]) { if (S.pdl) pdl_launch_dependents(); return; }
-    const AtSeq seq = at_seq(P, s_place[1]);
-    const int row0 = s_place[2] * ROWS, tok0 = row0 / group, tok1 = min((row0 + ROWS - 1) / group, seq.count - 1);
+    ta_fence_after();
+    const uint32_t tmem = s_tmem;
+    if (S.pdl) pdl_launch_dependents();
+    if (!s_place.have)
+    {
+        if (warp == 4 * NQ) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((uint32_t) TMEM) : "memory");
+        return;
+    }
+    const AtSeq seq = s_place.s;
+    const int row0 = s_place.tile * ROWS, tok0 = row0 / group, tok1 = min((row0 + ROWS - 1) / group, seq.count - 1);
     const AtKeys keys = at_keys(P, seq.first + tok0, tok1 - tok0 + 1);
     const int n_all = (keys.count() + KB - 1) / KB;
     const int j0 = (int) ((long long) n_all * slice / S.slices), n = (int) ((long long) n_all * (slice + 1) / S.slices) - j0;
     const uint32_t q_s = smem_u32(ta_mem), kv_s = q_s + NQ * Q_BYTES;
     const uint32_t full_s = smem_u32(&kv_full[0]), free_s = smem_u32(&kv_free[0]), sf = smem_u32(&s_full[0]), pf = smem_u32(&p_full[0]);
     const bool aligned = (q_s & 1023) == 0;    // (the swizzle needs the alignment that the declaration asks for)
-
-    if (warp == 4 * NQ)
-    {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&s_tmem)), "r"((uint32_t) TMEM) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    ta_fence_before();
-    __syncthreads();
-    ta_fence_after();
-    const uint32_t tmem = s_tmem;
-    if (S.pdl) pdl_launch_dependents();
 
     bool ok = aligned;
     if (!aligned && t == 0) atomicExch(&g_at_status, 2);
@@ -415,6 +430,7 @@ void attention_tc_kernel(const TaPlan S)
         }
         else if (ok)
         {
+            const float f = at_factor(P, p, l);
             #pragma unroll
             for (int c = 0; c < D; c += 32)
             {
@@ -427,7 +443,7 @@ void attention_tc_kernel(const TaPlan S)
                     {
                         const float4 a = n > 0 ? make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])) : make_float4(0, 0, 0, 0);
                         const float4 b = n > 0 ? make_float4(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]), __uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])) : make_float4(0, 0, 0, 0);
-                        at_store8<T>(P, seq, tok, head, c + e, a, b, m2, l);
+                        at_store8<T>(P, seq, tok, head, c + e, a, b, f, m2, l);
                     }
                 }
             }
@@ -519,7 +535,7 @@ void attention_tc_kernel(const TaPlan S)
         const int w = warp - 4 * NQ - 1, r_lane = CH >= 32 ? 0 : lane / CH, c_lane = lane % CH, count = keys.count();
         const unsigned char* const k_base = reinterpret_cast<const unsigned char*>(P.k_cache) + h * P.k_head * 2 + c_lane * 16;
         const unsigned char* const v_base = reinterpret_cast<const unsigned char*>(P.v_cache) + h * P.v_head * 2 + c_lane * 16;
-        const int* const table = P.table + (long long) s_place[1] * P.table_row;
+        const int* const table = P.table + (long long) s_place.b * P.table_row;
         // lane l looks up the l-th, (l + 32)-th ... of the warp's rows: page and row in it
         struct Rows { int page[LOOKS], row[LOOKS]; };        // (row -1: behind the last key, -2: no row of this warp)
         auto look_up = [&](int j, Rows& x)
@@ -636,19 +652,18 @@ void attention_tc_join_kernel(const TaPlan S)
 {
     const amp_attention_args& P = S.P;
     constexpr int ROWS = ta_rows<NQ>;
-    __shared__ int s_place[3];
-    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
+    __shared__ TaPlace s_place;
     const int t = threadIdx.x, h = blockIdx.x % P.kv_heads, x = blockIdx.x / P.kv_heads, group = P.heads / P.kv_heads;
     if (t < 32)
     {
-        int b = 0, tile = 0;
-        const bool have = ta_find<NQ>(S, x, b, tile);
-        if (t == 0) { s_place[0] = have; s_place[1] = b; s_place[2] = tile; }
+        const TaPlace f = ta_find<NQ>(S, x);
+        if (t == 0) s_place = f;
     }
     __syncthreads();
-    if (!s_place[0]) return;
-    const AtSeq seq = at_seq(P, s_place[1]);
-    const int row = s_place[2] * ROWS + t, tok = row / group;
+    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
+    if (!s_place.have) return;
+    const AtSeq seq = s_place.s;
+    const int row = s_place.tile * ROWS + t, tok = row / group;
     if (tok >= seq.count) return;
     const float* const parts = reinterpret_cast<const float*>(reinterpret_cast<const unsigned char*>(P.workspace) + S.part_offset)
                                + (size_t) blockIdx.x * S.slices * ta_part_floats(ROWS, D);
@@ -675,8 +690,9 @@ void attention_tc_join_kernel(const TaPlan S)
         }
     }
     const int head = h * group + row - tok * group;
-    at_store8<T>(P, seq, tok, head, blockIdx.y * 16, o[0], o[1], m, l);
-    at_store8<T>(P, seq, tok, head, blockIdx.y * 16 + 8, o[2], o[3], m, l);
+    const float f = at_factor(P, seq.first + tok, l);
+    at_store8<T>(P, seq, tok, head, blockIdx.y * 16, o[0], o[1], f, m, l);
+    at_store8<T>(P, seq, tok, head, blockIdx.y * 16 + 8, o[2], o[3], f, m, l);
 }
 
 template <typename T, int D, int NQ>
