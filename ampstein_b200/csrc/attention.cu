@@ -560,9 +560,9 @@ void attention_split_kernel(const AtPlan S)
     }
 }
 
-// Joins the parts of a segment, one row of it (blockIdx.y) per CTA: of segment blockIdx.x, or of the one that the range of CTA
-// blockIdx.x is the second to hold. Which parts those are is found while the split kernel's last CTAs still run.
-template <typename T, int D>
+// Joins the parts of a segment, row blockIdx.y of it (LOOP: every gridDim.y-th from there): of segment blockIdx.x, or of the one that the range of
+// CTA blockIdx.x is the second to hold. Which parts those are is found while the split kernel's last CTAs still run.
+template <typename T, int D, bool LOOP>
 __global__ __launch_bounds__(128)
 void attention_join_kernel(const AtPlan S)
 {
@@ -570,7 +570,7 @@ void attention_join_kernel(const AtPlan S)
     __shared__ float s_red[4], s_sum[4];
     __shared__ float4 s_o[4][D / 4];
     __shared__ int s_scan[4], s_found[2];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, r = blockIdx.y, group = P.heads / P.kv_heads;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, group = P.heads / P.kv_heads;
     AtCount C;
     C.count<128>(S, s_scan);
     AtCursor in;
@@ -601,74 +601,80 @@ void attention_join_kernel(const AtPlan S)
         last = C.cta_of(g0 + in.units - 1);
         join = first < last && (S.by_segment || first == (int) blockIdx.x - 1);
     }
-    const int row = join ? in.rt * S.rows + r : 0, tok = row / group;
     if (S.pdl) pdl_wait();
     if (S.pdl) pdl_launch_dependents();
-    if (!join || tok >= in.s.count) return;
+    if (!join) return;
 
     // part i of the segment: the first is the end of its CTA's range, the others are the beginning of theirs
     const size_t size = at_part_floats(S.rows, D);
     const float* const parts = reinterpret_cast<const float*>(P.workspace);
     const int n = last - first + 1;
     auto part = [&](int i) { return parts + (size_t) (2 * (first + i) + (i ? 0 : 1)) * size; };
-    float m = -INFINITY;
-    for (int i = t; i < n; i += 128) m = fmaxf(m, part(i)[(size_t) S.rows * D + 2 * r]);
-    // a warp adds every fourth part up, a lane D / 32 values of the row (in pieces of four); the first parts are on their way while m is found
-    constexpr int PIECES = D / 4, EACH = (PIECES + 31) / 32, AHEAD = D == 256 ? 4 : 8;
-    float4 x[AHEAD][EACH];
-    float2 ml[AHEAD];
-    auto fetch = [&](int i0) {
-        #pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
-        {
-            const int i = i0 + 4 * a;
-            ml[a] = make_float2(-INFINITY, 0.0f);
-            if (i >= n) continue;
-            const float* p = part(i);
-            ml[a] = *reinterpret_cast<const float2*>(p + (size_t) S.rows * D + 2 * r);
-            #pragma unroll
-            for (int e = 0; e < EACH; ++e)
-                if (PIECES % 32 == 0 || lane + 32 * e < PIECES) x[a][e] = reinterpret_cast<const float4*>(p + r * D)[lane + 32 * e];
-        }
-    };
-    fetch(warp);
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) s_red[warp] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    const float base = m == -INFINITY ? 0.0f : m;
-    float4 acc[EACH];
-    #pragma unroll
-    for (int e = 0; e < EACH; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
-    for (int i0 = warp; i0 < n; i0 += 4 * AHEAD)
+    for (int r = blockIdx.y; r < (LOOP ? S.rows : (int) blockIdx.y + 1); r += gridDim.y)
     {
-        #pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
-        {
-            if (i0 + 4 * a >= n) continue;
-            const float f = at_exp2(ml[a].x - base);
-            l += ml[a].x == -INFINITY ? ml[a].y : ml[a].y * f;
+        const int row = in.rt * S.rows + r, tok = row / group;
+        if (tok >= in.s.count) return;
+        float m = -INFINITY;
+        for (int i = t; i < n; i += 128) m = fmaxf(m, part(i)[(size_t) S.rows * D + 2 * r]);
+        // a warp adds every fourth part up, a lane D / 32 values of the row (in pieces of four); the first parts are on their way while m is found
+        constexpr int PIECES = D / 4, EACH = (PIECES + 31) / 32, AHEAD = D == 256 ? 4 : 8;
+        float4 x[AHEAD][EACH];
+        float2 ml[AHEAD];
+        auto fetch = [&](int i0) {
             #pragma unroll
-            for (int e = 0; e < EACH; ++e)
+            for (int a = 0; a < AHEAD; ++a)
             {
-                acc[e].x += x[a][e].x * f; acc[e].y += x[a][e].y * f; acc[e].z += x[a][e].z * f; acc[e].w += x[a][e].w * f;
+                const int i = i0 + 4 * a;
+                ml[a] = make_float2(-INFINITY, 0.0f);
+                if (i >= n) continue;
+                const float* p = part(i);
+                ml[a] = *reinterpret_cast<const float2*>(p + (size_t) S.rows * D + 2 * r);
+                #pragma unroll
+                for (int e = 0; e < EACH; ++e)
+                    if (PIECES % 32 == 0 || lane + 32 * e < PIECES) x[a][e] = reinterpret_cast<const float4*>(p + r * D)[lane + 32 * e];
             }
-        }
-        if (i0 + 4 * AHEAD < n) fetch(i0 + 4 * AHEAD);
-    }
-    if (lane == 0) s_sum[warp] = l;
-    #pragma unroll
-    for (int e = 0; e < EACH; ++e) if (PIECES % 32 == 0 || lane + 32 * e < PIECES) s_o[warp][lane + 32 * e] = acc[e];
-    __syncthreads();
-    l = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-    for (int c = t; c < PIECES; c += 128)
-    {
-        float4 y = s_o[0][c];
+        };
+        fetch(warp);
         #pragma unroll
-        for (int w = 1; w < 4; ++w) { const float4 z = s_o[w][c]; y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w; }
-        at_store<T>(P, in.s, tok, in.h * group + row - tok * group, c * 4, y, m, l);
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) s_red[warp] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+        const float base = m == -INFINITY ? 0.0f : m;
+        float4 acc[EACH];
+        #pragma unroll
+        for (int e = 0; e < EACH; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
+        for (int i0 = warp; i0 < n; i0 += 4 * AHEAD)
+        {
+            #pragma unroll
+            for (int a = 0; a < AHEAD; ++a)
+            {
+                if (i0 + 4 * a >= n) continue;
+                const float f = at_exp2(ml[a].x - base);
+                l += ml[a].x == -INFINITY ? ml[a].y : ml[a].y * f;       // (an l of NaN stays one)
+                #pragma unroll
+                for (int e = 0; e < EACH; ++e)
+                {
+                    acc[e].x += x[a][e].x * f; acc[e].y += x[a][e].y * f; acc[e].z += x[a][e].z * f; acc[e].w += x[a][e].w * f;
+                }
+            }
+            if (i0 + 4 * AHEAD < n) fetch(i0 + 4 * AHEAD);
+        }
+        if (lane == 0) s_sum[warp] = l;
+        #pragma unroll
+        for (int e = 0; e < EACH; ++e) if (PIECES % 32 == 0 || lane + 32 * e < PIECES) s_o[warp][lane + 32 * e] = acc[e];
+        __syncthreads();
+        l = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+        for (int c = t; c < PIECES; c += 128)
+        {
+            float4 y = s_o[0][c];
+            #pragma unroll
+            for (int w = 1; w < 4; ++w) { const float4 z = s_o[w][c]; y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w; }
+            at_store<T>(P, in.s, tok, in.h * group + row - tok * group, c * 4, y, m, l);
+        }
+        if constexpr (LOOP) __syncthreads();
+        else return;
     }
 }
 
@@ -778,10 +784,13 @@ static int at_launch(AtPlan& S, cudaStream_t stream)
     if (cudaError_t e = cudaLaunchKernelEx(&cfg, attention_split_kernel<T, D, WR>, (const AtPlan) S)) return cuda_rc(e, "attention launch");
     if (S.whole) return 0;
     S.by_segment = !P.cu && segments < S.grid;
-    cfg.gridDim = dim3(S.by_segment ? (unsigned) segments : S.grid, P.cu ? S.rows : (int) min((long) S.rows, rows), 1);
+    // a row per CTA; with cu there may be up to 64 of them and most CTAs have none: four CTAs go through all (2333 tokens of six prompts,
+    // none of which is the split form's: 49.1 us with a row per CTA, 44.4)
+    cfg.gridDim = dim3(S.by_segment ? (unsigned) segments : S.grid, P.cu ? 4 : (unsigned) min((long) S.rows, rows), 1);
     cfg.blockDim = dim3(128, 1, 1);
     cfg.dynamicSmemBytes = 0;
-    return cuda_rc(cudaLaunchKernelEx(&cfg, attention_join_kernel<T, D>, (const AtPlan) S), "attention join launch");
+    return cuda_rc(P.cu ? cudaLaunchKernelEx(&cfg, attention_join_kernel<T, D, true>, (const AtPlan) S)
+                        : cudaLaunchKernelEx(&cfg, attention_join_kernel<T, D, false>, (const AtPlan) S), "attention join launch");
 }
 
 template <typename T, int D>
