@@ -57,35 +57,24 @@ __device__ __forceinline__ void rope_pairs(uint4& a, uint4& b, const float2 (&cs
     }
 }
 
-// Where head h of the token (queries, then keys, then values) is read and written; to == null: it is not stored
+// Where head h of token n (queries, then keys, then values) is read, and written; null: it is not stored
 template <typename T>
-struct RopeHead
+__device__ __forceinline__ const T* rope_from(const amp_rope_args& P, int n, int h)
 {
-    const T* from;
-    T* to;
-};
+    if (h < P.heads) return reinterpret_cast<const T*>(P.q) + (long long) n * P.q_token + (long long) h * P.q_head;
+    h -= P.heads;
+    if (h < P.kv_heads) return reinterpret_cast<const T*>(P.k) + (long long) n * P.k_token + (long long) h * P.k_head;
+    return reinterpret_cast<const T*>(P.v) + (long long) n * P.v_token + (long long) (h - P.kv_heads) * P.v_head;
+}
 
 template <typename T>
-__device__ __forceinline__ RopeHead<T> rope_head(const amp_rope_args& P, int n, int h, long long kc, long long vc)
+__device__ __forceinline__ T* rope_to(const amp_rope_args& P, int n, int h, long long kc, long long vc)
 {
-    RopeHead<T> r;
-    if (h < P.heads)
-    {
-        r.from = reinterpret_cast<const T*>(P.q) + (long long) n * P.q_token + (long long) h * P.q_head;
-        r.to = reinterpret_cast<T*>(P.q_out) + (long long) n * P.out_token + (long long) h * P.out_head;
-        return r;
-    }
+    if (h < P.heads) return reinterpret_cast<T*>(P.q_out) + (long long) n * P.out_token + (long long) h * P.out_head;
     h -= P.heads;
-    if (h < P.kv_heads)
-    {
-        r.from = reinterpret_cast<const T*>(P.k) + (long long) n * P.k_token + (long long) h * P.k_head;
-        r.to = kc < 0 ? nullptr : reinterpret_cast<T*>(P.k_cache) + kc + (long long) h * P.kc_head;
-        return r;
-    }
-    h -= P.kv_heads;
-    r.from = reinterpret_cast<const T*>(P.v) + (long long) n * P.v_token + (long long) h * P.v_head;
-    r.to = vc < 0 ? nullptr : reinterpret_cast<T*>(P.v_cache) + vc + (long long) h * P.vc_head;
-    return r;
+    if (kc < 0) return nullptr;
+    if (h < P.kv_heads) return reinterpret_cast<T*>(P.k_cache) + kc + (long long) h * P.kc_head;
+    return reinterpret_cast<T*>(P.v_cache) + vc + (long long) (h - P.kv_heads) * P.vc_head;
 }
 
 // VEC: 16 bytes at a time; else value by value (a rotated part or a head that is not a multiple of 16 values, or other alignments)
@@ -97,101 +86,132 @@ void rope_kernel(const amp_rope_args P, int pdl)
     __shared__ int s_seq;
     const int t = threadIdx.x, n = blockIdx.x;
     if (pdl) { pdl_wait(); pdl_launch_dependents(); }
+    const int total = P.heads + (P.k ? 2 * P.kv_heads : 0), rotated = P.heads + (P.k ? P.kv_heads : 0);
 
-    int b, first_row;
-    if (P.cu)
+    // a thread's place in every head, and its first heads: requested before anything else is known of the token
+    constexpr int BATCH = 4;                                 // (and of the value-by-value form)
+    const int places = P.dim / 16, step = VEC ? ROPE_THREADS / places : 0, turning = P.rot / 16;
+    const int c = VEC ? t % places : 0, h0 = VEC ? t / places : 0;
+    const bool turns = c < turning, mine = h0 < step;        // (128 is not a multiple of every width)
+    const int at0 = 8 * (turns && !P.interleaved ? c : 2 * c), at1 = 8 * (turns && !P.interleaved ? c + turning : 2 * c + 1);
+    uint4 x[BATCH], y[BATCH];
+    auto fetch = [&](int h) {
+        #pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+        {
+            if (!mine || h + i * step >= total) continue;
+            const T* from = rope_from<T>(P, n, h + i * step);
+            x[i] = *reinterpret_cast<const uint4*>(from + at0);
+            y[i] = *reinterpret_cast<const uint4*>(from + at1);
+        }
+    };
+    if constexpr (VEC) fetch(h0);
+
+    int b = n, first_row;
+    long long p;
+    auto position = [&](int i) { return P.pos64 ? reinterpret_cast<const long long*>(P.pos)[i] : (long long) reinterpret_cast<const int*>(P.pos)[i]; };
+    if (P.cu && P.seqs <= 32)
+    {
+        // every warp by itself: a sequence per lane, its position on the way with its rows
+        const int lane = t & 31;
+        int lo = 0, hi = 0;
+        p = 0;
+        if (lane < P.seqs) { lo = P.cu[lane]; hi = P.cu[lane + 1]; p = position(lane); }
+        const uint32_t hit = __ballot_sync(0xffffffffu, lo <= n && n < hi);
+        if (!hit) return;                                    // behind the last sequence
+        b = __ffs(hit) - 1;
+        first_row = __shfl_sync(0xffffffffu, lo, b);
+        p = __shfl_sync(0xffffffffu, p, b);
+    }
+    else if (P.cu)
     {
         if (t == 0) s_seq = -1;
         __syncthreads();
         for (int i = t; i < P.seqs; i += ROPE_THREADS) if (P.cu[i] <= n && n < P.cu[i + 1]) s_seq = i;
         __syncthreads();
         b = s_seq;
-        if (b < 0) return;                                   // behind the last sequence
+        if (b < 0) return;
         first_row = P.cu[b];
+        p = position(b);
     }
     else
     {
         const int each = P.tokens / P.seqs;
         b = n / each;
         first_row = b * each;
+        p = position(b);
     }
-    const long long p = (P.pos64 ? reinterpret_cast<const long long*>(P.pos)[b] : (long long) reinterpret_cast<const int*>(P.pos)[b]) + (n - first_row);
-
-    long long kc = -1, vc = -1;
+    p += n - first_row;
+    int page = -1, row = 0;
     if (P.k && p >= 0 && p < (long long) P.max_pages * P.page_size)
     {
-        const int pg = (int) p / P.page_size, row = (int) p - pg * P.page_size, page = P.table[(long long) b * P.table_row + pg];
-        if (page >= 0 && page < P.pages)
-        {
-            kc = page * P.kc_page + row * P.kc_row;
-            vc = page * P.vc_page + row * P.vc_row;
-        }
+        const int pg = (int) p / P.page_size;
+        row = (int) p - pg * P.page_size;
+        page = P.table[(long long) b * P.table_row + pg];
     }
-    const int total = P.heads + (P.k ? 2 * P.kv_heads : 0), rotated = P.heads + (P.k ? P.kv_heads : 0);
+    // (under the table's entry)
+    for (int i = t; i < P.rot / 2; i += ROPE_THREADS) s_cs[i] = rope_turn((double) p, P.inv_freq[i], P.mscale);
+    __syncthreads();
+    const bool stored = page >= 0 && page < P.pages;
+    const long long kc = stored ? page * P.kc_page + row * P.kc_row : -1, vc = stored ? page * P.vc_page + row * P.vc_row : -1;
 
     if constexpr (VEC)
     {
-        const int places = P.dim / 16, step = ROPE_THREADS / places, turning = P.rot / 16;
-        const int c = t % places, h0 = t / places;
-        const bool turns = c < turning;
-        const int at0 = 8 * (turns && !P.interleaved ? c : 2 * c), at1 = 8 * (turns && !P.interleaved ? c + turning : 2 * c + 1);
-        const bool mine = h0 < step;                         // (128 is not a multiple of every width)
-        constexpr int BATCH = 4;
+        if (!mine) return;
         float2 cs[8];
-        bool have = false;
-        for (int h = h0; ; h += BATCH * step)
+        if (turns)
         {
-            uint4 x[BATCH], y[BATCH];
             #pragma unroll
-            for (int i = 0; i < BATCH; ++i)
-            {
-                if (!mine || h + i * step >= total) continue;
-                const RopeHead<T> r = rope_head<T>(P, n, h + i * step, kc, vc);
-                x[i] = *reinterpret_cast<const uint4*>(r.from + at0);
-                y[i] = *reinterpret_cast<const uint4*>(r.from + at1);
-            }
-            if (!have)
-            {
-                for (int i = t; i < P.rot / 2; i += ROPE_THREADS) s_cs[i] = rope_turn((double) p, P.inv_freq[i], P.mscale);
-                __syncthreads();
-                if (turns)
-                {
-                    #pragma unroll
-                    for (int i = 0; i < 8; ++i) cs[i] = s_cs[8 * c + i];
-                }
-                have = true;
-            }
-            if (!mine || h >= total) break;
+            for (int i = 0; i < 8; ++i) cs[i] = s_cs[8 * c + i];
+        }
+        for (int h = h0; h < total; h += BATCH * step)
+        {
+            if (h > h0) fetch(h);
             #pragma unroll
             for (int i = 0; i < BATCH; ++i)
             {
                 if (h + i * step >= total) continue;
-                const RopeHead<T> r = rope_head<T>(P, n, h + i * step, kc, vc);
-                if (!r.to) continue;
+                T* to = rope_to<T>(P, n, h + i * step, kc, vc);
+                if (!to) continue;
                 if (turns && h + i * step < rotated) rope_pairs<T>(x[i], y[i], cs, P.interleaved);
-                *reinterpret_cast<uint4*>(r.to + at0) = x[i];
-                *reinterpret_cast<uint4*>(r.to + at1) = y[i];
+                *reinterpret_cast<uint4*>(to + at0) = x[i];
+                *reinterpret_cast<uint4*>(to + at1) = y[i];
             }
         }
     }
     else
     {
-        for (int i = t; i < P.rot / 2; i += ROPE_THREADS) s_cs[i] = rope_turn((double) p, P.inv_freq[i], P.mscale);
-        __syncthreads();
-        const int half = P.rot / 2, each = half + P.dim - P.rot;        // a thread owns both values of a pair: q_out may be q
-        for (int i = t; i < total * each; i += ROPE_THREADS)
+        // a thread owns both values of a pair: q_out may be q. Four at a time, all read before the first is turned
+        const int half = P.rot / 2, each = half + P.dim - P.rot;
+        for (int i0 = t; i0 < total * each; i0 += BATCH * ROPE_THREADS)
         {
-            const int h = i / each, e = i - h * each;
-            const RopeHead<T> r = rope_head<T>(P, n, h, kc, vc);
-            if (!r.to) continue;
-            if (e >= half) { r.to[P.rot + e - half] = r.from[P.rot + e - half]; continue; }
-            const int a = P.interleaved ? 2 * e : e, z = P.interleaved ? 2 * e + 1 : e + half;
-            const T u = r.from[a], v = r.from[z];
-            if (h >= rotated) { r.to[a] = u; r.to[z] = v; continue; }
-            const float uf = rope_value(u), vf = rope_value(v);
-            const float2 cs = s_cs[e];
-            r.to[a] = AtType<T>::from(uf * cs.x - vf * cs.y);
-            r.to[z] = AtType<T>::from(vf * cs.x + uf * cs.y);
+            T u[BATCH], v[BATCH];
+            #pragma unroll
+            for (int k = 0; k < BATCH; ++k)
+            {
+                const int i = i0 + k * ROPE_THREADS, h = i / each, e = i - h * each;
+                if (i >= total * each) continue;
+                const T* from = rope_from<T>(P, n, h);
+                u[k] = from[e >= half ? P.rot + e - half : P.interleaved ? 2 * e : e];
+                if (e < half) v[k] = from[P.interleaved ? 2 * e + 1 : e + half];
+            }
+            #pragma unroll
+            for (int k = 0; k < BATCH; ++k)
+            {
+                const int i = i0 + k * ROPE_THREADS, h = i / each, e = i - h * each;
+                T* to = i < total * each ? rope_to<T>(P, n, h, kc, vc) : nullptr;
+                if (!to) continue;
+                if (e >= half) { to[P.rot + e - half] = u[k]; continue; }
+                if (h < rotated)
+                {
+                    const float uf = rope_value(u[k]), vf = rope_value(v[k]);
+                    const float2 cs = s_cs[e];
+                    u[k] = AtType<T>::from(uf * cs.x - vf * cs.y);
+                    v[k] = AtType<T>::from(vf * cs.x + uf * cs.y);
+                }
+                to[P.interleaved ? 2 * e : e] = u[k];
+                to[P.interleaved ? 2 * e + 1 : e + half] = v[k];
+            }
         }
     }
 }
