@@ -1,6 +1,7 @@
 """Host-side mirror of the reference's linear classes and CUDA-graph decode step, restricted to
 the EXL3 linears (reference: src/ucode/ampstein/models.uc:49-107 LinearEXL3,
-src/ucode/ampstein/graphdec.uc:151-282 step capture and replay).
+src/ucode/ampstein/graphdec.uc:151-282 step capture and replay), and a paged key-value cache with
+the attention block over it.
 
 LinearEXL3 derives everything from the trellis tensor:
     K = trellis.shape[-1] / 16, in_features = trellis.shape[0] * 16, out_features = shape[1] * 16
@@ -9,7 +10,7 @@ exactly as the reference does.
 """
 import torch
 
-from . import exl3
+from . import attention, exl3
 
 RECON_ROWS = 144          # models.uc:36
 RECON_MAX_N = 32768       # models.uc:37
@@ -239,6 +240,186 @@ class Sliced:
         a = self.linears[0]
         exl3.mgemm_normed(y, ssq, norm_w, eps, self.B, self.carrier, self.suh, self.svh, a.K, a.mcg, a.mul1, self.opts)
         return self.outs
+
+
+class PagedCache:
+    """Key-value cache of a model in pages: k, v (layers, pages, page_size, kv_heads, dim) and table (slots, max_pages) int32 on the
+    device, the bookkeeping on the host. A sequence has a slot, that is a row of the table; its pages are the same in every layer.
+    Forks share pages until one of them writes. Entries of pages that a sequence does not have (any more) are -1.
+
+    The host knows every length (extend() announces tokens before they are written), nothing is read back. Calls that copy pages or
+    change the table run on the current stream: those of one cache belong on one stream, in the order of the work on it."""
+
+    def __init__(self, layers, pages, page_size, kv_heads, dim, slots, max_pages, dtype=torch.float16, device="cuda"):
+        if min(layers, pages, page_size, kv_heads, dim, slots, max_pages) < 1:
+            raise ValueError("PagedCache: sizes must be positive")
+        # (zeros: whatever a page holds behind a sequence's end is finite)
+        self.k = torch.zeros((layers, pages, page_size, kv_heads, dim), dtype=dtype, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.table = torch.full((slots, max_pages), -1, dtype=torch.int32, device=device)
+        self.page_size, self.max_pages = page_size, max_pages
+        self._free = list(range(pages - 1, -1, -1))          # (popped from the end: low numbers first)
+        self._uses = [0] * pages                              # sequences that have the page
+        self._seqs = [None] * slots                           # per slot: [pages (None: given up), tokens]
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def _seq(self, slot):
+        if not 0 <= slot < len(self._seqs) or self._seqs[slot] is None:
+            raise ValueError("PagedCache: slot %s holds no sequence" % (slot,))
+        return self._seqs[slot]
+
+    def length(self, slot):
+        """Tokens announced for the sequence: the position of its next one"""
+        return self._seq(slot)[1]
+
+    def _write_row(self, slot):
+        pages = self._seqs[slot][0] if self._seqs[slot] is not None else []
+        row = [-1 if p is None else p for p in pages] + [-1] * (self.max_pages - len(pages))
+        self.table[slot].copy_(torch.tensor(row, dtype=torch.int32))
+
+    def _drop(self, page):
+        self._uses[page] -= 1
+        if self._uses[page] == 0:
+            self._free.append(page)
+
+    def add(self):
+        """A slot for a new sequence"""
+        for slot, seq in enumerate(self._seqs):
+            if seq is None:
+                self._seqs[slot] = [[], 0]
+                return slot
+        raise RuntimeError("PagedCache: all %d slots are taken" % len(self._seqs))
+
+    def extend(self, slot, tokens):
+        """Room for `tokens` more tokens of the sequence, which may then be written (rope_append). A page that a fork shares gets a
+        copy of its own where they go into it. Returns the position of the first of them. RuntimeError, and nothing changed, without
+        room."""
+        seq = self._seq(slot)
+        pages, at = seq
+        if tokens < 0:
+            raise ValueError("PagedCache.extend: tokens must not be negative")
+        need = -(-(at + tokens) // self.page_size)
+        if need > self.max_pages:
+            raise RuntimeError("PagedCache: %d tokens do not fit into %d pages" % (at + tokens, self.max_pages))
+        last = at // self.page_size if tokens and at % self.page_size else None           # the half-filled page that is written on
+        own = last is not None and pages[last] is not None and self._uses[pages[last]] > 1
+        if last is not None and pages[last] is None:
+            raise ValueError("PagedCache: the page of position %d has been given up" % at)
+        if need - len(pages) + own > len(self._free):
+            raise RuntimeError("PagedCache: %d pages are free, %d are needed" % (len(self._free), need - len(pages) + own))
+        changed = own
+        if own:
+            page = self._free.pop()
+            attention.copy_pages([self.k, self.v], [pages[last]], [page])
+            self._drop(pages[last])
+            self._uses[page] = 1
+            pages[last] = page
+        while len(pages) < need:
+            page = self._free.pop()
+            self._uses[page] = 1
+            pages.append(page)
+            changed = True
+        seq[1] = at + tokens
+        if changed:
+            self._write_row(slot)
+        return at
+
+    def fork(self, slot):
+        """A new sequence with the same tokens; shares the pages. Returns its slot."""
+        pages, at = self._seq(slot)
+        new = self.add()
+        self._seqs[new] = [list(pages), at]
+        for page in pages:
+            if page is not None:
+                self._uses[page] += 1
+        self._write_row(new)
+        return new
+
+    def truncate(self, slot, tokens):
+        """Takes back what stands behind the first `tokens` tokens (rejected drafts)"""
+        seq = self._seq(slot)
+        if not 0 <= tokens <= seq[1]:
+            raise ValueError("PagedCache.truncate: %d of %d tokens" % (tokens, seq[1]))
+        keep = -(-tokens // self.page_size)
+        for page in seq[0][keep:]:
+            if page is not None:
+                self._drop(page)
+        changed = len(seq[0]) > keep
+        del seq[0][keep:]
+        seq[1] = tokens
+        if changed:
+            self._write_row(slot)
+
+    def leave_behind(self, slot, window, sinks=0):
+        """Gives up the pages that no further token of the sequence sees: those that hold neither one of the first `sinks` tokens nor one
+        of the last `window` - 1"""
+        pages, at = self._seq(slot)
+        if window < 1 or sinks < 0:
+            raise ValueError("PagedCache.leave_behind: window must be positive, sinks not negative")
+        changed = False
+        for i in range(-(-sinks // self.page_size), max(0, at - window + 1) // self.page_size):
+            if pages[i] is not None:
+                self._drop(pages[i])
+                pages[i] = None
+                changed = True
+        if changed:
+            self._write_row(slot)
+
+    def free(self, slot):
+        """The sequence is over: its slot and the pages that no fork has are free again"""
+        for page in self._seq(slot)[0]:
+            if page is not None:
+                self._drop(page)
+        self._seqs[slot] = None
+        self._write_row(slot)
+
+    def compact(self):
+        """Moves pages so that the used ones are the first of the pool (which may then be cut off, or given to another cache). Returns how
+        many are used."""
+        used = sum(1 for n in self._uses if n)
+        src = [p for p in range(used, len(self._uses)) if self._uses[p]]
+        dst = [p for p in range(used) if not self._uses[p]]
+        if src:
+            attention.copy_pages([self.k, self.v], src, dst)
+            to = dict(zip(src, dst))
+            for a, b in to.items():
+                self._uses[b], self._uses[a] = self._uses[a], 0
+            for slot, seq in enumerate(self._seqs):
+                if seq is not None and any(p in to for p in seq[0]):
+                    seq[0] = [to.get(p, p) for p in seq[0]]
+                    self._write_row(slot)
+        self._free = list(range(len(self._uses) - 1, used - 1, -1))
+        return used
+
+
+class PagedAttention:
+    """The attention block of a decoder layer over a PagedCache: q|k|v bundle, rotary positions with the write into the cache,
+    attention, o. One object serves prompts, drafted and single tokens, eagerly or inside a DecodeGraph."""
+
+    def __init__(self, qkv, o, cache, layer, dim, inv_freq, mscale=1.0, interleaved=False, window=0, sinks=0, scale=None):
+        widths = [w.out_features for w in qkv.linears]
+        kv_heads = cache.k.shape[3]
+        if len(widths) != 3 or cache.k.shape[4] != dim or widths[1] != kv_heads * dim or widths[2] != kv_heads * dim or widths[0] % (kv_heads * dim):
+            raise ValueError("PagedAttention: q|k|v of %s columns do not fit a cache of %d heads of %d" % (widths, kv_heads, dim))
+        if o.in_features != widths[0]:
+            raise ValueError("PagedAttention: o takes %d columns, q gives %d" % (o.in_features, widths[0]))
+        if not 0 <= layer < cache.k.shape[0]:
+            raise ValueError("PagedAttention: layer %d of %d" % (layer, cache.k.shape[0]))
+        self.qkv, self.o, self.dim = qkv, o, dim
+        self.k, self.v = cache.k[layer], cache.v[layer]
+        self.rope = dict(interleaved=interleaved, mscale=mscale)
+        self.inv_freq, self.view = inv_freq, dict(window=window, sinks=sinks, scale=scale)
+
+    def run(self, x, pos, table, cu=None, out=None):
+        """x (1, rows, hidden); pos, cu as paged_attention, table (seqs, max_pages) the sequences' rows of the cache's. Returns (rows,
+        hidden)."""
+        q, k, v = (t[0].view(t.shape[1], -1, self.dim) for t in self.qkv.run(x))
+        q = attention.rope_append(q, k, v, pos, self.inv_freq, self.k, self.v, table, cu=cu, out=q, **self.rope)
+        a = attention.paged_attention(q, self.k, self.v, table, pos, cu=cu, **self.view)
+        return self.o.forward(a.view(a.shape[0], -1), out)
 
 
 class DecodeGraph:
