@@ -77,6 +77,15 @@ def _cache(name, what, t, dtype, dev, shape):
     return tuple(s[i] if z[i] > 1 else 0 for i in range(3))
 
 
+def _apart(name, what, t):
+    """Whether what is written lies at places of its own: no stride inside the extent of a smaller one"""
+    extent = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st < extent:
+            raise ValueError("%s: places of %s overlap" % (name, what))
+        extent = st * (n - 1) + extent
+
+
 def _sequences(name, rows, pos, cu, dev):
     _cuda(name, "pos", pos, dev)
     if pos.dtype not in (torch.int32, torch.int64) or pos.dim() != 1 or not pos.is_contiguous():
@@ -175,6 +184,7 @@ def _rope(name, q, kv, pos, inv_freq, cu, interleaved, mscale, out):
         os = (heads * dim, dim)
     else:
         os = _rows(name, "out", out, dtype, dev, (rows, heads, dim))
+        _apart(name, "out", out)
         if out.data_ptr() == q.data_ptr() and os != qs:
             raise ValueError("%s: out overlaps q (it may be q itself)" % name)
     if kv is None:
@@ -194,6 +204,8 @@ def _rope(name, q, kv, pos, inv_freq, cu, interleaved, mscale, out):
         if tuple(kc.shape[2:]) != (kv_heads, dim) or pages < 1 or page_size < 1:
             raise ValueError("%s: the caches must be (pages, page_size, %d, %d)" % (name, kv_heads, dim))
         vcs = _cache(name, "v_cache", vc, dtype, dev, tuple(kc.shape))
+        _apart(name, "k_cache", kc)
+        _apart(name, "v_cache", vc)
         max_pages, tr = _table(name, table, seqs, page_size, dev)
         cs = kcs + vcs + (tr,)
     if rows == 0 or seqs == 0:
@@ -236,7 +248,7 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
     """Attention of q (rows, heads, dim), fp16 or bf16, dim 64 / 128 / 256, over caches that hold the rows' own keys and values
     already (rope_append). The token at position p sees the keys at positions j <= p, with window > 0 only the last `window` of
     them (its own among them) and the first `sinks`. heads is a multiple of kv_heads; query head h reads key-value head
-    h // (heads / kv_heads). scale: 1 / sqrt(dim) by default. Returns out (rows, heads, dim), q's type; lse (rows, heads) float32, if
+    h // (heads / kv_heads). scale: 1 / sqrt(dim) by default. Returns out (rows, heads, dim), q's type, which must not overlap q; lse (rows, heads) float32, if
     given, takes ln sum_j exp(scale * q . k_j).
 
     A token that sees nothing gets 0 (lse -inf). Pages that no token of the call can see are not read, and their table entries may hold
@@ -278,6 +290,7 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
         os = (heads * dim, dim)
     else:
         os = _rows(name, "out", out, dtype, dev, (rows, heads, dim))
+        _apart(name, "out", out)
         if out.data_ptr() == q.data_ptr():
             raise ValueError("%s: out must not be q" % name)
     if lse is not None:
@@ -296,6 +309,16 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
                            1 if pos.dtype is torch.int64 else 0, scale)
     _launch(q, "amp_b200_attention", args)
     return out
+
+
+def attention_status(device=None):
+    """0, or 1: a bounded wait in a call of paged_attention with prompt chunks ran out since the last look, and what depended on it was not
+    stored. Waits for the device."""
+    import ctypes
+    v = ctypes.c_int(0)
+    with torch.cuda.device(device):
+        _lib.call("amp_b200_attention_status", ctypes.byref(v))
+    return v.value
 
 
 def _page_list(what, xs):

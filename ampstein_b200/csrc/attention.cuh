@@ -22,6 +22,13 @@ struct AtSeq
     int first, count, row0;                    // position of the first query token, tokens, first row of q
 };
 
+// Tokens of sequence b with cu
+__device__ __forceinline__ int at_count(const amp_attention_args& P, int b)
+{
+    const int row0 = max(0, min(P.cu[b], P.tokens));
+    return max(row0, min(P.cu[b + 1], P.tokens)) - row0;
+}
+
 // Sequence b. Whatever pos and cu hold, the rows stay inside the tensors.
 __device__ __forceinline__ AtSeq at_seq(const amp_attention_args& P, int b)
 {
@@ -31,7 +38,7 @@ __device__ __forceinline__ AtSeq at_seq(const amp_attention_args& P, int b)
     if (P.cu)
     {
         s.row0 = max(0, min(P.cu[b], P.tokens));
-        s.count = max(s.row0, min(P.cu[b + 1], P.tokens)) - s.row0;
+        s.count = at_count(P, b);
     }
     else
     {

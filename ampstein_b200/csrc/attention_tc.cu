@@ -169,24 +169,32 @@ __device__ __forceinline__ TaPlace ta_find(const TaPlan& S, int x)
         if (f.have) f.s = at_seq(P, f.b);
         return f;
     }
-    for (int b0 = 0; b0 < P.seqs; b0 += 32)
+    // four sequences per lane at a time
+    constexpr int EACH = 4;
+    for (int b0 = 0; b0 < P.seqs; b0 += 32 * EACH)
     {
-        AtSeq s = {};
-        if (b0 + lane < P.seqs) s = at_seq(P, b0 + lane);
-        const int n = tiles(s.count * group);
-        int sum = n;
+        int n[EACH], mine = 0;
+        #pragma unroll
+        for (int i = 0; i < EACH; ++i)
+        {
+            const int b = b0 + lane * EACH + i;
+            n[i] = b < P.seqs ? tiles(at_count(P, b) * group) : 0;
+            mine += n[i];
+        }
+        int sum = mine;
         #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += y; }
         const uint32_t hit = __ballot_sync(0xffffffffu, x < sum);
         if (hit)
         {
             const int l = __ffs(hit) - 1;
+            int left = x - (sum - mine), at = 0;             // (of lane l)
+            #pragma unroll
+            for (int i = 0; i < EACH - 1; ++i) if (at == i && left >= n[i]) { left -= n[i]; ++at; }
             f.have = 1;
-            f.b = b0 + l;
-            f.tile = x - (__shfl_sync(0xffffffffu, sum, l) - __shfl_sync(0xffffffffu, n, l));
-            f.s.first = __shfl_sync(0xffffffffu, s.first, l);
-            f.s.count = __shfl_sync(0xffffffffu, s.count, l);
-            f.s.row0 = __shfl_sync(0xffffffffu, s.row0, l);
+            f.b = __shfl_sync(0xffffffffu, b0 + lane * EACH + at, l);
+            f.tile = __shfl_sync(0xffffffffu, left, l);
+            f.s = at_seq(P, f.b);
             return f;
         }
         x -= __shfl_sync(0xffffffffu, sum, 31);

@@ -70,6 +70,24 @@ static int tc_cache(const DLTensor* t, int64_t kv_heads, int64_t dim)
            tc_fits(t->shape[0]) && tc_fits(t->shape[1]);
 }
 
+/* no stride inside the extent of a smaller one: every place of what is written is its own */
+static int tc_apart(const DLTensor* t)
+{
+    int64_t extent = 1;
+    int done[8] = { 0 }, d, k;
+    if (t->ndim > 8) return 0;
+    for (k = 0; k < t->ndim; ++k)
+    {
+        int best = -1;
+        for (d = 0; d < t->ndim; ++d) if (!done[d] && t->shape[d] > 1 && (best < 0 || t->strides[d] < t->strides[best])) best = d;
+        if (best < 0) return 1;
+        if (t->strides[best] < extent) return 0;
+        extent += t->strides[best] * (t->shape[best] - 1);
+        done[best] = 1;
+    }
+    return 1;
+}
+
 /* pos and cu (None) of `rows` rows */
 static int tc_sequences(PyObject* pos_o, PyObject* cu_o, int64_t rows, int dev, const void** pos, const int** cu, int* seqs, int* pos64)
 {
@@ -116,7 +134,7 @@ ENTRY(rope_call)
     memset(&P, 0, sizeof P);
     if (!tc_get(a[0], &q, -1) || !tc_rows(&q) || !tc_half(&q, &P.bf16) || q.shape[0] < 1) Py_RETURN_NONE;
     dev = q.device.device_id;
-    if (!tc_get(a[11], &out, dev) || !tc_rows(&out) || !tc_same(&out, &q) || !tc_shape(&out, q.shape[0], q.shape[1], q.shape[2])) Py_RETURN_NONE;
+    if (!tc_get(a[11], &out, dev) || !tc_rows(&out) || !tc_same(&out, &q) || !tc_shape(&out, q.shape[0], q.shape[1], q.shape[2]) || !tc_apart(&out)) Py_RETURN_NONE;
     if (!tc_get(a[4], &f, dev) || f.ndim != 1 || !tc_dense(&f, 0) || !tc_is(&f, kDLFloat, 32) || 2 * f.shape[0] > q.shape[2]) Py_RETURN_NONE;
     if (!tc_sequences(a[3], a[8], q.shape[0], dev, &P.pos, &P.cu, &P.seqs, &P.pos64)) Py_RETURN_NONE;
     P.q = tc_ptr(&q); P.q_out = tc_ptr(&out); P.inv_freq = (const float*) tc_ptr(&f);
@@ -132,7 +150,8 @@ ENTRY(rope_call)
         if (!tc_get(a[1], &k, dev) || !tc_rows(&k) || !tc_same(&k, &q) || k.shape[0] != q.shape[0] || k.shape[2] != q.shape[2]) Py_RETURN_NONE;
         if (!tc_get(a[2], &v, dev) || !tc_rows(&v) || !tc_same(&v, &q) || !tc_shape(&v, k.shape[0], k.shape[1], k.shape[2])) Py_RETURN_NONE;
         if (!tc_get(a[5], &kc, dev) || !tc_same(&kc, &q) || !tc_cache(&kc, k.shape[1], k.shape[2])) Py_RETURN_NONE;
-        if (!tc_get(a[6], &vc, dev) || !tc_same(&vc, &q) || !tc_cache(&vc, k.shape[1], k.shape[2]) || vc.shape[0] != kc.shape[0] || vc.shape[1] != kc.shape[1]) Py_RETURN_NONE;
+        if (!tc_get(a[6], &vc, dev) || !tc_same(&vc, &q) || !tc_cache(&vc, k.shape[1], k.shape[2]) || vc.shape[0] != kc.shape[0] || vc.shape[1] != kc.shape[1] ||
+            !tc_apart(&kc) || !tc_apart(&vc)) Py_RETURN_NONE;
         if (!tc_table(a[7], P.seqs, kc.shape[1], dev, &P.table, &P.table_row, &P.max_pages)) Py_RETURN_NONE;
         P.k = tc_ptr(&k); P.v = tc_ptr(&v); P.k_cache = tc_ptr(&kc); P.v_cache = tc_ptr(&vc);
         P.k_token = tc_stride(&k, 0); P.k_head = tc_stride(&k, 1); P.v_token = tc_stride(&v, 0); P.v_head = tc_stride(&v, 1);
@@ -162,7 +181,7 @@ ENTRY(attention_call)
     if (!tc_get(a[2], &vc, dev) || !tc_same(&vc, &q) || !tc_cache(&vc, kc.shape[2], q.shape[2]) || vc.shape[0] != kc.shape[0] || vc.shape[1] != kc.shape[1]) Py_RETURN_NONE;
     if (!tc_sequences(a[4], a[5], q.shape[0], dev, &P.pos, &P.cu, &P.seqs, &P.pos64)) Py_RETURN_NONE;
     if (!tc_table(a[3], P.seqs, kc.shape[1], dev, &P.table, &P.table_row, &P.max_pages)) Py_RETURN_NONE;
-    if (!tc_get(a[9], &out, dev) || !tc_rows(&out) || !tc_same(&out, &q) || !tc_shape(&out, q.shape[0], q.shape[1], q.shape[2])) Py_RETURN_NONE;
+    if (!tc_get(a[9], &out, dev) || !tc_rows(&out) || !tc_same(&out, &q) || !tc_shape(&out, q.shape[0], q.shape[1], q.shape[2]) || !tc_apart(&out)) Py_RETURN_NONE;
     window = PyLong_AsLong(a[6]);
     sinks = PyLong_AsLong(a[7]);
     scale = PyFloat_AsDouble(a[8]);

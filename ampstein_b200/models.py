@@ -248,7 +248,8 @@ class PagedCache:
     Forks share pages until one of them writes. Entries of pages that a sequence does not have (any more) are -1.
 
     The host knows every length (extend() announces tokens before they are written), nothing is read back. Calls that copy pages or
-    change the table run on the current stream: those of one cache belong on one stream, in the order of the work on it."""
+    change the table run on the current stream and do not wait: those of one cache belong on one stream, in the order of the work on it,
+    and not inside a captured graph."""
 
     def __init__(self, layers, pages, page_size, kv_heads, dim, slots, max_pages, dtype=torch.float16, device="cuda"):
         if min(layers, pages, page_size, kv_heads, dim, slots, max_pages) < 1:
@@ -278,7 +279,10 @@ class PagedCache:
     def _write_row(self, slot):
         pages = self._seqs[slot][0] if self._seqs[slot] is not None else []
         row = [-1 if p is None else p for p in pages] + [-1] * (self.max_pages - len(pages))
-        self.table[slot].copy_(torch.tensor(row, dtype=torch.int32))
+        row = torch.tensor(row, dtype=torch.int32)
+        if self.table.is_cuda:
+            row = row.pin_memory()                           # (torch keeps the pinned memory until the copy is done: no wait here)
+        self.table[slot].copy_(row, non_blocking=True)
 
     def _drop(self, page):
         self._uses[page] -= 1

@@ -277,12 +277,28 @@ def test_refusals(amp):
         (ValueError, lambda: f(q, k, v, table, pos, lse=torch.zeros((2, 3), device="cuda"))),
         (ValueError, lambda: f(q.transpose(1, 2).contiguous().transpose(1, 2), k, v, table, pos)),
         (RuntimeError, lambda: f(torch.zeros(2 * 4 * 64 + 1, dtype=H, device="cuda")[1:].view(2, 4, 64), k, v, table, pos)),
+        (ValueError, lambda: f(q, k, v, table, pos, out=q[:1].clone().expand(2, 4, 64))),
         (ValueError, lambda: f(q, k, v, torch.zeros((2, 1 << 27), dtype=torch.int32, device="cuda"), pos)),
     ]
     for i, (kind, call) in enumerate(bad):
         with pytest.raises(kind):
             call()
             pytest.fail("call %d was taken" % i)
+
+
+@pytest.mark.parametrize("seqs", [33, 150, 700])
+def test_prompts_among_many_sequences(amp, seqs):
+    """Row tiles of prompts found behind hundreds of single tokens and empty sequences"""
+    g = torch.Generator().manual_seed(seqs)
+    counts = torch.randint(0, 2, (seqs,), generator=g).tolist()
+    pos = torch.randint(-1, 60, (seqs,), generator=g).tolist()
+    for b, n in ((0, 70), (31, 40), (32, 129), (seqs - 2, 33), (seqs - 1, 90)):
+        counts[b], pos[b] = n, b % 7
+    check(amp, pos, counts, 4, 2, 64, 16, H, ragged=True)
+
+
+def test_no_wait_was_lost(amp):
+    assert amp.attention_status() == 0
 
 
 def test_calls_without_the_tensor_table(amp, monkeypatch):

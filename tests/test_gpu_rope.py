@@ -147,6 +147,8 @@ def test_refusals(amp):
         (ValueError, lambda: amp.rope(q, torch.zeros(3, dtype=torch.int32, device="cuda"), inv_freq)),
         (ValueError, lambda: amp.rope(q, pos, inv_freq, out=q.new_empty((2, 4, 32)))),
         (ValueError, lambda: amp.rope(q[:, :2], pos, inv_freq, out=q.view(-1)[:2 * 2 * 64].view(2, 2, 64))),
+        (ValueError, lambda: amp.rope(q, pos, inv_freq, out=q[:, :1].clone().expand(2, 4, 64))),
+        (ValueError, lambda: f(q, k, v, pos, inv_freq, kc[:1].expand(3, 16, 2, 64), vc, table)),
         (RuntimeError, lambda: amp.rope(rand((1, 1, 1040), H, 1), pos[:1], inv_freq)),
     ]
     for i, (kind, call) in enumerate(bad):
