@@ -12,6 +12,15 @@
 // The warps of a CTA are WK groups of WR: a group owns KW keys of every unit, its warps 16 rows each. A group has a ring of half
 // stages (KW keys, then their values), filled by its own lanes with 16-byte asynchronous copies, and meets nobody else until the segment
 // ends: every warp keeps m, l and o of its rows over its keys. The rings run ahead over the ends of segments.
+//
+// What bounds it: memory, and a fixed 8 us (launch, positions, table, first keys: 4.5; the second kernel 3.5), of which a table of up to
+// 256 keys leaves out the second. 32 query heads on 8 key-value heads of 128 values, fp16, us on the device: one sequence of 512 keys 8.0,
+// 4096 10.3, 32768 30, 131072 88 (6.1 TB/s, 0.94 of the measured copy rate; between 131072 and 262144 keys 7 TB/s), 32 sequences of
+// 2048 keys 53 (5.1 TB/s), of 100 to 8192 keys 56 (before the end of a segment was counted as a unit, 71: a range of
+// many short sequences took as long again as its keys). mma.sync and not tcgen05: at 16 rows and 128 values a warp needs 400 issue cycles
+// for the 16 KB that a scheduler's share of the memory brings in 2850. 32 keys per step where the registers allow it: the
+// look-ups, the row maxima and the loop are per step (32 x 2048 keys, 16 / 32 keys: 60.0 / 53.3). Wide heads keep q in shared
+// memory (256 values: 49.7 -> 41.0 for seven sequences of 1000 to 30000 keys).
 #include "attention_tc.cuh"
 
 namespace amp {
@@ -697,7 +706,7 @@ static const AtDevice* at_device(int* rc)
 
 // Sequences that fit into this many keys are not split: nothing is joined then
 constexpr int AT_WHOLE_KEYS = 256;
-// Rows (tokens x group) up to which a sequence takes the split form; beyond, the prompt form
+// Rows (tokens x group) up to which a sequence takes the split form, whose ranges follow the lengths; beyond, the prompt form
 constexpr int AT_SPLIT_ROWS = 64;
 
 static int at_grid(int dim, int sms) { return sms * (dim == 64 ? at_ctas<64> : dim == 128 ? at_ctas<128> : at_ctas<256>); }

@@ -1,6 +1,7 @@
 // Copies of whole pages inside paged caches, all layers of all caches in one launch: a fork's own last page, moves of a
 // defragmentation. The page lists come from the host (where the cache's bookkeeping is) and travel as launch parameters.
-// Bound by memory: a CTA moves 16 KB, every thread with four 16-byte loads in flight.
+// Bound by memory: a CTA moves 16 KB, every thread with four 16-byte loads in flight. 101 pages of 131 KB in 16 layers of both caches 129 us
+// (6.6 TB/s in and out, the measured copy rate), one page of 32 KB in 32 layers 2.2 us.
 #include "exl3_common.cuh"
 #include "host_common.h"
 #include "../../include/ampstein_b200.h"
