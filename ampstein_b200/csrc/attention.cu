@@ -13,8 +13,8 @@
 // stages (KW keys, then their values), filled by its own lanes with 16-byte asynchronous copies, and meets nobody else until the segment
 // ends: every warp keeps m, l and o of its rows over its keys. The rings run ahead over the ends of segments.
 //
-// What bounds it: memory, and a fixed 8 us (launch, positions, table, first keys: 4.5; the second kernel 3.5), of which a table of up to
-// 256 keys leaves out the second. 32 query heads on 8 key-value heads of 128 values, fp16, us on the device: one sequence of 512 keys 8.0,
+// What bounds it: memory, and a fixed 8 us (launch, positions, table, first keys: 4.5; the second kernel 3.5), of which sequences
+// that see few keys are spared the second (AT_CLUSTER_KEYS). 32 query heads on 8 key-value heads of 128 values, fp16, us on the device: one sequence of 512 keys 8.0,
 // 4096 10.3, 32768 30, 131072 88 (6.1 TB/s, 0.94 of the measured copy rate; between 131072 and 262144 keys 7 TB/s), 32 sequences of
 // 2048 keys 53 (5.1 TB/s), of 100 to 8192 keys 56 (before the end of a segment was counted as a unit, 71: a range of
 // many short sequences took as long again as its keys). mma.sync and not tcgen05: at 16 rows and 128 values a warp needs 400 issue cycles
@@ -45,7 +45,7 @@ struct AtPlan
     int grid;                                  // CTAs of the split form
     int unit, rows;                            // keys of a unit, rows of a row tile
     int split_rows;                            // with cu: sequences of more rows (tokens x group) are the prompt form's
-    int whole;                                 // 1: every (sequence, head, row tile) belongs to one CTA, nothing to join
+    int cluster;                               // > 0: every (sequence, head, row tile) belongs to a cluster of so many CTAs, which join in shared memory
     int by_segment;                            // join: blockIdx.x is a segment, else the CTA whose range begins inside it
     int pdl;
     float scale2;                              // scale * log2(e)
@@ -73,6 +73,35 @@ __device__ __forceinline__ void at_mma(float (&c)[4], const uint32_t (&a)[4], ui
     else
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+constexpr int AT_MAX_CLUSTER = 8;              // portable
+
+__device__ __forceinline__ void at_cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The same place of shared memory in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t at_map(uint32_t addr, int rank)
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+
+__device__ __forceinline__ float2 at_ld_cluster2(uint32_t addr)
+{
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ float4 at_ld_cluster4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
 }
 
 // Row tiles of a sequence, and units of each of them (one at least: a segment without keys stores its zeros)
@@ -221,7 +250,7 @@ struct AtCount
 // one that it does not end
 __host__ __device__ constexpr size_t at_part_floats(int rows, int dim) { return (size_t) rows * (dim + 2); }
 
-template <typename T, int D, int WR>
+template <typename T, int D, int WR, bool CLUSTER>
 __global__ __launch_bounds__(AT_THREADS, at_ctas<D>)
 void attention_split_kernel(const AtPlan S)
 {
@@ -241,13 +270,17 @@ void attention_split_kernel(const AtPlan S)
     // the CTA's range of units
     AtCursor in;
     int left;
-    if (S.whole)
+    if (CLUSTER)
     {
         in.b = 0; in.load(S);                                // (all sequences have as many tokens)
-        const int per = P.kv_heads * in.tiles;
-        in.place(S, cta / per, 0);
-        in.h = cta % per / in.tiles; in.rt = cta % in.tiles;
-        left = in.units;
+        const int per = P.kv_heads * in.tiles, segment = cta / S.cluster, rank = cta - segment * S.cluster;
+        in.place(S, segment / per, 0);
+        in.h = segment % per / in.tiles; in.rt = segment % in.tiles;
+        // (a share may be empty: it then is of a cluster that has more CTAs than units)
+        in.u = in.units * rank / S.cluster;
+        left = in.units * (rank + 1) / S.cluster - in.u;
+        in.units = in.u + left;                              // the share ends like a segment
+        left += left > 0;
     }
     else
     {
@@ -492,8 +525,10 @@ void attention_split_kernel(const AtPlan S)
             left -= ends ? 2 : 1;
             if (hold)
             {
-                const bool before = first_segment && began_before, shared = !S.whole && (before || !ends);
-                float* const part = reinterpret_cast<float*>(P.workspace) + (size_t) (2 * cta + (before ? 0 : 1)) * at_part_floats(ROWS, D);
+                const bool before = first_segment && began_before, shared = CLUSTER ? S.cluster > 1 : before || !ends;
+                // (a cluster's part stays in shared memory, behind the rows of q)
+                float* const part = CLUSTER ? reinterpret_cast<float*>(smem + at_smem<D, WR>)
+                                            : reinterpret_cast<float*>(P.workspace) + (size_t) (2 * cta + (before ? 0 : 1)) * at_part_floats(ROWS, D);
                 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                 {
@@ -566,6 +601,42 @@ void attention_split_kernel(const AtPlan S)
         }
         slot = slot + 1 == H ? 0 : slot + 1;
         --ahead;
+    }
+
+    if (CLUSTER && S.cluster > 1)
+    {
+        // every CTA of the cluster finishes its share of the segment's values, in order of the keys. (The barrier in front: all parts are
+        // there, and all CTAs run. The one behind: nobody leaves with a part that is still read.)
+        const int C = S.cluster, units = at_units(S, in.k), per = (ROWS * D / 4 + C - 1) / C, rank = cta % C;
+        at_cluster_sync();
+        const uint32_t mine = smem_u32(smem) + at_smem<D, WR>;
+        for (int i = rank * per + t; i < min((rank + 1) * per, ROWS * D / 4); i += NT)
+        {
+            const int r = i / (D / 4), c = (i % (D / 4)) * 4, row = in.rt * ROWS + r, tok = row / group;
+            if (tok >= in.s.count) break;
+            float m = -INFINITY, l = 0.0f;
+            float2 ml[AT_MAX_CLUSTER];
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y[AT_MAX_CLUSTER];
+            #pragma unroll
+            for (int k = 0; k < AT_MAX_CLUSTER; ++k)
+            {
+                // (an empty share has no part)
+                const bool part = k < C && units * k / C < units * (k + 1) / C;
+                ml[k] = part ? at_ld_cluster2(at_map(mine + (ROWS * D + 2 * r) * 4, k)) : make_float2(-INFINITY, 0.0f);
+                y[k] = part ? at_ld_cluster4(at_map(mine + (r * D + c) * 4, k)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                m = fmaxf(m, ml[k].x);
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+            #pragma unroll
+            for (int k = 0; k < AT_MAX_CLUSTER; ++k)
+            {
+                const float f = at_exp2(ml[k].x - base);
+                l += ml[k].x == -INFINITY ? ml[k].y : ml[k].y * f;           // (an l of NaN stays one)
+                x.x += y[k].x * f; x.y += y[k].y * f; x.z += y[k].z * f; x.w += y[k].w * f;
+            }
+            at_store<T>(P, in.s, tok, in.h * group + row - tok * group, c, x, m, l);
+        }
+        at_cluster_sync();
     }
 }
 
@@ -704,10 +775,19 @@ static const AtDevice* at_device(int* rc)
     return &devices[dev];
 }
 
-// Sequences that fit into this many keys are not split: nothing is joined then
-constexpr int AT_WHOLE_KEYS = 256;
+// Sequences that see few keys are not cut into ranges: a cluster of up to eight CTAs has each of their segments and joins in shared memory, no
+// second kernel follows. Up to AT_WHOLE_KEYS however many segments there are, beyond where at least two CTAs find places for each (the
+// lengths may differ). us, equal ranges / this (32 query heads on 8 key-value heads of 128 values): one sequence of 512 and 1024 keys 8.1 / 6.6
+// and 8.4 / 7.0, of 2048 8.9 / 9.0; four of 300 and 2000 11.5 / 9.4 and 14.6 / 12.8; 32 of 300 19.1 / 13.0; but 32 of 50 to 2000 keys,
+// a CTA each, 29.6 / 39.4
+constexpr int AT_WHOLE_KEYS = 512, AT_CLUSTER_KEYS = 2048;
 // Rows (tokens x group) up to which a sequence takes the split form, whose ranges follow the lengths; beyond, the prompt form
 constexpr int AT_SPLIT_ROWS = 64;
+
+constexpr long AT_SM_BYTES = 228 * 1024;       // of shared memory, per SM
+
+template <int D> static int at_smem_rows(int wr) { return wr == 1 ? at_smem<D, 1> : wr == 2 ? at_smem<D, 2> : at_smem<D, 4>; }
+static int at_smem_bytes(int dim, int wr) { return dim == 64 ? at_smem_rows<64>(wr) : dim == 128 ? at_smem_rows<128>(wr) : at_smem_rows<256>(wr); }
 
 static int at_grid(int dim, int sms) { return sms * (dim == 64 ? at_ctas<64> : dim == 128 ? at_ctas<128> : at_ctas<256>); }
 
@@ -715,7 +795,7 @@ static int at_grid(int dim, int sms) { return sms * (dim == 64 ? at_ctas<64> : d
 struct AtCut
 {
     bool split, tc;                            // forms that are launched
-    int whole, grid, wr;                       // split form: 16 * wr rows per row tile
+    int cluster, grid, wr;                     // split form: CTAs per segment (0: equal ranges), CTAs, 16 * wr rows per row tile
     int nq, tiles, slices;                     // prompt form
     size_t tc_offset, bytes;                   // of the workspace
 };
@@ -740,11 +820,18 @@ static AtCut at_cut(int tokens, int seqs, int heads, int kv_heads, int dim, bool
     const long group = heads / kv_heads, all = tokens * group, each = all / seqs;
     C.split = ragged || each <= AT_SPLIT_ROWS;
     C.tc = ragged ? all > AT_SPLIT_ROWS : !C.split;
-    C.whole = C.split && !ragged && max_keys <= AT_WHOLE_KEYS;
     C.grid = at_grid(dim, sms);
     const long rows = ragged ? group : each;   // (ragged: single tokens are the rule)
     C.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    if (C.split && !C.whole) C.bytes = (2 * C.grid * at_part_floats(16 * C.wr, dim) * 4 + 127) / 128 * 128;
+    const long seen = window ? min(max_keys, (long) window + sinks + tokens / seqs) : max_keys;
+    if (C.split && !ragged && seen <= AT_CLUSTER_KEYS)
+    {
+        const long segments = seqs * kv_heads * ((each + 16 * C.wr - 1) / (16 * C.wr)), unit = 4 / C.wr * (dim == 256 ? 16 : 32);
+        const long places = sms * min((long) C.grid / sms, AT_SM_BYTES / (at_smem_bytes(dim, C.wr) + (long) at_part_floats(16 * C.wr, dim) * 4 + 2048));
+        for (C.cluster = 1; C.cluster < AT_MAX_CLUSTER && 2 * C.cluster * segments <= places && 2 * C.cluster * unit < seen + unit; C.cluster *= 2) { }
+        if (C.cluster == 1 && seen > AT_WHOLE_KEYS) C.cluster = 0;
+    }
+    if (C.split && !C.cluster) C.bytes = (2 * C.grid * at_part_floats(16 * C.wr, dim) * 4 + 127) / 128 * 128;
     C.tc_offset = C.bytes;
     C.slices = 1;
     if (C.tc)
@@ -764,13 +851,15 @@ static AtCut at_cut(int tokens, int seqs, int heads, int kv_heads, int dim, bool
     return C;
 }
 
-template <typename T, int D, int WR>
+template <typename T, int D, int WR, bool CLUSTER>
 static int at_launch(AtPlan& S, cudaStream_t stream)
 {
     const amp_attention_args& P = S.P;
+    // (a cluster's part)
+    const int bytes = at_smem<D, WR> + (CLUSTER && S.cluster > 1 ? (int) at_part_floats(at_rows<WR>, D) * 4 : 0);
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return cuda_rc(e, "attention device");
-    if (cudaError_t e = ensure_smem(attention_split_kernel<T, D, WR>, at_smem<D, WR>, dev)) return cuda_rc(e, "attention shared memory");
+    if (cudaError_t e = ensure_smem(attention_split_kernel<T, D, WR, CLUSTER>, bytes, dev)) return cuda_rc(e, "attention shared memory");
     S.unit = at_unit<D, WR>;
     S.rows = 16 * WR;
     const long group = P.heads / P.kv_heads;
@@ -778,20 +867,29 @@ static int at_launch(AtPlan& S, cudaStream_t stream)
                 "attention: more keys than one call takes (%d sequences of up to %ld)", P.seqs, (long) P.max_pages * P.page_size);
     // (segments of the call, where the host knows them)
     const long rows = (long) (P.tokens / P.seqs) * group, segments = (long) P.seqs * P.kv_heads * ((rows + S.rows - 1) / S.rows);
-    const long grid = S.whole ? segments : S.grid;
+    const long grid = CLUSTER ? segments * S.cluster : S.grid;
     AMP_REQUIRE(grid < (1l << 31), "attention: too many sequences");
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    int attrs = S.pdl ? 1 : 0;
+    if (CLUSTER && S.cluster > 1)
+    {
+        attr[attrs].id = cudaLaunchAttributeClusterDimension;
+        attr[attrs].val.clusterDim.x = S.cluster;
+        attr[attrs].val.clusterDim.y = attr[attrs].val.clusterDim.z = 1;
+        ++attrs;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) grid, 1, 1);
     cfg.blockDim = dim3(AT_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = at_smem<D, WR>;
+    cfg.dynamicSmemBytes = bytes;
     cfg.stream = stream;
     cfg.attrs = attr;
+    cfg.numAttrs = attrs;
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, attention_split_kernel<T, D, WR, CLUSTER>, (const AtPlan) S)) return cuda_rc(e, "attention launch");
+    if (CLUSTER) return 0;
     cfg.numAttrs = S.pdl ? 1 : 0;
-    if (cudaError_t e = cudaLaunchKernelEx(&cfg, attention_split_kernel<T, D, WR>, (const AtPlan) S)) return cuda_rc(e, "attention launch");
-    if (S.whole) return 0;
     S.by_segment = !P.cu && segments < S.grid;
     // a row per CTA; with cu there may be up to 64 of them and most CTAs have none: four CTAs go through all (2333 tokens of six prompts,
     // none of which is the split form's: 49.1 us with a row per CTA, 44.4)
@@ -805,7 +903,8 @@ static int at_launch(AtPlan& S, cudaStream_t stream)
 template <typename T, int D>
 static int at_launch_rows(AtPlan& S, int wr, cudaStream_t stream)
 {
-    return wr == 1 ? at_launch<T, D, 1>(S, stream) : wr == 2 ? at_launch<T, D, 2>(S, stream) : at_launch<T, D, 4>(S, stream);
+    if (S.cluster) return wr == 1 ? at_launch<T, D, 1, true>(S, stream) : wr == 2 ? at_launch<T, D, 2, true>(S, stream) : at_launch<T, D, 4, true>(S, stream);
+    return wr == 1 ? at_launch<T, D, 1, false>(S, stream) : wr == 2 ? at_launch<T, D, 2, false>(S, stream) : at_launch<T, D, 4, false>(S, stream);
 }
 
 template <typename T>
@@ -858,7 +957,7 @@ AMP_API int amp_b200_attention(const amp_attention_args* args, cudaStream_t stre
         AMP_REQUIRE(P.workspace && ((uintptr_t) P.workspace & 15) == 0 && P.workspace_bytes >= (long) C.bytes, "attention: workspace too small or misaligned");
     if (C.split)
     {
-        S.grid = C.grid; S.whole = C.whole; S.pdl = g_pdl; S.split_rows = P.cu ? AT_SPLIT_ROWS : 1 << 30;
+        S.grid = C.grid; S.cluster = C.cluster; S.pdl = g_pdl; S.split_rows = P.cu ? AT_SPLIT_ROWS : 1 << 30;
         S.scale2 = P.scale * 1.4426950408889634f; S.g = g;
         rc = P.bf16 ? at_launch_dim<__nv_bfloat16>(S, C.wr, stream) : at_launch_dim<__half>(S, C.wr, stream);
         if (rc) return rc;
