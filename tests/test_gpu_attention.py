@@ -46,18 +46,21 @@ def check(amp, pos, counts, hq, hkv, d, page, dtype, window=0, sinks=0, ragged=F
     return out
 
 
-@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("dtype,wide", [(H, 0), (B, 0), (H, 200)])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (8, 8), (8, 2), (6, 1), (5, 1), (14, 2), (16, 1), (40, 2)])
-def test_one_token(amp, dtype, d, hq, hkv):
+def test_one_token(amp, dtype, d, hq, hkv, wide):
     """Every group size, rows that fill a row tile and rows that do not; lengths 1, 2, around the units' ends, none"""
     pos = [0, 1, 14, 15, 16, 62, 63, 64, 127, 128, -1, 700]
-    check(amp, pos, [1] * len(pos), hq, hkv, d, 16, dtype)
+    check(amp, pos, [1] * len(pos), hq, hkv, d, 16, dtype, wide=wide)
 
 
 @pytest.mark.parametrize("page", [1, 3, 16, 24, 64, 100, 256, 1000])
 def test_pages_that_end_inside_a_unit(amp, page):
     check(amp, [0, 99, 517, 64], [1] * 4, 8, 2, 128, page, H, wide=2)
+    check(amp, [0, 99, 517, 64], [1] * 4, 8, 2, 128, page, H, wide=-(-2500 // page))
+    for wide in (2, -(-2500 // page)):
+        check(amp, [0, 117], [70, 70], 8, 2, 128, page, B, wide=wide)
 
 
 @pytest.mark.parametrize("length", [1, 63, 64, 65, 255, 256, 257, 1000, 9001])
@@ -65,12 +68,13 @@ def test_one_sequence_over_the_whole_device(amp, length):
     check(amp, [length - 1], [1], 4, 1, 128, 64, B, pos_dtype=torch.int64)
 
 
+@pytest.mark.parametrize("wide", [0, 200])                              # (long tables: equal ranges instead of clusters)
 @pytest.mark.parametrize("count", [2, 3, 4, 5, 7, 16, 33])
 @pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (6, 1, 64), (3, 3, 256), (32, 2, 128)])
-def test_several_tokens_per_sequence(amp, count, hq, hkv, d):
+def test_several_tokens_per_sequence(amp, count, hq, hkv, d, wide):
     """Drafted tokens: each sees the ones in front of it; sequences that begin with the call, and one that begins inside it"""
     pos = [0, 100, 300, 1, -1, -count]
-    check(amp, pos, [count] * len(pos), hq, hkv, d, 16, B)
+    check(amp, pos, [count] * len(pos), hq, hkv, d, 16, B, wide=wide)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (2, 4), (16, 0), (64, 4), (100, 1), (100, 200), (5000, 3)])
@@ -86,24 +90,84 @@ def test_sinks_without_a_window_change_nothing(amp):
     assert torch.equal(amp.paged_attention(q, k, v, table, pos), amp.paged_attention(q, k, v, table, pos, sinks=4))
 
 
-@pytest.mark.parametrize("d,dtype", [(64, B), (128, H), (128, B), (256, H)])
+@pytest.mark.parametrize("d,dtype,wide", [(64, B, 0), (128, H, 0), (128, B, 100), (256, H, 0), (64, H, 100)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
-def test_mixed_ragged(amp, d, dtype, window, sinks):
+def test_mixed_ragged(amp, d, dtype, window, sinks, wide):
     """Single tokens, drafts, prompts, empty sequences in one call"""
     counts = [1, 200, 0, 3, 77, 1, 0, 129]
     pos = [900, 0, 5, 63, 64, -1, 0, 31]
-    check(amp, pos, counts, 8, 2, d, 16, dtype, window, sinks, ragged=True)
+    check(amp, pos, counts, 8, 2, d, 16, dtype, window, sinks, ragged=True, wide=wide)
 
 
+@pytest.mark.parametrize("wide", [0, 200])                              # (long tables: two row tiles per CTA instead of one)
 @pytest.mark.parametrize("count,first", [(64, 0), (300, 0), (257, 1000), (130, 7)])
 @pytest.mark.parametrize("hq,hkv,d,dtype", [(8, 2, 128, H), (5, 1, 64, B), (4, 4, 128, B), (2, 1, 256, B), (32, 2, 64, H)])
-def test_prompt_chunks(amp, count, first, hq, hkv, d, dtype):
-    check(amp, [first], [count], hq, hkv, d, 24, dtype)
+def test_prompt_chunks(amp, count, first, hq, hkv, d, dtype, wide):
+    check(amp, [first], [count], hq, hkv, d, 24, dtype, wide=wide)
+
+
+def test_a_prompt_of_many_tiles(amp):
+    """Whole waves of CTAs, no slices; every eleventh row is checked"""
+    n, hq, hkv, d = 2600, 8, 8, 128
+    q, k, v, table = make([0], [n], hq, hkv, d, 64, H)
+    out = amp.paged_attention(q, k, v, table, torch.tensor([0], device="cuda"))
+    rows = list(range(0, n, 11)) + [n - 1]
+    for r0 in range(0, len(rows), 60):
+        part = rows[r0:r0 + 60]
+        pos = part
+        want, _, tol, _ = ac.attention(q[part], k, v, table.expand(len(part), -1), pos, [1] * len(part), 0, 0, d ** -0.5)
+        assert ((out[part].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.5, 1.0, 0.003])
+@pytest.mark.parametrize("wide", [0, 200])
+def test_scales_of_prompts(amp, scale, wide):
+    check(amp, [40], [90], 4, 2, 128, 16, H, scale=scale, wide=wide)
+
+
+def test_many_sequences_of_different_lengths(amp):
+    """More segments than CTAs, more sequences than a warp counts by itself: ranges over all of them"""
+    g = torch.Generator().manual_seed(6)
+    pos = torch.randint(-1, 120, (220,), generator=g).tolist()
+    pos[7], pos[100], pos[219] = 2500, 1900, 3000
+    check(amp, pos, [1] * 220, 8, 2, 128, 16, H)
+    check(amp, pos, [1] * 220, 4, 4, 64, 16, B)
+    check(amp, pos[:40], [1] * 40, 4, 2, 256, 64, B)
+
+
+@pytest.mark.parametrize("counts", [[1, 60, 0, 3], [64, 0, 0, 0], [0, 0, 0, 0], [16, 16, 16, 16]])
+def test_captured_ragged_calls_replay_with_other_cuts(amp, counts):
+    rows = 64
+    q, k, v, table = make([300] * 4, [rows] * 4, 4, 2, 128, 16, H)
+    k, v = torch.nan_to_num(k, 1.0, 1.0, -1.0), torch.nan_to_num(v, 1.0, 1.0, -1.0)
+    table = table.clamp(0, k.shape[0] - 1)
+    q = q[:rows].contiguous()
+    pos, cu, out = torch.tensor([5, 5, 5, 5], device="cuda"), cu_of([16, 16, 16, 16]), torch.zeros_like(q)
+    amp.paged_attention(q, k, v, table, pos, cu=cu, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        amp.paged_attention(q, k, v, table, pos, cu=cu, out=out)
+    pos.copy_(torch.tensor([200, 17, -1, 90]))
+    cu.copy_(cu_of(counts))
+    out.fill_(5.0)
+    graph.replay()
+    want = amp.paged_attention(q, k, v, table, pos, cu=cu, out=torch.full_like(q, 5.0))
+    assert torch.equal(out, want) and (out[sum(counts):] == 5.0).all()
+    ref, _, tol, _ = ac.attention(q, k, v, table, [200, 17, -1, 90], counts, 0, 0, 128 ** -0.5)
+    n = sum(counts)
+    assert ((out[:n].double() - ref[:n]).abs() <= tol[:n]).all()
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (30, 4), (128, 4), (200, 500)])
-def test_prompt_chunks_in_a_window(amp, window, sinks):
-    check(amp, [0, 600], [260, 260], 8, 2, 64, 16, B, window, sinks)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompt_chunks_in_a_window(amp, window, sinks, d):
+    check(amp, [0, 600], [260, 260], 8, 2, d, 16, B, window, sinks)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_chunks_in_a_long_window(amp, d):
+    """Windows long enough for two row tiles per CTA, in a context longer than they are"""
+    check(amp, [2300], [140], 4, 1, d, 16, H, 1700, 5)
 
 
 def test_scales(amp):
@@ -121,17 +185,19 @@ def test_peaked_scores(amp):
     assert ((out.double() - want).abs() <= tol).all()
 
 
-def test_strides(amp):
+@pytest.mark.parametrize("count,extra", [(2, 0), (2, 200), (90, 0), (90, 200)])
+def test_strides(amp, count, extra):
     """q out of a packed q|k|v row, caches stored per head, caches that are one layer of a larger tensor, out inside a larger one"""
-    pos, counts, hq, hkv, d = [333, 20], [2, 2], 8, 2, 128
-    q, k, v, table = make(pos, counts, hq, hkv, d, 16, H)
+    pos, counts, hq, hkv, d = [333, 20], [count] * 2, 8, 2, 128
+    n = 2 * count
+    q, k, v, table = make(pos, counts, hq, hkv, d, 16, H, wide=extra)
     want = amp.paged_attention(q, k, v, table, torch.tensor(pos, device="cuda"))
-    packed = torch.randn((4, (hq + 2 * hkv) * d), device="cuda").to(H)
-    packed[:, :hq * d] = q.view(4, -1)
-    qs = packed[:, :hq * d].view(4, hq, d)
+    packed = torch.randn((n, (hq + 2 * hkv) * d), device="cuda").to(H)
+    packed[:, :hq * d] = q.view(n, -1)
+    qs = packed[:, :hq * d].view(n, hq, d)
     kh, vh = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (k, v))
     both = torch.stack((k, v), 1)                                       # (pages, 2, page_size, ...)
-    wide = torch.zeros((4, 2 * hq, d), dtype=H, device="cuda")
+    wide = torch.zeros((n, 2 * hq, d), dtype=H, device="cuda")
     tab = torch.cat((table, table), 1)[:, :table.shape[1]]
     for kk, vv in ((kh, vh), (k, vh), (both[:, 0], both[:, 1])):
         got = amp.paged_attention(qs, kk, vv, tab, torch.tensor(pos, device="cuda"), out=wide[:, hq:])
@@ -158,11 +224,12 @@ def test_rows_behind_the_last_sequence_are_left(amp, counts):
     assert (out[n:] == 3.0).all() and (lse[n:] == 5.0).all() and torch.isfinite(out[:n]).all()
 
 
+@pytest.mark.parametrize("wide", [0, 200])
 @pytest.mark.parametrize("count", [1, 3, 200])
-def test_pages_outside_the_pool_give_nan_in_their_rows_alone(amp, count):
+def test_pages_outside_the_pool_give_nan_in_their_rows_alone(amp, count, wide):
     """A table that names no page, or ends too early, is not read from; the other sequences keep their bits"""
     pos = [500, 500, 500, 1 << 40]
-    q, k, v, table = make([500] * 4, [count] * 4, 4, 2, 128, 16, H)
+    q, k, v, table = make([500] * 4, [count] * 4, 4, 2, 128, 16, H, wide=wide)
     p = torch.tensor([500] * 4, dtype=torch.int64, device="cuda")
     want = amp.paged_attention(q, k, v, table, p)
     broken = table.clone()
@@ -186,10 +253,12 @@ def test_far_positions_of_a_large_cache(amp):
     g = torch.Generator(device="cuda").manual_seed(3)
     for t in (k, v):
         t[pages - 8:] = torch.randn((8, page, hkv, d), device="cuda", generator=g).to(H)
-    q = torch.randn((1, 16, d), device="cuda", generator=g).to(H)
-    out = amp.paged_attention(q, k, v, table, torch.tensor([500], device="cuda"))
     small = torch.arange(7, -1, -1, dtype=torch.int32, device="cuda").view(1, 8)
-    assert torch.equal(out, amp.paged_attention(q, k[pages - 8:].clone(), v[pages - 8:].clone(), small, torch.tensor([500], device="cuda")))
+    for n in (1, 90):
+        q = torch.randn((n, 16, d), device="cuda", generator=g).to(H)
+        pos = torch.tensor([511 - n], device="cuda")
+        out = amp.paged_attention(q, k, v, table, pos)
+        assert torch.equal(out, amp.paged_attention(q, k[pages - 8:].clone(), v[pages - 8:].clone(), small, pos))
 
 
 def test_many_sequences(amp):

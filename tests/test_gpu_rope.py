@@ -79,6 +79,14 @@ def test_ragged_rows(amp, page, in_place):
     run(amp, [7, 0, 99, 3, 1], [1, 0, 33, 5, 0], 8, 2, 64, 30, page, B, True, ragged=True, extra=4, in_place=in_place)
 
 
+@pytest.mark.parametrize("seqs", [32, 33, 300])
+def test_rows_of_many_sequences(amp, seqs):
+    """Sequences found by a warp, and by the block"""
+    counts = torch.randint(0, 3, (seqs,), generator=torch.Generator().manual_seed(seqs)).tolist()
+    counts[-1] = 2
+    run(amp, [(7 * b) % 50 for b in range(seqs)], counts, 4, 2, 64, 64, 16, H, False, ragged=True, extra=3)
+
+
 @pytest.mark.parametrize("p", [131071, (1 << 20) - 1, (1 << 30) - 2])
 def test_far_positions(amp, p):
     """The angle is exact where an fp32 product is off by radians"""
