@@ -251,7 +251,7 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
     h // (heads / kv_heads). scale: 1 / sqrt(dim) by default. Returns out (rows, heads, dim), q's type, which must not overlap q; lse (rows, heads) float32, if
     given, takes ln sum_j exp(scale * q . k_j).
 
-    A token that sees nothing gets 0 (lse -inf). Pages that no token of the call can see are not read, and their table entries may hold
+    An infinite or NaN key or value reaches the tokens that see it, no others. A token that sees nothing gets 0 (lse -inf). Pages that no token of the call can see are not read, and their table entries may hold
     anything; a token with a visible key on a page outside the pool, or beyond the table, gets NaN. Single tokens, a few drafted ones and
     prompt chunks may be mixed in one call with cu."""
     name = "paged_attention"
@@ -283,8 +283,8 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
     if window < 0 or sinks < 0:
         raise ValueError("%s: window and sinks must not be negative" % name)
     scale = dim ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("%s: scale must be finite" % name)
+    if not abs(scale) * math.log2(math.e) < 3.4e38:
+        raise ValueError("%s: scale must be finite (in float32, as scores in powers of two)" % name)
     if out is None:
         out = torch.empty((rows, heads, dim), dtype=dtype, device=q.device)
         os = (heads * dim, dim)

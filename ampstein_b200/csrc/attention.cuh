@@ -6,6 +6,7 @@
 // Key j lives in row j % page_size of page table[b][j / page_size]. A token that sees nothing gets o = 0, lse = -inf; one whose
 // keys lie on a page outside the pool, or whose position is beyond the table, gets NaN (nothing outside the pool is read).
 #pragma once
+#include <cmath>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "exl3_gemv_kernel.cuh"
@@ -112,17 +113,47 @@ __device__ __forceinline__ float at_exp2(float x)
     return y;
 }
 
+// odd: bits 15 and 31 are set for a value without a finite magnitude (its exponent is all ones: one more carries out of it), the others are
+// of no matter
 template <typename T> struct AtType;
 template <> struct AtType<__half>
 {
+    static __device__ __forceinline__ uint32_t odd(uint32_t x) { return (x & 0x7c007c00u) + 0x04000400u; }
+    static __device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
     static __device__ __forceinline__ __half from(float a) { return __float2half_rn(a); }
 };
 template <> struct AtType<__nv_bfloat16>
 {
+    static __device__ __forceinline__ uint32_t odd(uint32_t x) { return (x & 0x7f807f80u) + 0x00800080u; }
+    static __device__ __forceinline__ float2 unpack(uint32_t x) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x)); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
     static __device__ __forceinline__ __nv_bfloat16 from(float a) { return __float2bfloat16_rn(a); }
 };
+
+// An infinite or NaN value times the weight 0 of a row that does not see its key would be NaN. Where keys are seen by some rows only,
+// such values are therefore taken out of the product, and added to the rows that do see them.
+constexpr uint32_t AT_ODD = 0x80008000u;
+
+template <typename T>
+__device__ __forceinline__ uint32_t at_odd(uint4 v) { return (AtType<T>::odd(v.x) | AtType<T>::odd(v.y) | AtType<T>::odd(v.z) | AtType<T>::odd(v.w)) & AT_ODD; }
+
+template <typename T>
+__device__ __forceinline__ uint32_t at_even(uint32_t x) { return x & ~((AtType<T>::odd(x) >> 15 & 0x00010001u) * 0xffffu); }      // they are 0
+
+__device__ __forceinline__ uint4 at_lds16(uint32_t addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void at_sts16_even(uint32_t addr, uint4 v)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                 :: "r"(addr), "r"(at_even<T>(v.x)), "r"(at_even<T>(v.y)), "r"(at_even<T>(v.z)), "r"(at_even<T>(v.w)) : "memory");
+}
 
 // 16 bytes to shared memory, or zeros
 __device__ __forceinline__ void at_copy16(uint32_t dst, const void* src, bool live)

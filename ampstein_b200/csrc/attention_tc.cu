@@ -210,6 +210,41 @@ __device__ __forceinline__ TaPlace ta_find(const TaPlan& S, int x)
     return f;
 }
 
+// A tile of values loses what has no finite magnitude, of keys that not all rows see, [0, from) and [to, count). By one warp, the one that
+// multiplies: it has nothing to do while the weights are made, and its loop bears another branch: 8192 tokens 495 -> 497 us, six
+// prompts of 390 tokens in windows of 128 32.3 -> 32.8 (the same work in the loading warps' loop: 4 to 26 us, and 2.5). Whether there was any.
+template <typename T, int D, int KB>
+__device__ __forceinline__ bool ta_sift(uint32_t at, int from, int to, int count)
+{
+    constexpr int CH = D / 8, PER = CH >= 32 ? 1 : 32 / CH, COPIES = KB / PER, BATCH = 4;
+    const int lane = threadIdx.x & 31, r_lane = CH >= 32 ? 0 : lane / CH, c_lane = lane % CH;
+    at += (c_lane >> 3) * (KB * 128);
+    auto place = [&](int r) { return at + r * 128 + (((c_lane & 7) ^ (r & 7)) << 4); };
+    // (of a tile that begins or ends among the keys that all rows see, only the other end)
+    const int first = from <= 0 && to > 0 ? to / PER : 0, end = from > 0 && to >= KB ? min(from, count) : count, last = min(COPIES, (end + PER - 1) / PER);
+    uint32_t odd = 0;
+    #pragma unroll 1
+    for (int i = first; i < last; i += BATCH)
+    {
+        uint4 v[BATCH];
+        #pragma unroll
+        for (int a = 0; a < BATCH; ++a) v[a] = at_lds16(place(min(i + a, last - 1) * PER + r_lane));
+        #pragma unroll
+        for (int a = 0; a < BATCH; ++a) odd |= at_odd<T>(v[a]);
+    }
+    if (!__any_sync(0xffffffffu, odd)) return false;
+    #pragma unroll 1
+    for (int i = first; i < last; ++i)
+    {
+        const int r = i * PER + r_lane;
+        const uint4 v = at_lds16(place(r));
+        if (at_odd<T>(v) && (r < from || r >= to)) at_sts16_even<T>(place(r), v);
+    }
+    ta_fence_async();
+    __syncwarp();
+    return true;
+}
+
 template <typename T, int D, int NQ>
 __global__ __launch_bounds__(ta_threads<NQ>, (ta_ctas<D, NQ>))
 void attention_tc_kernel(const TaPlan S)
@@ -225,6 +260,7 @@ void attention_tc_kernel(const TaPlan S)
     extern __shared__ __align__(1024) unsigned char ta_mem[];
     __shared__ uint64_t q_full, kv_full[ST], kv_free[ST], s_full[2], p_full[4], pv_done, o_full, end;
     __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_odd;             // values without a finite magnitude were taken out of tiles that some rows see in part
     __shared__ TaPlace s_place;
 
     const int t = threadIdx.x, lane = t & 31, warp = __shfl_sync(0xffffffffu, t >> 5, 0);
@@ -245,6 +281,7 @@ void attention_tc_kernel(const TaPlan S)
     }
     else if (warp == 1 && lane == 0)
     {
+        s_odd = 0;
         mbar_init(&q_full, 128 * NQ);
         for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], TA_LOADERS); mbar_init(&kv_free[i], 1); }
         for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
@@ -420,6 +457,52 @@ void attention_tc_kernel(const TaPlan S)
             wait(smem_u32(&o_full), 0);
             ta_fence_after();
         }
+        // columns to which such values are added: infinity, minus infinity (both: NaN)
+        uint32_t up[D / 32] = {}, down[D / 32] = {};
+        const bool odd = s_odd;
+        if (odd)
+        {
+            int whole_from, whole_to;          // (as the warp that multiplies has them)
+            at_whole_keys(P, keys, seq.first + tok0, seq.first + tok1, whole_from, whole_to);
+            const int end = min((j0 + n) * KB, keys.count());
+            #pragma unroll 1
+            for (int c = j0 * KB; c < end; ++c)
+            {
+                if (c >= whole_from && c < whole_to) { c = whole_to - 1; continue; }
+                if (!have || !(c < n0 || (uint32_t) (c - c1) <= (uint32_t) len)) continue;
+                const int key = keys.key(c), pg = S.g.page_of(key), page = P.table[(long long) s_place.b * P.table_row + pg];
+                if ((unsigned) page >= (unsigned) P.pages) continue;
+                const uint4* const v = reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(P.v_cache) + h * P.v_head * 2
+                                       + (unsigned long long) (page * S.g.v_page + (key - pg * P.page_size) * S.g.v_row) * 16);
+                #pragma unroll
+                for (int i = 0; i < D / 32; ++i)
+                {
+                    #pragma unroll 1
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        const uint4 x = v[4 * i + e];
+                        if (!at_odd<T>(x)) continue;
+                        const uint32_t y[4] = { x.x, x.y, x.z, x.w };
+                        #pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                        {
+                            const float2 z = AtType<T>::unpack(y[k]);
+                            const uint32_t is = AtType<T>::odd(y[k]), first = (is >> 15 & 1u) << (8 * e + 2 * k), second = (is >> 31) << (8 * e + 2 * k + 1);
+                            up[i] |= (z.x < 0.0f ? 0 : first) | (z.y < 0.0f ? 0 : second);
+                            down[i] |= (z.x > 0.0f ? 0 : first) | (z.y > 0.0f ? 0 : second);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+        }
+        auto mend = [&](int i, uint32_t* o)
+        {
+            if (!odd) return;
+            #pragma unroll
+            for (int e = 0; e < 32; ++e)
+                o[e] = __float_as_uint(__uint_as_float(o[e]) + (up[i] >> e & 1 ? INFINITY : 0.0f) + (down[i] >> e & 1 ? -INFINITY : 0.0f));
+        };
         const float m2 = m == -INFINITY ? m : m * sc;
         if (S.slices > 1)
         {
@@ -434,6 +517,7 @@ void attention_tc_kernel(const TaPlan S)
                     uint32_t o[32];
                     ta_ld32(o_t + c, o);
                     ta_wait_ld();
+                    mend(c / 32, o);
                     if (have)
                     {
                         #pragma unroll
@@ -451,7 +535,7 @@ void attention_tc_kernel(const TaPlan S)
             for (int c = 0; c < D; c += 32)
             {
                 uint32_t o[32];
-                if (n > 0) { ta_ld32(o_t + c, o); ta_wait_ld(); }
+                if (n > 0) { ta_ld32(o_t + c, o); ta_wait_ld(); mend(c / 32, o); }
                 if (have)
                 {
                     #pragma unroll
@@ -493,6 +577,9 @@ void attention_tc_kernel(const TaPlan S)
             }
             __syncwarp();
         };
+        int whole_from, whole_to;              // keys that all rows of the CTA see
+        at_whole_keys(P, keys, seq.first + tok0, seq.first + tok1, whole_from, whole_to);
+        const int count = keys.count();
         auto commit = [&](uint32_t bar) { if (ta_elect()) ta_commit(bar); __syncwarp(); };
         if (n > 0 && wait(smem_u32(&q_full), 0) && wait(full_s + 8 * stage, wrap))
         {
@@ -517,6 +604,9 @@ void attention_tc_kernel(const TaPlan S)
                 if (!wait(full_s + 8 * stage, wrap)) break;
                 const int vst = stage;
                 next();
+                const int k0 = (j0 + j) * KB;
+                if ((k0 < whole_from || min(k0 + KB, count) > whole_to) && ta_sift<T, D, KB>(kv_s + vst * KV_BYTES, whole_from - k0, whole_to - k0, count - k0))
+                    s_odd = 1;
                 #pragma unroll
                 for (int i = 0; i < NQ; ++i)
                 {

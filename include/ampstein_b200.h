@@ -274,8 +274,7 @@ int amp_b200_rope(const amp_rope_args* args, cudaStream_t stream);
  * 0: a slot without a sequence) gets 0 and an lse of -inf. A token whose visible keys lie on a page outside the pool, or
  * that stands beyond the table, gets NaN. Scores, softmax and sums are in fp32, the weights are rounded to the values' type for the
  * product with them. A call gives the same bits every time. dim: 64, 128 or 256.
- * A key or value that some token of a sequence sees should be finite where another of its tokens in the call does not see it:
- * an infinite or NaN value reaches the row of a token nearby through a weight of 0.
+ * An infinite or NaN key or value reaches the tokens that see it, no others.
  * workspace: amp_b200_attention_workspace bytes on the device, 16-byte aligned, contents of no matter (ragged: with cu; max_keys =
  * max_pages * page_size; 0 bytes: none is needed); calls that may overlap need one each.
  */

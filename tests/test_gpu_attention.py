@@ -243,6 +243,49 @@ def test_pages_outside_the_pool_give_nan_in_their_rows_alone(amp, count, wide):
     assert (none[:count] == 0).all() and none[count:2 * count].isnan().all()
 
 
+@pytest.mark.parametrize("wide", [0, 200])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (30, 3)])
+@pytest.mark.parametrize("count", [2, 5, 16, 40, 150])
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(8, 2, 128, H), (3, 1, 64, B), (4, 2, 256, H)])
+def test_infinities_and_nan_reach_the_rows_that_see_them_alone(amp, hq, hkv, d, dtype, count, window, sinks, wide):
+    """A padded batch's spare rows, a token whose projections overflowed: other tokens of the call do not see those keys"""
+    pos, page = [300, 0], 16
+    q, k, v, table = make(pos, [count] * 2, hq, hkv, d, page, dtype, window, sinks, wide=wide)
+    odd = torch.zeros_like(v, dtype=torch.bool)
+    inf, nan = math.inf, math.nan
+
+    def put(b, j, head, values):
+        if j < 0 or not any(j in ac.visible(pos[b] + t, window, sinks) for t in range(count)):
+            return
+        at = int(table[b, j // page]), j % page, head
+        for c, x in values.items():
+            v[at][c % d] = x
+            odd[at][c % d] = True
+
+    for b in range(2):
+        last = pos[b] + count - 1
+        put(b, last, 0, {0: inf, 1: -inf, 2: nan, 33: inf, d - 1: -inf})
+        put(b, last - 1, 0, {0: inf, 33: -inf, 40: nan, 63: inf})
+        put(b, last, hkv - 1, {5: nan})
+        put(b, pos[b] + count // 2, hkv - 1, {c: inf for c in range(d // 2, d)})
+        put(b, pos[b] - window + 2, 0, {7: inf, 8: -inf, 62: nan})          # the window leaves it behind soon
+        put(b, pos[b] + 1, 0, {9: nan})
+    clean = torch.where(odd, torch.zeros_like(v), v)
+    lse = torch.zeros((2 * count, hq), device="cuda")
+    out = amp.paged_attention(q, k, v, table, torch.tensor(pos, device="cuda"), window=window, sinks=sinks, lse=lse)
+    want, wlse, tol, ltol = ac.attention(q, k, clean, table, pos, [count] * 2, window, sinks, d ** -0.5)
+    up, down = torch.zeros_like(out, dtype=torch.bool), torch.zeros_like(out, dtype=torch.bool)
+    kinds = [(odd & ~(v < 0)).repeat_interleave(hq // hkv, 2), (odd & ~(v > 0)).repeat_interleave(hq // hkv, 2)]
+    for row, (b, p) in enumerate(ac.tokens(pos, [count] * 2)):
+        js = torch.tensor(ac.visible(p, window, sinks), device="cuda")
+        pages, rows = table[b, js // page].long(), js % page
+        up[row], down[row] = (x[pages, rows].any(0) for x in kinds)
+    fine = ~up & ~down
+    assert fine.any() and up.any() and down.any() and ((out.double() - want).abs() <= tol)[fine].all()
+    assert (out[up & ~down] == inf).all() and (out[down & ~up] == -inf).all() and out[up & down].isnan().all()
+    assert ((lse.double() - wlse).abs() <= ltol).all()
+
+
 def test_far_positions_of_a_large_cache(amp):
     """Offsets that pass 32 bits: 5 GB of keys"""
     page, hkv, d = 64, 8, 128
@@ -342,6 +385,7 @@ def test_refusals(amp):
         (ValueError, lambda: f(torch.cat((q, q[:1])), k, v, table, pos)),
         (ValueError, lambda: f(q, k, v, table, pos, window=-1)),
         (ValueError, lambda: f(q, k, v, table, pos, scale=math.nan)),
+        (ValueError, lambda: f(q, k, v, table, pos, scale=3e38)),
         (ValueError, lambda: f(q, k, v, table, pos, out=q)),
         (ValueError, lambda: f(q, k, v, table, pos, lse=torch.zeros((2, 3), device="cuda"))),
         (ValueError, lambda: f(q.transpose(1, 2).contiguous().transpose(1, 2), k, v, table, pos)),

@@ -217,7 +217,7 @@ def test_entries_refuse_before_any_cuda_call():
         assert rc < 0 and text.startswith("rope"), (change, rc, text)
     for change in (dict(q=0), dict(out=0), dict(table=0), dict(pos=0), dict(tokens=-3), dict(tokens=5), dict(seqs=1 << 21, tokens=1 << 21), dict(heads=3, kv_heads=2),
                    dict(kv_heads=0), dict(dim=96), dict(pages=0), dict(page_size=0), dict(max_pages=1 << 28), dict(window=-1), dict(sinks=-1), dict(q=p + 2),
-                   dict(strides=[64] * 4 + [60] + [64] * 6), dict(scale=float("nan"))):
+                   dict(strides=[64] * 4 + [60] + [64] * 6), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=-3e38)):
         rc, text = run("amp_b200_attention", attention._ATTENTION, att, **change)
         assert rc < 0 and text.startswith("attention"), (change, rc, text)
     assert run("amp_b200_rope", attention._ROPE, rope, tokens=0)[0] == 0 and run("amp_b200_attention", attention._ATTENTION, att, seqs=0)[0] == 0
