@@ -48,6 +48,7 @@ struct AtPlan
     int cluster;                               // > 0: every (sequence, head, row tile) belongs to a cluster of so many CTAs, which join in shared memory
     int by_segment;                            // join: blockIdx.x is a segment, else the CTA whose range begins inside it
     int pdl;
+    int late;                                  // split form: the launches in front are the prompt form's, of other rows: waited for at the end
     float scale2;                              // scale * log2(e)
     AtPages g;
 };
@@ -265,7 +266,8 @@ void attention_split_kernel(const AtPlan S)
 
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, grp = warp / WR, wr = warp % WR, cta = blockIdx.x;
     const int group = P.heads / P.kv_heads;
-    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
+    // (late: what is in front of the prompt form is over, or that form had not let this one begin)
+    if (S.pdl) { if (!S.late) pdl_wait(); pdl_launch_dependents(); }
 
     // the CTA's range of units
     AtCursor in;
@@ -286,7 +288,7 @@ void attention_split_kernel(const AtPlan S)
     {
         AtCount C;
         C.count<NT>(S, s_scan);
-        if (cta >= C.ctas) return;
+        if (cta >= C.ctas) { if (S.late) pdl_wait(); return; }
         const int u0 = C.begin(cta);
         left = C.begin(cta + 1) - u0;
         int b, front;
@@ -294,7 +296,7 @@ void attention_split_kernel(const AtPlan S)
         in.place(S, b, u0 - front);
         if (in.u == in.units)                                // (the CTA in front ends that segment)
         {
-            if (--left == 0) return;
+            if (--left == 0) { if (S.late) pdl_wait(); return; }
             in.advance(S);
         }
     }
@@ -668,6 +670,7 @@ void attention_split_kernel(const AtPlan S)
         }
         at_cluster_sync();
     }
+    if (S.late) pdl_wait();
 }
 
 // Joins the parts of a segment, row blockIdx.y of it (LOOP: every gridDim.y-th from there): of segment blockIdx.x, or of the one that the range of
@@ -819,6 +822,7 @@ constexpr long AT_SM_BYTES = 228 * 1024;       // of shared memory, per SM
 template <int D> static int at_smem_rows(int wr) { return wr == 1 ? at_smem<D, 1> : wr == 2 ? at_smem<D, 2> : at_smem<D, 4>; }
 static int at_smem_bytes(int dim, int wr) { return dim == 64 ? at_smem_rows<64>(wr) : dim == 128 ? at_smem_rows<128>(wr) : at_smem_rows<256>(wr); }
 
+static int at_unit_keys(int dim, int wr) { return AT_WARPS / wr * (dim == 64 ? at_kw<64> : dim == 128 ? at_kw<128> : at_kw<256>); }
 static int at_grid(int dim, int sms) { return sms * (dim == 64 ? at_ctas<64> : dim == 128 ? at_ctas<128> : at_ctas<256>); }
 
 // How a call is cut up: by its sizes alone (the lengths are on the device)
@@ -856,7 +860,7 @@ static AtCut at_cut(int tokens, int seqs, int heads, int kv_heads, int dim, bool
     const long seen = window ? min(max_keys, (long) window + sinks + tokens / seqs) : max_keys;
     if (C.split && !ragged && seen <= AT_CLUSTER_KEYS)
     {
-        const long segments = seqs * kv_heads * ((each + 16 * C.wr - 1) / (16 * C.wr)), unit = 4 / C.wr * (dim == 256 ? 16 : 32);
+        const long segments = seqs * kv_heads * ((each + 16 * C.wr - 1) / (16 * C.wr)), unit = at_unit_keys(dim, C.wr);
         const long places = sms * min((long) C.grid / sms, AT_SM_BYTES / (at_smem_bytes(dim, C.wr) + (long) at_part_floats(16 * C.wr, dim) * 4 + 2048));
         for (C.cluster = 1; C.cluster < AT_MAX_CLUSTER && 2 * C.cluster * segments <= places && 2 * C.cluster * unit < seen + unit; C.cluster *= 2) { }
         if (C.cluster == 1 && seen > AT_WHOLE_KEYS) C.cluster = 0;
@@ -893,10 +897,6 @@ static int at_launch(AtPlan& S, cudaStream_t stream)
     S.unit = at_unit<D, WR>;
     S.rows = 16 * WR;
     const long group = P.heads / P.kv_heads;
-    // (whatever cu holds, a sequence has at most split_rows rows here)
-    const double tiles = P.cu ? (double) P.seqs * ((min((long) S.split_rows, P.tokens * group) + S.rows - 1) / S.rows) : (double) (P.tokens * group / S.rows + P.seqs);
-    AMP_REQUIRE(P.kv_heads * tiles * (P.max_pages * (double) P.page_size / S.unit + 2) < 2147483648.0,
-                "attention: more keys than one call takes (%d sequences of up to %ld)", P.seqs, (long) P.max_pages * P.page_size);
     // (segments of the call, where the host knows them)
     const long rows = (long) (P.tokens / P.seqs) * group, segments = (long) P.seqs * P.kv_heads * ((rows + S.rows - 1) / S.rows);
     const long grid = CLUSTER ? segments * S.cluster : S.grid;
@@ -989,14 +989,23 @@ AMP_API int amp_b200_attention(const amp_attention_args* args, cudaStream_t stre
         AMP_REQUIRE(P.workspace && ((uintptr_t) P.workspace & 15) == 0 && P.workspace_bytes >= (long) C.bytes, "attention: workspace too small or misaligned");
     if (C.split)
     {
-        S.grid = C.grid; S.cluster = C.cluster; S.pdl = g_pdl; S.split_rows = P.cu ? AT_SPLIT_ROWS : 1 << 30;
-        S.scale2 = P.scale * 1.4426950408889634f; S.g = g;
-        rc = P.bf16 ? at_launch_dim<__nv_bfloat16>(S, C.wr, stream) : at_launch_dim<__half>(S, C.wr, stream);
-        if (rc) return rc;
+        // units are counted in 32 bits (whatever cu holds, a sequence has at most AT_SPLIT_ROWS rows there)
+        const long group = P.heads / P.kv_heads, rows = 16 * C.wr;
+        const double tiles = P.cu ? (double) P.seqs * ((min((long) AT_SPLIT_ROWS, P.tokens * group) + rows - 1) / rows) : (double) (P.tokens * group / rows + P.seqs);
+        AMP_REQUIRE(P.kv_heads * tiles * (P.max_pages * (double) P.page_size / at_unit_keys(P.dim, C.wr) + 2) < 2147483648.0,
+                    "attention: more keys than one call takes (%d sequences of up to %ld)", P.seqs, (long) P.max_pages * P.page_size);
     }
-    if (!C.tc) return 0;
-    TaPlan A;
-    A.P = P; A.nq = C.nq; A.tiles = C.tiles; A.slices = C.slices; A.split_rows = P.cu ? AT_SPLIT_ROWS : 0; A.pdl = g_pdl;
-    A.scale2 = P.scale * 1.4426950408889634f; A.part_offset = C.tc_offset; A.g = g;
-    return attention_tc(A, stream);
+    if (C.tc)
+    {
+        // (first: the split form of the other sequences begins on the SMs that its last CTAs leave. us in a graph, before / since: 2333 tokens
+        // of six prompts 40.2 / 35.5, 64 single tokens of 1000 keys beside a prompt of 2048 tokens 130 / 120)
+        TaPlan A;
+        A.P = P; A.nq = C.nq; A.tiles = C.tiles; A.slices = C.slices; A.split_rows = P.cu ? AT_SPLIT_ROWS : 0; A.pdl = g_pdl;
+        A.scale2 = P.scale * 1.4426950408889634f; A.part_offset = C.tc_offset; A.g = g;
+        if ((rc = attention_tc(A, stream))) return rc;
+    }
+    if (!C.split) return 0;
+    S.grid = C.grid; S.cluster = C.cluster; S.pdl = g_pdl; S.late = g_pdl && C.tc && C.tiles; S.split_rows = P.cu ? AT_SPLIT_ROWS : 1 << 30;
+    S.scale2 = P.scale * 1.4426950408889634f; S.g = g;
+    return P.bf16 ? at_launch_dim<__nv_bfloat16>(S, C.wr, stream) : at_launch_dim<__half>(S, C.wr, stream);
 }
