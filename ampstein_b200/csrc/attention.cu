@@ -43,7 +43,9 @@ struct AtPlan
 {
     amp_attention_args P;
     int grid;                                  // CTAs of the split form
-    int unit, rows;                            // keys of a unit, rows of a row tile
+    int unit, rows;                            // keys of a unit, rows of a row tile: powers of two
+    int unit_shift, rows_shift, cluster_shift;
+    int group, group_mul, each;                // heads / kv_heads, ceil(2^16 / group); tokens of every sequence without cu
     int split_rows;                            // with cu: sequences of more rows (tokens x group) are the prompt form's
     int cluster;                               // > 0: every (sequence, head, row tile) belongs to a cluster of so many CTAs, which join in shared memory
     int by_segment;                            // join: blockIdx.x is a segment, else the CTA whose range begins inside it
@@ -105,14 +107,20 @@ __device__ __forceinline__ float4 at_ld_cluster4(uint32_t addr)
     return v;
 }
 
-// Row tiles of a sequence, and units of each of them (one at least: a segment without keys stores its zeros)
+// Row tiles of a sequence, and units of each of them (one at least: a segment without keys stores its zeros). (No division where a shift
+// or a product will do: what stands in front of the first load and behind the last is a chain of such steps. us with divisions / so: one
+// sequence of 128, 512, 4000 keys 4.9 / 4.3, 6.8 / 5.6, 10.6 / 9.9; 48 windows of 1024 12.7 / 11.3; seven of 1000 to 30000 keys and three tokens,
+// 256 values 64 / 56)
 __device__ __forceinline__ int at_row_tiles(const AtPlan& S, const AtSeq& s)
 {
-    const int rows = s.count * (S.P.heads / S.P.kv_heads);
-    return rows > S.split_rows ? 0 : (rows + S.rows - 1) / S.rows;
+    const int rows = s.count * S.group;
+    return rows > S.split_rows ? 0 : (rows + S.rows - 1) >> S.rows_shift;
 }
 
-__device__ __forceinline__ int at_units(const AtPlan& S, const AtKeys& k) { return max(1, (k.count() + S.unit - 1) / S.unit); }
+__device__ __forceinline__ int at_units(const AtPlan& S, const AtKeys& k) { return max(1, (k.count() + S.unit - 1) >> S.unit_shift); }
+
+// Token of a row: row / group, exact for the up to 64 rows of this form (the product is too large by less than row group / 2^16 / group)
+__device__ __forceinline__ int at_tok(const AtPlan& S, int row) { return row * S.group_mul >> 16; }
 
 // A place in the order of units. The end of a segment, where its parts meet and the next rows are fetched, counts as one more unit
 // (u == units): it takes a CTA about as long, and the many ends of short sequences would come on top of a full range.
@@ -124,7 +132,7 @@ struct AtCursor
 
     __device__ __forceinline__ void load(const AtPlan& S)
     {
-        s = at_seq(S.P, b);
+        s = at_seq(S.P, b, S.each);
         k = at_keys(S.P, s.first, s.count);
         tiles = at_row_tiles(S, s);
         units = at_units(S, k);
@@ -136,7 +144,7 @@ struct AtCursor
         load(S);
         const int row_tile = at / (units + 1);
         u = at - row_tile * (units + 1);
-        h = row_tile / tiles;
+        h = tiles == 1 ? row_tile : row_tile / tiles;
         rt = row_tile - h * tiles;
     }
     // to the next unit with keys, or segment; the caller knows that there is one
@@ -163,7 +171,7 @@ struct AtCount
 
     static __device__ __forceinline__ int units_of(const AtPlan& S, int b)
     {
-        const AtSeq s = at_seq(S.P, b);
+        const AtSeq s = at_seq(S.P, b, S.each);
         return S.P.kv_heads * at_row_tiles(S, s) * (at_units(S, at_keys(S.P, s.first, s.count)) + 1);
     }
 
@@ -265,7 +273,7 @@ void attention_split_kernel(const AtPlan S)
     __shared__ int s_scan[AT_WARPS], s_found[2];
 
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, grp = warp / WR, wr = warp % WR, cta = blockIdx.x;
-    const int group = P.heads / P.kv_heads;
+    const int group = S.group;
     // (late: what is in front of the prompt form is over, or that form had not let this one begin)
     if (S.pdl) { if (!S.late) pdl_wait(); pdl_launch_dependents(); }
 
@@ -274,13 +282,14 @@ void attention_split_kernel(const AtPlan S)
     int left;
     if (CLUSTER)
     {
-        in.b = 0; in.load(S);                                // (all sequences have as many tokens)
-        const int per = P.kv_heads * in.tiles, segment = cta / S.cluster, rank = cta - segment * S.cluster;
-        in.place(S, segment / per, 0);
-        in.h = segment % per / in.tiles; in.rt = segment % in.tiles;
+        in.b = cta >> S.cluster_shift;
+        in.load(S);
+        in.h = in.tiles == 1 ? blockIdx.y : blockIdx.y / in.tiles;
+        in.rt = blockIdx.y - in.h * in.tiles;
         // (a share may be empty: it then is of a cluster that has more CTAs than units)
-        in.u = in.units * rank / S.cluster;
-        left = in.units * (rank + 1) / S.cluster - in.u;
+        const int rank = cta - (in.b << S.cluster_shift);
+        in.u = in.units * rank >> S.cluster_shift;
+        left = (in.units * (rank + 1) >> S.cluster_shift) - in.u;
         in.units = in.u + left;                              // the share ends like a segment
         left += left > 0;
     }
@@ -413,7 +422,7 @@ void attention_split_kernel(const AtPlan S)
             {
                 for (int i = t; i < ROWS * CH; i += NT)
                 {
-                    const int r = i / CH, c = i % CH, row = in.rt * ROWS + r, tok = row / group;
+                    const int r = i / CH, c = i % CH, row = in.rt * ROWS + r, tok = at_tok(S, row);
                     uint4 v = make_uint4(0, 0, 0, 0);
                     if (tok < in.s.count)
                         v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(P.q) + (long long) (in.s.row0 + tok) * P.q_token
@@ -425,7 +434,7 @@ void attention_split_kernel(const AtPlan S)
                 {
                     m[i] = -INFINITY;
                     l[i] = 0.0f;
-                    at_row_keys(P, in.k, in.s.first + (in.rt * ROWS + wr * 16 + (lane >> 2) + 8 * i) / group, n0[i], c1[i], len[i]);
+                    at_row_keys(P, in.k, in.s.first + at_tok(S, in.rt * ROWS + wr * 16 + (lane >> 2) + 8 * i), n0[i], c1[i], len[i]);
                 }
                 at_whole_keys(P, in.k, in.s.first, in.s.first + in.s.count - 1, whole_from, whole_to);
                 #pragma unroll
@@ -602,7 +611,7 @@ void attention_split_kernel(const AtPlan S)
                     for (int i = t; i < ROWS * COLS / 4; i += NT)
                     {
                         const int r = i / (COLS / 4), c = (i % (COLS / 4)) * 4;
-                        const int row = in.rt * ROWS + r, tok = row / group;
+                        const int row = in.rt * ROWS + r, tok = at_tok(S, row);
                         if (tok >= in.s.count) break;        // (rows ascend with i)
                         float top = s_ml[0][r][0], sum = 0.0f;
                         #pragma unroll
@@ -639,12 +648,12 @@ void attention_split_kernel(const AtPlan S)
     {
         // every CTA of the cluster finishes its share of the segment's values, in order of the keys. (The barrier in front: all parts are
         // there, and all CTAs run. The one behind: nobody leaves with a part that is still read.)
-        const int C = S.cluster, units = at_units(S, in.k), per = (ROWS * D / 4 + C - 1) / C, rank = cta % C;
+        const int C = S.cluster, units = at_units(S, in.k), per = (ROWS * D / 4) >> S.cluster_shift, rank = cta & (C - 1);
         at_cluster_sync();
         const uint32_t mine = smem_u32(smem) + at_smem<D, WR>;
-        for (int i = rank * per + t; i < min((rank + 1) * per, ROWS * D / 4); i += NT)
+        for (int i = rank * per + t; i < (rank + 1) * per; i += NT)
         {
-            const int r = i / (D / 4), c = (i % (D / 4)) * 4, row = in.rt * ROWS + r, tok = row / group;
+            const int r = i / (D / 4), c = (i % (D / 4)) * 4, row = in.rt * ROWS + r, tok = at_tok(S, row);
             if (tok >= in.s.count) break;
             float m = -INFINITY, l = 0.0f;
             float2 ml[AT_MAX_CLUSTER];
@@ -653,7 +662,7 @@ void attention_split_kernel(const AtPlan S)
             for (int k = 0; k < AT_MAX_CLUSTER; ++k)
             {
                 // (an empty share has no part)
-                const bool part = k < C && units * k / C < units * (k + 1) / C;
+                const bool part = k < C && units * k >> S.cluster_shift < units * (k + 1) >> S.cluster_shift;
                 ml[k] = part ? at_ld_cluster2(at_map(mine + (ROWS * D + 2 * r) * 4, k)) : make_float2(-INFINITY, 0.0f);
                 y[k] = part ? at_ld_cluster4(at_map(mine + (r * D + c) * 4, k)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 m = fmaxf(m, ml[k].x);
@@ -683,7 +692,7 @@ void attention_join_kernel(const AtPlan S)
     __shared__ float s_red[4], s_sum[4];
     __shared__ float4 s_o[4][D / 4];
     __shared__ int s_scan[4], s_found[2];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, group = P.heads / P.kv_heads;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, group = S.group;
     AtCount C;
     C.count<128>(S, s_scan);
     AtCursor in;
@@ -692,9 +701,8 @@ void attention_join_kernel(const AtPlan S)
     bool join = false;
     if (S.by_segment)
     {
-        in.b = 0; in.load(S);                                // (all sequences have as many tokens)
-        const int per = P.kv_heads * in.tiles, b = blockIdx.x / per;
-        in.b = b; in.h = blockIdx.x % per / in.tiles; in.rt = blockIdx.x % in.tiles;
+        const int tiles = (S.each * group + S.rows - 1) >> S.rows_shift, at = tiles == 1 ? blockIdx.x : blockIdx.x / tiles, b = at / P.kv_heads;
+        in.b = b; in.h = at - b * P.kv_heads; in.rt = blockIdx.x - at * tiles;
         in.load(S);
         g0 = C.front_of(S, b, s_found) + (in.h * in.tiles + in.rt) * (in.units + 1);
         join = true;
@@ -725,7 +733,7 @@ void attention_join_kernel(const AtPlan S)
     auto part = [&](int i) { return parts + (size_t) (2 * (first + i) + (i ? 0 : 1)) * size; };
     for (int r = blockIdx.y; r < (LOOP ? S.rows : (int) blockIdx.y + 1); r += gridDim.y)
     {
-        const int row = in.rt * S.rows + r, tok = row / group;
+        const int row = in.rt * S.rows + r, tok = at_tok(S, row);
         if (tok >= in.s.count) return;
         float m = -INFINITY;
         for (int i = t; i < n; i += 128) m = fmaxf(m, part(i)[(size_t) S.rows * D + 2 * r]);
@@ -896,11 +904,13 @@ static int at_launch(AtPlan& S, cudaStream_t stream)
     if (cudaError_t e = ensure_smem(attention_split_kernel<T, D, WR, CLUSTER>, bytes, dev)) return cuda_rc(e, "attention shared memory");
     S.unit = at_unit<D, WR>;
     S.rows = 16 * WR;
+    static_assert((at_unit<D, WR> & (at_unit<D, WR> - 1)) == 0 && (WR & (WR - 1)) == 0, "shifts");
+    S.unit_shift = __builtin_ctz(S.unit); S.rows_shift = __builtin_ctz(S.rows); S.cluster_shift = CLUSTER ? __builtin_ctz(S.cluster) : 0;
     const long group = P.heads / P.kv_heads;
+    S.group = (int) group; S.group_mul = (int) ((65536 + group - 1) / group); S.each = P.tokens / P.seqs;
     // (segments of the call, where the host knows them)
     const long rows = (long) (P.tokens / P.seqs) * group, segments = (long) P.seqs * P.kv_heads * ((rows + S.rows - 1) / S.rows);
-    const long grid = CLUSTER ? segments * S.cluster : S.grid;
-    AMP_REQUIRE(grid < (1l << 31), "attention: too many sequences");
+    const long grid = CLUSTER ? (long) P.seqs * S.cluster : S.grid;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -913,7 +923,7 @@ static int at_launch(AtPlan& S, cudaStream_t stream)
         ++attrs;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned) grid, 1, 1);
+    cfg.gridDim = dim3((unsigned) grid, CLUSTER ? (unsigned) (segments / P.seqs) : 1, 1);
     cfg.blockDim = dim3(AT_THREADS, 1, 1);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = stream;

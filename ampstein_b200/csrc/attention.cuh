@@ -30,8 +30,8 @@ __device__ __forceinline__ int at_count(const amp_attention_args& P, int b)
     return max(row0, min(P.cu[b + 1], P.tokens)) - row0;
 }
 
-// Sequence b. Whatever pos and cu hold, the rows stay inside the tensors.
-__device__ __forceinline__ AtSeq at_seq(const amp_attention_args& P, int b)
+// Sequence b; each: tokens of every sequence without cu. Whatever pos and cu hold, the rows stay inside the tensors.
+__device__ __forceinline__ AtSeq at_seq(const amp_attention_args& P, int b, int each)
 {
     AtSeq s;
     const long long p = P.pos64 ? reinterpret_cast<const long long*>(P.pos)[b] : (long long) reinterpret_cast<const int*>(P.pos)[b];
@@ -43,8 +43,8 @@ __device__ __forceinline__ AtSeq at_seq(const amp_attention_args& P, int b)
     }
     else
     {
-        s.count = P.tokens / P.seqs;
-        s.row0 = b * s.count;
+        s.count = each;
+        s.row0 = b * each;
     }
     return s;
 }

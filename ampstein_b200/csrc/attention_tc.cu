@@ -170,11 +170,11 @@ __device__ __forceinline__ TaPlace ta_find(const TaPlan& S, int x)
     TaPlace f = {};
     if (!P.cu)
     {
-        const int each = tiles(P.tokens / P.seqs * group);
+        const int count = P.tokens / P.seqs, each = tiles(count * group);
         f.b = each ? x / each : P.seqs;
         f.tile = x - f.b * each;
         f.have = f.b < P.seqs;
-        if (f.have) f.s = at_seq(P, f.b);
+        if (f.have) f.s = at_seq(P, f.b, count);
         return f;
     }
     // four sequences per lane at a time
@@ -202,7 +202,7 @@ __device__ __forceinline__ TaPlace ta_find(const TaPlan& S, int x)
             f.have = 1;
             f.b = __shfl_sync(0xffffffffu, b0 + lane * EACH + at, l);
             f.tile = __shfl_sync(0xffffffffu, left, l);
-            f.s = at_seq(P, f.b);
+            f.s = at_seq(P, f.b, 0);
             return f;
         }
         x -= __shfl_sync(0xffffffffu, sum, 31);
