@@ -1007,6 +1007,8 @@ AMP_API int amp_b200_attention(const amp_attention_args* args, cudaStream_t stre
     }
     if (C.tc)
     {
+        // (rows and CTAs are divided in 30 bits)
+        AMP_REQUIRE((double) P.tokens * (P.heads / P.kv_heads) + 512 < 1073741824.0 && (double) C.tiles * C.slices * P.kv_heads < 1073741824.0, "attention: too many tokens in one call");
         // (first: the split form of the other sequences begins on the SMs that its last CTAs leave. us in a graph, before / since: 2333 tokens
         // of six prompts 40.2 / 35.5, 64 single tokens of 1000 keys beside a prompt of 2048 tokens 130 / 120)
         TaPlan A;

@@ -66,13 +66,27 @@ __device__ __forceinline__ AtKeys at_keys(const amp_attention_args& P, int first
     return k;
 }
 
-// Strides of the caches in pieces of 16 bytes (offsets inside a cache of up to 64 GB are 32-bit counts of them), and the division by
-// the page size, exact below 2^30: with 2^(s - 1) < page_size <= 2^s and mul = ceil(2^(30 + s) / page_size), j * mul / 2^(30 + s) is too
-// large by less than j / 2^30 / page_size
+// Division by what the host knows, exact for 0 <= j < 2^30: with 2^(s - 1) < d <= 2^s and mul = ceil(2^(30 + s) / d), j * mul / 2^(30 + s) is
+// too large by less than j / 2^30 / d
+struct AtDiv
+{
+    uint32_t mul, shift;
+    __device__ __forceinline__ int of(int j) const { return (int) ((unsigned long long) (uint32_t) j * mul >> shift); }
+};
+
+inline AtDiv at_div(long d)
+{
+    int s = 0;
+    while (s < 30 && (1l << s) < d) ++s;
+    return { (uint32_t) (((1ull << (30 + s)) + d - 1) / d), (uint32_t) (30 + s) };
+}
+
+// Strides of the caches in pieces of 16 bytes (offsets inside a cache of up to 64 GB are 32-bit counts of them)
 struct AtPages
 {
-    uint32_t k_page, k_row, v_page, v_row, mul, shift;
-    __device__ __forceinline__ int page_of(int j) const { return (int) ((unsigned long long) (uint32_t) j * mul >> shift); }
+    uint32_t k_page, k_row, v_page, v_row;
+    AtDiv page_size;
+    __device__ __forceinline__ int page_of(int j) const { return page_size.of(j); }
 };
 
 inline bool at_pages(const amp_attention_args& P, AtPages& g)
@@ -83,10 +97,7 @@ inline bool at_pages(const amp_attention_args& P, AtPages& g)
     };
     if (!fits(P.k_page, P.k_row, P.k_head) || !fits(P.v_page, P.v_row, P.v_head)) return false;
     g.k_page = (uint32_t) (P.k_page / 8); g.k_row = (uint32_t) (P.k_row / 8); g.v_page = (uint32_t) (P.v_page / 8); g.v_row = (uint32_t) (P.v_row / 8);
-    int s = 0;
-    while (s < 30 && (1l << s) < P.page_size) ++s;
-    g.shift = 30 + s;
-    g.mul = (uint32_t) (((1ull << g.shift) + P.page_size - 1) / P.page_size);
+    g.page_size = at_div(P.page_size);
     return true;
 }
 

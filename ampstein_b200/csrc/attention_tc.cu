@@ -165,16 +165,15 @@ template <int NQ>
 __device__ __forceinline__ TaPlace ta_find(const TaPlan& S, int x)
 {
     const amp_attention_args& P = S.P;
-    const int group = P.heads / P.kv_heads, lane = threadIdx.x & 31;
+    const int group = S.group, lane = threadIdx.x & 31;
     auto tiles = [&](int rows) { return rows <= S.split_rows ? 0 : (rows + ta_rows<NQ> - 1) / ta_rows<NQ>; };
     TaPlace f = {};
     if (!P.cu)
     {
-        const int count = P.tokens / P.seqs, each = tiles(count * group);
-        f.b = each ? x / each : P.seqs;
-        f.tile = x - f.b * each;
-        f.have = f.b < P.seqs;
-        if (f.have) f.s = at_seq(P, f.b, count);
+        f.b = S.by_tiles.of(x);
+        f.tile = x - f.b * tiles(S.each * group);
+        f.have = 1;
+        f.s = at_seq(P, f.b, S.each);
         return f;
     }
     // four sequences per lane at a time
@@ -264,11 +263,11 @@ void attention_tc_kernel(const TaPlan S)
     __shared__ TaPlace s_place;
 
     const int t = threadIdx.x, lane = t & 31, warp = __shfl_sync(0xffffffffu, t >> 5, 0);
-    const int group = P.heads / P.kv_heads;
+    const int group = S.group;
     // (before tensor memory is taken: a CTA in front may still have to take its own here; those behind are let in when it is taken)
     if (S.pdl) pdl_wait();
-    const int h = blockIdx.x % P.kv_heads, slice = blockIdx.x / P.kv_heads % S.slices;
-    const int x = S.tiles - 1 - (int) (blockIdx.x / P.kv_heads / S.slices);      // (the last tiles see most keys: first)
+    const int hx = S.by_kv.of(blockIdx.x), h = blockIdx.x - hx * P.kv_heads, from_last = S.by_slices.of(hx), slice = hx - from_last * S.slices;
+    const int x = S.tiles - 1 - from_last;     // (the last tiles see most keys: first)
     if (warp == 0)
     {
         const TaPlace f = ta_find<NQ>(S, x);
@@ -302,10 +301,12 @@ void attention_tc_kernel(const TaPlan S)
         return;
     }
     const AtSeq seq = s_place.s;
-    const int row0 = s_place.tile * ROWS, tok0 = row0 / group, tok1 = min((row0 + ROWS - 1) / group, seq.count - 1);
+    const int row0 = s_place.tile * ROWS, tok0 = S.by_group.of(row0), tok1 = min(S.by_group.of(row0 + ROWS - 1), seq.count - 1);
     const AtKeys keys = at_keys(P, seq.first + tok0, tok1 - tok0 + 1);
     const int n_all = (keys.count() + KB - 1) / KB;
-    const int j0 = (int) ((long long) n_all * slice / S.slices), n = (int) ((long long) n_all * (slice + 1) / S.slices) - j0;
+    // (2^24 tiles of keys and 256 slices at most: the products are below 2^32)
+    const int j0 = slice == 0 ? 0 : (int) ((unsigned) n_all * (unsigned) slice / (unsigned) S.slices);
+    const int n = (slice + 1 == S.slices ? n_all : (int) ((unsigned) n_all * (unsigned) (slice + 1) / (unsigned) S.slices)) - j0;
     const uint32_t q_s = smem_u32(ta_mem), kv_s = q_s + NQ * Q_BYTES;
     const uint32_t full_s = smem_u32(&kv_full[0]), free_s = smem_u32(&kv_free[0]), sf = smem_u32(&s_full[0]), pf = smem_u32(&p_full[0]);
     const bool aligned = (q_s & 1023) == 0;    // (the swizzle needs the alignment that the declaration asks for)
@@ -329,7 +330,7 @@ void attention_tc_kernel(const TaPlan S)
     {
         // ---- softmax: thread t has row t of the CTA's ROWS ------------------------------------------------------------------
         const int i = warp >> 2;               // row tile
-        const int row = row0 + t, tok = row / group, head = h * group + row - tok * group;
+        const int row = row0 + t, tok = S.by_group.of(row), head = h * group + row - tok * group;
         const bool have = tok < seq.count;
         const int p = seq.first + tok;
         {
@@ -351,7 +352,7 @@ void attention_tc_kernel(const TaPlan S)
         // what its row sees of the keys, and a run of them that all rows of the row tile see: there no single key is looked at
         int n0, c1, len, from, to;
         at_row_keys(P, keys, p, n0, c1, len);
-        at_whole_keys(P, keys, seq.first + (row0 + 128 * i) / group, seq.first + min((row0 + 128 * i + 127) / group, seq.count - 1), from, to);
+        at_whole_keys(P, keys, seq.first + S.by_group.of(row0 + 128 * i), seq.first + min(S.by_group.of(row0 + 128 * i + 127), seq.count - 1), from, to);
 
         const float sc = P.scale == 0.0f ? 1.0f : fabsf(S.scale2);
         const uint32_t lane_base = tmem + ((uint32_t) (32 * (warp & 3)) << 16);
@@ -759,7 +760,7 @@ void attention_tc_join_kernel(const TaPlan S)
     const amp_attention_args& P = S.P;
     constexpr int ROWS = ta_rows<NQ>;
     __shared__ TaPlace s_place;
-    const int t = threadIdx.x, h = blockIdx.x % P.kv_heads, x = blockIdx.x / P.kv_heads, group = P.heads / P.kv_heads;
+    const int t = threadIdx.x, x = S.by_kv.of(blockIdx.x), h = blockIdx.x - x * P.kv_heads, group = S.group;
     if (t < 32)
     {
         const TaPlace f = ta_find<NQ>(S, x);
@@ -769,7 +770,7 @@ void attention_tc_join_kernel(const TaPlan S)
     if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
     if (!s_place.have) return;
     const AtSeq seq = s_place.s;
-    const int row = s_place.tile * ROWS + t, tok = row / group;
+    const int row = s_place.tile * ROWS + t, tok = S.by_group.of(row);
     if (tok >= seq.count) return;
     const float* const parts = reinterpret_cast<const float*>(reinterpret_cast<const unsigned char*>(P.workspace) + S.part_offset)
                                + (size_t) blockIdx.x * S.slices * ta_part_floats(ROWS, D);
@@ -834,9 +835,14 @@ static int ta_launch_dim(const TaPlan& S, cudaStream_t stream)
     return S.nq == 1 ? ta_launch<T, 64, 1>(S, stream) : ta_launch<T, 64, 2>(S, stream);
 }
 
-int attention_tc(const TaPlan& S, cudaStream_t stream)
+int attention_tc(TaPlan& S, cudaStream_t stream)
 {
+    const amp_attention_args& P = S.P;
     if (S.tiles == 0) return 0;
+    const int tile = 128 * S.nq;
+    S.group = P.heads / P.kv_heads; S.each = P.tokens / P.seqs;
+    S.by_group = at_div(S.group); S.by_kv = at_div(P.kv_heads); S.by_slices = at_div(S.slices);
+    S.by_tiles = at_div(P.cu ? 1 : ((long) S.each * S.group + tile - 1) / tile);
     return S.P.bf16 ? ta_launch_dim<__nv_bfloat16>(S, stream) : ta_launch_dim<__half>(S, stream);
 }
 

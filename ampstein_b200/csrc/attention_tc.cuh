@@ -23,11 +23,15 @@ struct TaPlan
     int slices;                                // of every tile's keys
     int split_rows;                            // sequences of up to so many rows (tokens x group) are the split form's
     int pdl;
+    int group, each;                           // heads / kv_heads; tokens of every sequence without cu
+    // what a CTA divides by before its first load (us with divisions / so: six prompts 33.6 / 32.5, six of 390 tokens in windows of 128 32.4 / 31.4);
+    // tiles: of a sequence without cu
+    AtDiv by_group, by_kv, by_slices, by_tiles;
     float scale2;                              // scale * log2(e)
     size_t part_offset;                        // of the parts in the workspace
     AtPages g;
 };
 
-int attention_tc(const TaPlan& S, cudaStream_t stream);
+int attention_tc(TaPlan& S, cudaStream_t stream);               // (fills group and what is behind it in)
 
 }  // namespace amp
