@@ -80,21 +80,30 @@ __device__ __forceinline__ T* rope_to(const amp_rope_args& P, int n, int h, long
     return reinterpret_cast<T*>(P.v_cache) + vc + (long long) (h - P.kv_heads) * P.vc_head;
 }
 
+// The arguments, and what a CTA divides by (products: one token 2.55 -> 2.43 us, 2048 level)
+struct RopePlan
+{
+    amp_rope_args P;
+    AtDiv by_page, by_each, by_places;
+    int each, pdl;
+};
+
 // VEC: 16 bytes at a time; else value by value (a rotated part or a head that is not a multiple of 16 values, or other alignments)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(ROPE_THREADS)
-void rope_kernel(const amp_rope_args P, int pdl)
+void rope_kernel(const RopePlan S)
 {
+    const amp_rope_args& P = S.P;
     __shared__ __align__(16) float2 s_cs[ROPE_MAX_DIM / 2];
     __shared__ int s_seq;
     const int t = threadIdx.x, n = blockIdx.x;
-    if (pdl) { pdl_wait(); pdl_launch_dependents(); }
+    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
     const int total = P.heads + (P.k ? 2 * P.kv_heads : 0), rotated = P.heads + (P.k ? P.kv_heads : 0);
 
     // a thread's place in every head, and its first heads: requested before anything else is known of the token
     constexpr int BATCH = 4;                                 // (and of the value-by-value form)
-    const int places = P.dim / 16, step = VEC ? ROPE_THREADS / places : 0, turning = P.rot / 16;
-    const int c = VEC ? t % places : 0, h0 = VEC ? t / places : 0;
+    const int places = P.dim / 16, step = VEC ? S.by_places.of(ROPE_THREADS) : 0, turning = P.rot / 16;
+    const int h0 = VEC ? S.by_places.of(t) : 0, c = VEC ? t - h0 * places : 0;
     const bool turns = c < turning, mine = h0 < step;        // (128 is not a multiple of every width)
     const int at0 = 8 * (turns && !P.interleaved ? c : 2 * c), at1 = 8 * (turns && !P.interleaved ? c + turning : 2 * c + 1);
     uint4 x[BATCH], y[BATCH];
@@ -139,16 +148,15 @@ void rope_kernel(const amp_rope_args P, int pdl)
     }
     else
     {
-        const int each = P.tokens / P.seqs;
-        b = n / each;
-        first_row = b * each;
+        b = S.by_each.of(n);
+        first_row = b * S.each;
         p = position(b);
     }
     p += n - first_row;
     int page = -1, row = 0;
     if (P.k && p >= 0 && p < (long long) P.max_pages * P.page_size)
     {
-        const int pg = (int) p / P.page_size;
+        const int pg = S.by_page.of((int) p);
         row = (int) p - pg * P.page_size;
         page = P.table[(long long) b * P.table_row + pg];
     }
@@ -231,8 +239,11 @@ static int rope_launch(const amp_rope_args& P, bool vec, cudaStream_t stream)
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = g_pdl ? 1 : 0;
-    return cuda_rc(vec ? cudaLaunchKernelEx(&cfg, rope_kernel<T, true>, (const amp_rope_args) P, g_pdl)
-                       : cudaLaunchKernelEx(&cfg, rope_kernel<T, false>, (const amp_rope_args) P, g_pdl), "rope launch");
+    RopePlan S;
+    S.P = P; S.each = max(1, P.tokens / P.seqs); S.pdl = g_pdl;
+    S.by_page = at_div(max(1, P.page_size)); S.by_each = at_div(S.each); S.by_places = at_div(max(1, P.dim / 16));
+    return cuda_rc(vec ? cudaLaunchKernelEx(&cfg, rope_kernel<T, true>, (const RopePlan) S)
+                       : cudaLaunchKernelEx(&cfg, rope_kernel<T, false>, (const RopePlan) S), "rope launch");
 }
 
 }  // namespace amp
