@@ -14,7 +14,7 @@
 // Warps: four per row tile do the softmax (a thread a row, the warp's quarter of tensor memory), then one issues the MMAs, three load
 // keys and values by 16-byte asynchronous copies (a page of any size, strides of any kind).
 //
-// What bounds it (8192 tokens, 32 query heads on 8 key-value heads of 128 values, fp16): 492 us, 1117 TFLOP/s, 0.68 of the measured burst
+// What bounds it (8192 tokens, 32 query heads on 8 key-value heads of 128 values, fp16): 497 us, 1106 TFLOP/s, 0.67 of the measured burst
 // rate; tensor and exponential pipe active in 54 % of the cycles each. A row tile's chain, scores read 0.15 us, maximum 0.2, weights
 // 0.75, its P V and the next Q K^T 0.5, is longer than the other tile's MMAs, and the rows of a page reach shared memory through three
 // warps at about 0.8 us per tile of keys or values. Measured and taken back: seven loading warps (registers of the softmax), TMA gathers of

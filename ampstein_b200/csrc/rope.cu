@@ -6,7 +6,7 @@
 // heads), then turns and stores. A thread keeps one place inside the head, 16 values wide, through all its heads: its eight
 // cos and sin stay in registers.
 //
-// Measured: 2.8 us for one token of 32 + 2 x 8 heads of 128 values; 2047 tokens of five sequences, 48 + 2 x 8 heads, 15.3 us (4.4 TB/s
+// Measured: 2.4 us for one token of 32 + 2 x 8 heads of 128 values; 2047 tokens of five sequences, 48 + 2 x 8 heads, 15.3 us (4.4 TB/s
 // in and out, 0.68 of the measured copy rate: a CTA's chain of positions, table entry, cos and sin, store is not hidden whole).
 //
 // The angle p * inv_freq is taken modulo a turn in fp64: at p = 10^6 an fp32 product is off by 0.06 rad.
