@@ -261,7 +261,8 @@ class PagedCache:
         self.page_size, self.max_pages = page_size, max_pages
         self._free = list(range(pages - 1, -1, -1))          # (popped from the end: low numbers first)
         self._uses = [0] * pages                              # sequences that have the page
-        self._seqs = [None] * slots                           # per slot: [pages (None: given up), tokens]
+        # per slot: [pages (None: given up), tokens, first position of the last extend(), first position that sees no given-up page]
+        self._seqs = [None] * slots
 
     @property
     def free_pages(self):
@@ -293,7 +294,7 @@ class PagedCache:
         """A slot for a new sequence"""
         for slot, seq in enumerate(self._seqs):
             if seq is None:
-                self._seqs[slot] = [[], 0]
+                self._seqs[slot] = [[], 0, 0, 0]
                 return slot
         raise RuntimeError("PagedCache: all %d slots are taken" % len(self._seqs))
 
@@ -302,16 +303,14 @@ class PagedCache:
         copy of its own where they go into it. Returns the position of the first of them. RuntimeError, and nothing changed, without
         room."""
         seq = self._seq(slot)
-        pages, at = seq
+        pages, at = seq[:2]
         if tokens < 0:
             raise ValueError("PagedCache.extend: tokens must not be negative")
         need = -(-(at + tokens) // self.page_size)
         if need > self.max_pages:
             raise RuntimeError("PagedCache: %d tokens do not fit into %d pages" % (at + tokens, self.max_pages))
         last = at // self.page_size if tokens and at % self.page_size else None           # the half-filled page that is written on
-        own = last is not None and pages[last] is not None and self._uses[pages[last]] > 1
-        if last is not None and pages[last] is None:
-            raise ValueError("PagedCache: the page of position %d has been given up" % at)
+        own = last is not None and self._uses[pages[last]] > 1
         if need - len(pages) + own > len(self._free):
             raise RuntimeError("PagedCache: %d pages are free, %d are needed" % (len(self._free), need - len(pages) + own))
         changed = own
@@ -326,16 +325,16 @@ class PagedCache:
             self._uses[page] = 1
             pages.append(page)
             changed = True
-        seq[1] = at + tokens
+        seq[1:3] = at + tokens, at
         if changed:
             self._write_row(slot)
         return at
 
     def fork(self, slot):
         """A new sequence with the same tokens; shares the pages. Returns its slot."""
-        pages, at = self._seq(slot)
+        pages, *rest = self._seq(slot)
         new = self.add()
-        self._seqs[new] = [list(pages), at]
+        self._seqs[new] = [list(pages), *rest]
         for page in pages:
             if page is not None:
                 self._uses[page] += 1
@@ -343,31 +342,43 @@ class PagedCache:
         return new
 
     def truncate(self, slot, tokens):
-        """Takes back what stands behind the first `tokens` tokens (rejected drafts)"""
+        """Takes back what stands behind the first `tokens` tokens (rejected drafts). ValueError, and nothing changed, where the next token
+        would see a page that has been given up."""
         seq = self._seq(slot)
         if not 0 <= tokens <= seq[1]:
             raise ValueError("PagedCache.truncate: %d of %d tokens" % (tokens, seq[1]))
         keep = -(-tokens // self.page_size)
+        gaps = None in seq[0][:keep]
+        if gaps and tokens < seq[3]:
+            raise ValueError("PagedCache.truncate: the token at position %d sees pages that have been given up (from %d on it does not)" % (tokens, seq[3]))
         for page in seq[0][keep:]:
             if page is not None:
                 self._drop(page)
         changed = len(seq[0]) > keep
         del seq[0][keep:]
-        seq[1] = tokens
+        seq[1:] = tokens, min(seq[2], tokens), seq[3] if gaps else 0
         if changed:
             self._write_row(slot)
 
-    def leave_behind(self, slot, window, sinks=0):
+    def leave_behind(self, slot, window, sinks=0, pending=None):
         """Gives up the pages that no further token of the sequence sees: those that hold neither one of the first `sinks` tokens nor one
-        of the last `window` - 1"""
-        pages, at = self._seq(slot)
+        that is visible, in a window of so many tokens, from the first token still to run. pending: how many of the announced tokens have
+        not run yet, or may be taken back (drafts). By default those of the last extend(), whose pages are then safe before and after they
+        run; but of a sequence's first tokens, its prompt, the last one alone: a prompt runs first, or pending says how long it is."""
+        seq = self._seq(slot)
+        pages, at, last = seq[:3]
         if window < 1 or sinks < 0:
             raise ValueError("PagedCache.leave_behind: window must be positive, sinks not negative")
+        if pending is None:
+            pending = at - last if last else min(1, at)
+        if not 0 <= pending <= at:
+            raise ValueError("PagedCache.leave_behind: %s of %d tokens are pending" % (pending, at))
         changed = False
-        for i in range(-(-sinks // self.page_size), max(0, at - window + 1) // self.page_size):
+        for i in range(-(-sinks // self.page_size), max(0, at - pending - window + 1) // self.page_size):
             if pages[i] is not None:
                 self._drop(pages[i])
                 pages[i] = None
+                seq[3] = max(seq[3], (i + 1) * self.page_size + window - 1)
                 changed = True
         if changed:
             self._write_row(slot)
