@@ -315,8 +315,9 @@ class PagedCache:
             raise RuntimeError("PagedCache: %d pages are free, %d are needed" % (len(self._free), need - len(pages) + own))
         changed = own
         if own:
-            page = self._free.pop()
-            attention.copy_pages([self.k, self.v], [pages[last]], [page])
+            page = self._free[-1]
+            attention.copy_pages([self.k, self.v], [pages[last]], [page])         # (may raise: nothing has changed yet)
+            self._free.pop()
             self._drop(pages[last])
             self._uses[page] = 1
             pages[last] = page
