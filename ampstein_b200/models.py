@@ -145,9 +145,16 @@ def _bundle_check(linears):
                              "(matrix %d differs)" % i)
 
 
+def _add_biases(linears, outs):
+    """What LinearEXL3.forward does behind the product, for the outputs of a bundle; in place"""
+    for i, w in enumerate(linears):
+        if w.bias is not None:
+            outs[i].add_(w.bias)
+
+
 class Multi:
     """Equal-shape bundle (reference: models.uc multi(), :338-361): run(x) writes all outputs
-    stacked into `out` (num, m, n) with ONE launch. x is (1, m, k)."""
+    stacked into `out` (num, m, n) with ONE launch, and one more for each linear with a bias. x is (1, m, k)."""
 
     def __init__(self, linears, out):
         _bundle_check(linears)
@@ -163,17 +170,23 @@ class Multi:
         m = x.shape[1]
         if a_had is None and (m >= 5 or x.dtype == torch.bfloat16):
             a_had = torch.empty((len(self.linears), m, a.in_features), dtype=torch.float16, device=x.device)
-        return exl3.mgemm(x, self.B, self.out, self.suh, a_had, self.svh, a.K, a.mcg, a.mul1)
+        exl3.mgemm(x, self.B, self.out, self.suh, a_had, self.svh, a.K, a.mcg, a.mul1)
+        _add_biases(self.linears, self.out)
+        return self.out
 
     def run_norm(self, x, res, norm_w, eps, y):
         """The bundle applied to RMSNorm(x + res) * norm_w, y = fp16(x + res): one launch (up to 16 rows)."""
-        return _run_norm(self, self.out, x, res, norm_w, eps, y, None)
+        _run_norm(self, self.out, x, res, norm_w, eps, y, None)
+        _add_biases(self.linears, self.out)
+        return self.out
 
     def run_normed(self, y, ssq, norm_w, eps):
         """The bundle applied to the norm of a residual stream whose block sums of squares the producing
         linear left in ssq (LinearEXL3.forward_add_res)."""
         a = self.linears[0]
-        return exl3.mgemm_normed(y, ssq, norm_w, eps, self.B, self.out, self.suh, self.svh, a.K, a.mcg, a.mul1)
+        exl3.mgemm_normed(y, ssq, norm_w, eps, self.B, self.out, self.suh, self.svh, a.K, a.mcg, a.mul1)
+        _add_biases(self.linears, self.out)
+        return self.out
 
 
 def _run_norm(bundle, carrier, x, res, norm_w, eps, y, opts):
@@ -184,7 +197,7 @@ def _run_norm(bundle, carrier, x, res, norm_w, eps, y, opts):
 class Sliced:
     """Bundle for unequal widths such as Q/K/V (reference: models.uc sliced(), :367-432): every
     matrix is cut into column slices of the widths' gcd (a multiple of 128); outputs are written
-    in place into `outs`, one (1, m, out_features) buffer per linear."""
+    in place into `outs`, one (1, m, out_features) buffer per linear; biases are added there, a launch each."""
 
     def __init__(self, linears, outs):
         import math
@@ -227,11 +240,13 @@ class Sliced:
         if a_had is None and (m >= 5 or x.dtype == torch.bfloat16):
             a_had = torch.empty((len(self.linears), m, a.in_features), dtype=torch.float16, device=x.device)
         exl3.mgemm(x, self.B, self.carrier, self.suh, a_had, self.svh, a.K, a.mcg, a.mul1, self.opts)
+        _add_biases(self.linears, self.outs)
         return self.outs
 
     def run_norm(self, x, res, norm_w, eps, y):
         """The bundle applied to RMSNorm(x + res) * norm_w, y = fp16(x + res): one launch (up to 16 rows)."""
         _run_norm(self, self.carrier, x, res, norm_w, eps, y, self.opts)
+        _add_biases(self.linears, self.outs)
         return self.outs
 
     def run_normed(self, y, ssq, norm_w, eps):
@@ -239,6 +254,7 @@ class Sliced:
         linear left in ssq (LinearEXL3.forward_add_res)."""
         a = self.linears[0]
         exl3.mgemm_normed(y, ssq, norm_w, eps, self.B, self.carrier, self.suh, self.svh, a.K, a.mcg, a.mul1, self.opts)
+        _add_biases(self.linears, self.outs)
         return self.outs
 
 
