@@ -32,6 +32,12 @@ class LinearEXL3:
         self.out_features = trellis.shape[1] * 16
         self._plan = None
 
+    def _biased(self, y, out):
+        """y, the product, and the bias; in `out` where the caller gave it"""
+        if self.bias is None:
+            return y
+        return y.add(self.bias) if out is None else y.add_(self.bias)
+
     def forward(self, x, out=None):
         m = x.shape[0]
         if out is None and m <= RECON_ROWS:
@@ -39,34 +45,30 @@ class LinearEXL3:
             plan = self._plan
             if plan is None or not plan.matches(self.trellis, self.suh, self.svh, self.mul1, self.mcg):
                 plan = self._plan = exl3.GemmPlan(self.trellis, self.suh, self.svh, self.mul1, self.mcg)
-            out = plan.run(x, self.trellis, self.suh, self.svh)
-            if out is not None:
-                return out if self.bias is None else out.add(self.bias)
+            y = plan.run(x, self.trellis, self.suh, self.svh)
+            if y is not None:
+                return y if self.bias is None else y.add(self.bias)
         if out is None and m > RECON_ROWS and self.out_features <= RECON_MAX_N:
-            out = exl3.exl3_gemm_recon(x.contiguous(), self.trellis, self.suh, self.svh, self.K,
-                                       self.mul1, self.mcg)
+            y = exl3.exl3_gemm_recon(x.contiguous(), self.trellis, self.suh, self.svh, self.K,
+                                     self.mul1, self.mcg)
         else:
-            if out is None:
-                out = x.new_empty((m, self.out_features), dtype=torch.float16)
-            exl3.exl3_gemm(x, self.trellis, out, self.suh, self.svh, self.mul1, self.mcg)
-        if self.bias is not None:
-            out = out.add(self.bias)
-        return out
+            y = x.new_empty((m, self.out_features), dtype=torch.float16) if out is None else out
+            exl3.exl3_gemm(x, self.trellis, y, self.suh, self.svh, self.mul1, self.mcg)
+        return self._biased(y, out)
 
     def forward_silu_mul(self, gate, up, out=None):
         """out = this linear of silu(gate) * up in one launch (the down projection behind a gate|up
         bundle, up to 16 rows); larger batches take the two-step path of the caller."""
         m = gate.shape[0]
-        if out is None:
-            out = torch.empty((m, self.out_features), dtype=torch.float16, device=gate.device)
-        exl3.exl3_gemm_silu_mul(gate, up, self.trellis, out, self.suh, self.svh, self.mul1, self.mcg)
-        if self.bias is not None:
-            out = out.add(self.bias)
-        return out
+        y = torch.empty((m, self.out_features), dtype=torch.float16, device=gate.device) if out is None else out
+        exl3.exl3_gemm_silu_mul(gate, up, self.trellis, y, self.suh, self.svh, self.mul1, self.mcg)
+        return self._biased(y, out)
 
     def forward_add_res(self, x, h, y, ssq):
         """y = fp16(h + this linear of x), ssq = block sums of squares of y: the linear and the residual
-        add of the norm that follows, in one launch (up to 16 rows)."""
+        add of the norm that follows, in one launch (up to 16 rows). Not for linears with a bias, which the launch does not add."""
+        if self.bias is not None:
+            raise ValueError("LinearEXL3.forward_add_res: the linear has a bias")
         return exl3.exl3_gemm_add_res(x, self.trellis, self.suh, self.svh, h, y, ssq, self.mul1, self.mcg)
 
     def weight_bytes(self):

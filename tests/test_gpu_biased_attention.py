@@ -37,3 +37,23 @@ def test_biases_of_q_k_v(oracle, rows):
     want = o.forward(a.view(rows, -1)).float()
     # (two chains of linears within 1e-2 of the largest value each, the framework's bound for a linear)
     assert (got - want).abs().max() <= 2e-2 * want.abs().max()
+
+
+def test_the_bias_of_o_reaches_the_buffer_of_a_captured_step(oracle):
+    import ampstein_b200 as amp
+    from ampstein_b200.models import DecodeGraph, PagedAttention, PagedCache, Sliced
+    lins = [linear(HIDDEN, n * D, i, True) for i, n in enumerate((HQ, HKV, HKV))]
+    o = linear(HQ * D, HIDDEN, 9, True)
+    inv_freq, _ = amp.rope_frequencies(D)
+    x = torch.randn((1, 1, HIDDEN), generator=torch.Generator().manual_seed(3)).to(torch.float16).cuda()
+    cache = PagedCache(1, 8, 16, HKV, D, 1, 8)
+    pos = torch.tensor([cache.extend(cache.add(), 1)], device="cuda")
+    block = PagedAttention(Sliced(lins, [torch.zeros((1, 1, w.out_features), dtype=torch.float16, device="cuda") for w in lins]), o, cache, 0, D, inv_freq)
+    out = torch.zeros((1, HIDDEN), dtype=torch.float16, device="cuda")
+    graph = DecodeGraph(lambda: block.run(x, pos, cache.table, out=out))
+    want = block.run(x, pos, cache.table)
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    # (one linear, in its two calls)
+    assert (out.float() - want.float()).abs().max() <= 1e-2 * want.float().abs().max()
