@@ -37,3 +37,13 @@ def test_the_fused_residual_add_refuses_a_bias(lin, monkeypatch):
     lin.bias = torch.ones(128, dtype=torch.float16)
     with pytest.raises(ValueError):
         lin.forward_add_res(x, x, x, None)
+
+
+def test_shards_have_their_part_of_the_bias(lin):
+    lin = models.LinearEXL3(torch.zeros((32, 32, 64), dtype=torch.int16), torch.ones(512), torch.ones(512), bias=torch.arange(512.0).half())
+    parts = [models.cols(lin, [(0, 128), (384, 128)]), models.cols(lin, [(128, 256)])]
+    assert torch.equal(torch.cat([p.bias for p in parts]), torch.cat((lin.bias[:128], lin.bias[384:], lin.bias[128:384])))
+    parts = [models.rows(lin, k0, 256) for k0 in (0, 256)]
+    assert torch.equal(sum(p.bias for p in parts if p.bias is not None), lin.bias)      # (once, whatever the number of shards)
+    lin.bias = None
+    assert models.cols(lin, [(0, 128)]).bias is None and models.rows(lin, 0, 128).bias is None
