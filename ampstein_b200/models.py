@@ -155,9 +155,22 @@ def _add_biases(linears, outs):
             outs[i].add_(w.bias)
 
 
+def _first_rows(t, m):
+    """The beginning of a (num, rows, n) buffer as (num, m, n)"""
+    return t if m == t.shape[1] else t.view(-1)[:t.shape[0] * m * t.shape[2]].view(t.shape[0], m, t.shape[2])
+
+
+def _bundle_rows(x, most):
+    m = x.shape[1]
+    if not 1 <= m <= most:
+        raise ValueError("models.bundle: %d rows, the bundle's buffers hold %d" % (m, most))
+    return m
+
+
 class Multi:
     """Equal-shape bundle (reference: models.uc multi(), :338-361): run(x) writes all outputs
-    stacked into `out` (num, m, n) with ONE launch, and one more for each linear with a bias. x is (1, m, k)."""
+    stacked into `out` (num, m, n) with ONE launch, and one more for each linear with a bias. x is (1, m, k);
+    with fewer rows than `out` has, the outputs are stacked at its beginning. Returns them, (num, rows of x, n)."""
 
     def __init__(self, linears, out):
         _bundle_check(linears)
@@ -170,26 +183,29 @@ class Multi:
     def run(self, x, a_had=None):
         """a_had: (num, m, k) fp16 scratch, used from five rows up (allocated here if missing)"""
         a = self.linears[0]
-        m = x.shape[1]
+        m = _bundle_rows(x, self.out.shape[1])
+        out = _first_rows(self.out, m)
         if a_had is None and (m >= 5 or x.dtype == torch.bfloat16):
             a_had = torch.empty((len(self.linears), m, a.in_features), dtype=torch.float16, device=x.device)
-        exl3.mgemm(x, self.B, self.out, self.suh, a_had, self.svh, a.K, a.mcg, a.mul1)
-        _add_biases(self.linears, self.out)
-        return self.out
+        exl3.mgemm(x, self.B, out, self.suh, a_had, self.svh, a.K, a.mcg, a.mul1)
+        _add_biases(self.linears, out)
+        return out
 
     def run_norm(self, x, res, norm_w, eps, y):
         """The bundle applied to RMSNorm(x + res) * norm_w, y = fp16(x + res): one launch (up to 16 rows)."""
-        _run_norm(self, self.out, x, res, norm_w, eps, y, None)
-        _add_biases(self.linears, self.out)
-        return self.out
+        out = _first_rows(self.out, _bundle_rows(x, self.out.shape[1]))
+        _run_norm(self, out, x, res, norm_w, eps, y, None)
+        _add_biases(self.linears, out)
+        return out
 
     def run_normed(self, y, ssq, norm_w, eps):
         """The bundle applied to the norm of a residual stream whose block sums of squares the producing
         linear left in ssq (LinearEXL3.forward_add_res)."""
         a = self.linears[0]
-        exl3.mgemm_normed(y, ssq, norm_w, eps, self.B, self.out, self.suh, self.svh, a.K, a.mcg, a.mul1)
-        _add_biases(self.linears, self.out)
-        return self.out
+        out = _first_rows(self.out, _bundle_rows(y, self.out.shape[1]))
+        exl3.mgemm_normed(y, ssq, norm_w, eps, self.B, out, self.suh, self.svh, a.K, a.mcg, a.mul1)
+        _add_biases(self.linears, out)
+        return out
 
 
 def _run_norm(bundle, carrier, x, res, norm_w, eps, y, opts):
@@ -200,7 +216,8 @@ def _run_norm(bundle, carrier, x, res, norm_w, eps, y, opts):
 class Sliced:
     """Bundle for unequal widths such as Q/K/V (reference: models.uc sliced(), :367-432): every
     matrix is cut into column slices of the widths' gcd (a multiple of 128); outputs are written
-    in place into `outs`, one (1, m, out_features) buffer per linear; biases are added there, a launch each."""
+    in place into `outs`, one (1, m, out_features) buffer per linear; biases are added there, a launch each.
+    An x of fewer rows than the buffers have goes into their first rows. Returns the outputs of x's rows."""
 
     def __init__(self, linears, outs):
         import math
@@ -236,29 +253,39 @@ class Sliced:
         # descriptor only: (num_slices, m, width); the data goes through c_ptrs
         self.carrier = torch.empty((len(t), m, width), dtype=torch.float16, device=dev)
 
+    def _rows(self, x):
+        """The descriptor and the buffers for x's rows"""
+        m = _bundle_rows(x, self.carrier.shape[1])
+        if m == self.carrier.shape[1]:
+            return self.carrier, self.outs
+        return _first_rows(self.carrier, m), [t[:, :m] for t in self.outs]
+
     def run(self, x, a_had=None):
         """a_had: (linears, m, k) fp16 scratch, used from five rows up (allocated here if missing)"""
         a = self.linears[0]
         m = x.shape[1]
+        carrier, outs = self._rows(x)
         if a_had is None and (m >= 5 or x.dtype == torch.bfloat16):
             a_had = torch.empty((len(self.linears), m, a.in_features), dtype=torch.float16, device=x.device)
-        exl3.mgemm(x, self.B, self.carrier, self.suh, a_had, self.svh, a.K, a.mcg, a.mul1, self.opts)
-        _add_biases(self.linears, self.outs)
-        return self.outs
+        exl3.mgemm(x, self.B, carrier, self.suh, a_had, self.svh, a.K, a.mcg, a.mul1, self.opts)
+        _add_biases(self.linears, outs)
+        return outs
 
     def run_norm(self, x, res, norm_w, eps, y):
         """The bundle applied to RMSNorm(x + res) * norm_w, y = fp16(x + res): one launch (up to 16 rows)."""
-        _run_norm(self, self.carrier, x, res, norm_w, eps, y, self.opts)
-        _add_biases(self.linears, self.outs)
-        return self.outs
+        carrier, outs = self._rows(x)
+        _run_norm(self, carrier, x, res, norm_w, eps, y, self.opts)
+        _add_biases(self.linears, outs)
+        return outs
 
     def run_normed(self, y, ssq, norm_w, eps):
         """The bundle applied to the norm of a residual stream whose block sums of squares the producing
         linear left in ssq (LinearEXL3.forward_add_res)."""
         a = self.linears[0]
-        exl3.mgemm_normed(y, ssq, norm_w, eps, self.B, self.carrier, self.suh, self.svh, a.K, a.mcg, a.mul1, self.opts)
-        _add_biases(self.linears, self.outs)
-        return self.outs
+        carrier, outs = self._rows(y)
+        exl3.mgemm_normed(y, ssq, norm_w, eps, self.B, carrier, self.suh, self.svh, a.K, a.mcg, a.mul1, self.opts)
+        _add_biases(self.linears, outs)
+        return outs
 
 
 class PagedCache:
@@ -432,7 +459,8 @@ class PagedCache:
 
 class PagedAttention:
     """The attention block of a decoder layer over a PagedCache: q|k|v bundle, rotary positions with the write into the cache,
-    attention, o. One object serves prompts, drafted and single tokens, eagerly or inside a DecodeGraph."""
+    attention, o. One object serves prompts, drafted and single tokens, eagerly or inside a DecodeGraph, up to the rows that the
+    bundle's buffers hold in a call (a longer prompt goes in chunks)."""
 
     def __init__(self, qkv, o, cache, layer, dim, inv_freq, mscale=1.0, interleaved=False, window=0, sinks=0, scale=None):
         widths = [w.out_features for w in qkv.linears]
