@@ -23,6 +23,7 @@ from . import _lib
 from .exl3 import _launch
 
 _DTYPES = (torch.float16, torch.bfloat16)
+WIDTHS = (64, 128, 256)                # values per head that paged_attention takes
 _MAX_POS = 1 << 30                     # positions of one sequence
 
 _ROPE = struct.Struct("=10q15q12if4x")             # amp_rope_args
@@ -276,7 +277,7 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
     pages, page_size, kv_heads, width = shape
     if width != dim or pages < 1 or page_size < 1 or kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("%s: incompatible shapes (q %s, cache %s)" % (name, tuple(q.shape), shape))
-    if dim not in (64, 128, 256):
+    if dim not in WIDTHS:
         raise ValueError("%s: head width %d (64, 128 or 256)" % (name, dim))
     vs = _cache(name, "v_cache", v_cache, dtype, dev, shape)
     max_pages, tr = _table(name, table, seqs, page_size, dev)

@@ -467,6 +467,8 @@ class PagedAttention:
         kv_heads = cache.k.shape[3]
         if len(widths) != 3 or cache.k.shape[4] != dim or widths[1] != kv_heads * dim or widths[2] != kv_heads * dim or widths[0] % (kv_heads * dim):
             raise ValueError("PagedAttention: q|k|v of %s columns do not fit a cache of %d heads of %d" % (widths, kv_heads, dim))
+        if dim not in attention.WIDTHS:
+            raise ValueError("PagedAttention: heads of %d values (the attention takes %s)" % (dim, ", ".join(map(str, attention.WIDTHS))))
         if o.in_features != widths[0]:
             raise ValueError("PagedAttention: o takes %d columns, q gives %d" % (o.in_features, widths[0]))
         if not 0 <= layer < cache.k.shape[0]:
