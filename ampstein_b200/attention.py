@@ -87,6 +87,37 @@ def _apart(name, what, t):
         extent = st * (n - 1) + extent
 
 
+def _span(t):
+    """First byte, and [(size, stride in bytes)] of a tensor's dimensions that go somewhere"""
+    z = t.element_size()
+    return t.data_ptr(), [(n, st * z) for n, st in zip(t.shape, t.stride()) if n > 1 and st], z
+
+
+def _extent(dims, period, z):
+    return z + sum((n - 1) * st for n, st in dims if not period or st % period)
+
+
+def _share(t, u):
+    """Whether two tensors may share memory: their extents meet, and do so round each of their strides as well (columns of one buffer,
+    or keys and values side by side in a page, do not share any)"""
+    if t.numel() == 0 or u.numel() == 0:
+        return False
+    (a, da, za), (b, db, zb) = _span(t), _span(u)
+    if a + _extent(da, 0, za) <= b or b + _extent(db, 0, zb) <= a:
+        return False
+    for _, p in da + db:
+        ea, eb, d = _extent(da, p, za), _extent(db, p, zb), (b - a) % p
+        if d >= ea and d + eb <= p:
+            return False
+    return True
+
+
+def _not_shared(name, what, t, others):
+    for which, u in others:
+        if u is not None and _share(t, u):
+            raise ValueError("%s: %s overlaps %s" % (name, what, which))
+
+
 def _sequences(name, rows, pos, cu, dev):
     _cuda(name, "pos", pos, dev)
     if pos.dtype not in (torch.int32, torch.int64) or pos.dim() != 1 or not pos.is_contiguous():
@@ -186,7 +217,7 @@ def _rope(name, q, kv, pos, inv_freq, cu, interleaved, mscale, out):
     else:
         os = _rows(name, "out", out, dtype, dev, (rows, heads, dim))
         _apart(name, "out", out)
-        if out.data_ptr() == q.data_ptr() and os != qs:
+        if (out.data_ptr() != q.data_ptr() or os != qs) and _share(out, q):
             raise ValueError("%s: out overlaps q (it may be q itself)" % name)
     if kv is None:
         k = v = kc = vc = table = None
@@ -207,6 +238,10 @@ def _rope(name, q, kv, pos, inv_freq, cu, interleaved, mscale, out):
         vcs = _cache(name, "v_cache", vc, dtype, dev, tuple(kc.shape))
         _apart(name, "k_cache", kc)
         _apart(name, "v_cache", vc)
+        for what, t in (("out", out), ("k_cache", kc), ("v_cache", vc)):
+            _not_shared(name, what, t, (("k", k), ("v", v)))
+        _not_shared(name, "k_cache", kc, (("v_cache", vc), ("q", q), ("out", out)))
+        _not_shared(name, "v_cache", vc, (("q", q), ("out", out)))
         max_pages, tr = _table(name, table, seqs, page_size, dev)
         cs = kcs + vcs + (tr,)
     if rows == 0 or seqs == 0:
@@ -224,14 +259,15 @@ def rope(q, pos, inv_freq, cu=None, interleaved=False, mscale=1.0, out=None):
     """Rotary positions: the first 2 * len(inv_freq) values of every head of q (rows, heads, dim) turn in pairs (i, i + len(inv_freq)),
     or (2 i, 2 i + 1) with interleaved, by position * inv_freq[i]; cos and sin are multiplied by mscale. fp16 or bf16, any even
     number of rotated values, heads up to 1024 wide. The angle is exact for any position, the turn is made in fp32 and rounded once.
-    out: where to (it may be q itself). Returns out."""
+    out: where to (it may be q itself, but must not overlap it otherwise). Returns out."""
     return _rope("rope", q, None, pos, inv_freq, cu, interleaved, mscale, out)
 
 
 def rope_append(q, k, v, pos, inv_freq, k_cache, v_cache, table, cu=None, interleaved=False, mscale=1.0, out=None):
     """rope of q and k, and the write of k (rotated) and v (rows, kv_heads, dim) into the caches' pages, in one launch: the token at
     position p goes to row p % page_size of page table[b][p / page_size]. A token before position 0, beyond the table or on a page
-    outside the pool is not stored. Two tokens of a call must not have the same place. Returns the rotated q; the rotated k is
+    outside the pool is not stored. Two tokens of a call must not have the same place; k, v and the caches must not overlap each other,
+    nor q and out. Returns the rotated q; the rotated k is
     only in the cache."""
     return _rope("rope_append", q, (k, v, k_cache, v_cache, table), pos, inv_freq, cu, interleaved, mscale, out)
 
@@ -249,8 +285,8 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
     """Attention of q (rows, heads, dim), fp16 or bf16, dim 64 / 128 / 256, over caches that hold the rows' own keys and values
     already (rope_append). The token at position p sees the keys at positions j <= p, with window > 0 only the last `window` of
     them (its own among them) and the first `sinks`. heads is a multiple of kv_heads; query head h reads key-value head
-    h // (heads / kv_heads). scale: 1 / sqrt(dim) by default. Returns out (rows, heads, dim), q's type, which must not overlap q; lse (rows, heads) float32, if
-    given, takes ln sum_j exp(scale * q . k_j).
+    h // (heads / kv_heads). scale: 1 / sqrt(dim) by default. Returns out (rows, heads, dim), q's type; lse (rows, heads) float32, if
+    given, takes ln sum_j exp(scale * q . k_j). Neither must overlap the other, q or a cache.
 
     An infinite or NaN key or value reaches the tokens that see it, no others. A token that sees nothing gets 0 (lse -inf). Pages that no token of the call can see are not read, and their table entries may hold
     anything; a token with a visible key on a page outside the pool, or beyond the table, gets NaN. Single tokens, a few drafted ones and
@@ -292,12 +328,12 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
     else:
         os = _rows(name, "out", out, dtype, dev, (rows, heads, dim))
         _apart(name, "out", out)
-        if out.data_ptr() == q.data_ptr():
-            raise ValueError("%s: out must not be q" % name)
+        _not_shared(name, "out", out, (("q", q), ("k_cache", k_cache), ("v_cache", v_cache)))
     if lse is not None:
         _cuda(name, "lse", lse, dev)
         if lse.dtype != torch.float32 or tuple(lse.shape) != (rows, heads) or not lse.is_contiguous():
             raise ValueError("%s: lse must be contiguous float32 (rows, heads)" % name)
+        _not_shared(name, "lse", lse, (("out", out), ("q", q), ("k_cache", k_cache), ("v_cache", v_cache)))
     if rows == 0 or seqs == 0:
         return out
     window, sinks = min(int(window), _MAX_POS), min(int(sinks), _MAX_POS)

@@ -987,6 +987,15 @@ AMP_API int amp_b200_attention(const amp_attention_args* args, cudaStream_t stre
                  ((P.q_token | P.q_head | P.out_token | P.out_head | P.k_page | P.k_row | P.k_head | P.v_page | P.v_row | P.v_head) & 7)) == 0,
                 "attention: pointers must be 16-byte aligned and strides multiples of 8 values");
     AMP_REQUIRE(std::isfinite(P.scale * 1.4426950408889634f), "attention: scale is not finite");
+    {
+        // (other CTAs may still read what one writes)
+        const Span q(P.q, P.dim * 2l, { { P.tokens, P.q_token * 2 }, { P.heads, P.q_head * 2 } }), out(P.out, P.dim * 2l, { { P.tokens, P.out_token * 2 }, { P.heads, P.out_head * 2 } });
+        const Span k(P.k_cache, P.dim * 2l, { { P.pages, P.k_page * 2 }, { P.page_size, P.k_row * 2 }, { P.kv_heads, P.k_head * 2 } });
+        const Span v(P.v_cache, P.dim * 2l, { { P.pages, P.v_page * 2 }, { P.page_size, P.v_row * 2 }, { P.kv_heads, P.v_head * 2 } });
+        AMP_REQUIRE(apart(out, q) && apart(out, k) && apart(out, v), "attention: out overlaps q or a cache");
+        const Span lse(P.lse, P.lse ? (long) P.tokens * P.heads * 4 : 0, {});
+        AMP_REQUIRE(!P.lse || (apart(lse, out) && apart(lse, q) && apart(lse, k) && apart(lse, v)), "attention: lse overlaps out, q or a cache");
+    }
     P.window = min(P.window, AT_MAX_POS);
     P.sinks = min(P.sinks, AT_MAX_POS);
     int rc = 0;

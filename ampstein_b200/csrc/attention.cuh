@@ -12,6 +12,7 @@
 #include "exl3_gemv_kernel.cuh"
 #include "exl3_gemv_host.h"
 #include "host_common.h"
+#include "spans.h"
 #include "../../include/ampstein_b200.h"
 
 namespace amp {

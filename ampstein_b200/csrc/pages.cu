@@ -4,6 +4,7 @@
 // (6.6 TB/s in and out, the measured copy rate), one page of 32 KB in 32 layers 2.2 us.
 #include "exl3_common.cuh"
 #include "host_common.h"
+#include "spans.h"
 #include "../../include/ampstein_b200.h"
 #include <cstdlib>
 
@@ -80,6 +81,11 @@ AMP_API int amp_b200_copy_pages(void* const* caches, const long* layer_strides, 
                     "copy_pages: cache %d: its pages overlap", i);
     }
     if (n_caches == 0 || layers == 0 || page_bytes == 0) return 0;
+    // (one cache twice: the same bytes to the same places)
+    auto span = [&](int i) { return Span(caches[i], page_bytes, { { layers, layer_strides[i] }, { pages, page_strides[i] } }); };
+    for (int i = 1; i < n_caches; ++i)
+        for (int j = 0; j < i; ++j)
+            AMP_REQUIRE(apart(span(i), span(j)) || span(i).same(span(j)), "copy_pages: caches %d and %d overlap", j, i);
     const long chunks = (page_bytes + CP_CHUNK - 1) / CP_CHUNK;
     CpParams P;
     for (int c0 = 0; c0 < n_caches; c0 += CP_CACHES)

@@ -260,6 +260,8 @@ AMP_API int amp_b200_rope(const amp_rope_args* args, cudaStream_t stream)
     AMP_REQUIRE(P.cu || P.tokens % P.seqs == 0, "rope: %d tokens do not divide into %d sequences", P.tokens, P.seqs);
     AMP_REQUIRE(P.dim > 0 && P.dim <= ROPE_MAX_DIM && P.rot >= 0 && P.rot <= P.dim && P.rot % 2 == 0 && P.heads > 0 && P.heads <= 1024,
                 "rope: heads of %d values (up to %d), an even number of them rotated, not %d", P.dim, ROPE_MAX_DIM, P.rot);
+    const Span q(P.q, P.dim * 2l, { { P.tokens, P.q_token * 2 }, { P.heads, P.q_head * 2 } }), out(P.q_out, P.dim * 2l, { { P.tokens, P.out_token * 2 }, { P.heads, P.out_head * 2 } });
+    AMP_REQUIRE(q.same(out) || apart(q, out), "rope: q_out overlaps q (it may be q itself)");
     uintptr_t ptrs = (uintptr_t) P.q | (uintptr_t) P.q_out;
     long strides = P.q_token | P.q_head | P.out_token | P.out_head;
     if (P.k || P.v || P.k_cache || P.v_cache || P.table)
@@ -267,6 +269,12 @@ AMP_API int amp_b200_rope(const amp_rope_args* args, cudaStream_t stream)
         AMP_REQUIRE(P.k && P.v && P.k_cache && P.v_cache && (P.table || P.max_pages == 0), "rope: k, v, both caches and the table go together");
         AMP_REQUIRE(P.kv_heads > 0 && P.kv_heads <= 1024 && P.pages > 0 && P.page_size > 0 && P.max_pages >= 0 && (long long) P.max_pages * P.page_size <= AT_MAX_POS,
                     "rope: page sizes (up to 2^30 positions per sequence)");
+        const Span k(P.k, P.dim * 2l, { { P.tokens, P.k_token * 2 }, { P.kv_heads, P.k_head * 2 } }), v(P.v, P.dim * 2l, { { P.tokens, P.v_token * 2 }, { P.kv_heads, P.v_head * 2 } });
+        const Span kc(P.k_cache, P.dim * 2l, { { P.pages, P.kc_page * 2 }, { P.page_size, P.kc_row * 2 }, { P.kv_heads, P.kc_head * 2 } });
+        const Span vc(P.v_cache, P.dim * 2l, { { P.pages, P.vc_page * 2 }, { P.page_size, P.vc_row * 2 }, { P.kv_heads, P.vc_head * 2 } });
+        for (const Span* w : { &out, &kc, &vc })
+            AMP_REQUIRE(apart(*w, k) && apart(*w, v), "rope: k or v overlaps %s", w == &out ? "q_out" : "a cache");
+        AMP_REQUIRE(apart(kc, vc) && apart(kc, q) && apart(vc, q) && apart(kc, out) && apart(vc, out), "rope: a cache overlaps the other one, q or q_out");
         ptrs |= (uintptr_t) P.k | (uintptr_t) P.v | (uintptr_t) P.k_cache | (uintptr_t) P.v_cache;
         strides |= P.k_token | P.k_head | P.v_token | P.v_head | P.kc_page | P.kc_row | P.kc_head | P.vc_page | P.vc_row | P.vc_head;
     }

@@ -244,7 +244,8 @@ int amp_b200_argmax_advance(const void* logits, int n, void* ids, void* pos, voi
  * rot / 2: (i, i + rot / 2), or (2 i, 2 i + 1) with `interleaved`; cos and sin are multiplied by mscale, the other values pass.
  * The angle is reduced in fp64, the turn is made in fp32, rounded once. k (rotated) and v go to row p % page_size of page
  * table[b][p / page_size]; tokens before position 0, beyond the table or on a page outside the pool are not stored.
- * q_out may be q. k, v, k_cache, v_cache, table may all be null: q is rotated alone. Strides count values (2 bytes).
+ * q_out may be q; otherwise what is written must not overlap what is read, nor the caches each other (AMP_E_ARG).
+ * k, v, k_cache, v_cache, table may all be null: q is rotated alone. Strides count values (2 bytes).
  */
 typedef struct amp_rope_args
 {
@@ -274,7 +275,7 @@ int amp_b200_rope(const amp_rope_args* args, cudaStream_t stream);
  * 0: a slot without a sequence) gets 0 and an lse of -inf. A token whose visible keys lie on a page outside the pool, or
  * that stands beyond the table, gets NaN. Scores, softmax and sums are in fp32, the weights are rounded to the values' type for the
  * product with them. A call gives the same bits every time. dim: 64, 128 or 256.
- * An infinite or NaN key or value reaches the tokens that see it, no others.
+ * An infinite or NaN key or value reaches the tokens that see it, no others. out and lse must not overlap each other, q or a cache.
  * workspace: amp_b200_attention_workspace bytes on the device, 16-byte aligned, contents of no matter (ragged: with cu; max_keys =
  * max_pages * page_size; 0 bytes: none is needed); calls that may overlap need one each.
  */
@@ -304,7 +305,8 @@ int amp_b200_attention_status(int* out);
  * Copies whole pages inside caches: page dst[i] := page src[i] in every layer of every cache, for forks, defragmentation and
  * moves. caches / layer_strides / page_strides: host arrays of one entry per cache (bytes; all multiples of 16), a page is
  * page_bytes (a multiple of 16) without gaps. src, dst: host arrays; they travel with the launch. Refused: a page outside
- * [0, pages), a destination named twice, a page that is both source and destination of different copies.
+ * [0, pages), a destination named twice, a page that is both source and destination of different copies, caches that overlap
+ * (the same one twice may be given).
  */
 int amp_b200_copy_pages(void* const* caches, const long* layer_strides, const long* page_strides, int n_caches, int layers,
                         int pages, long page_bytes, const int* src, const int* dst, int n, cudaStream_t stream);
