@@ -349,9 +349,12 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
 
 
 def attention_status(device=None):
-    """0, or 1: a bounded wait in a call of paged_attention with prompt chunks ran out since the last look, and what depended on it was not
-    stored. Waits for the device."""
+    """0; or 1, a bounded wait in a call of paged_attention with prompt chunks ran out since the last look, or 2, such a call got shared
+    memory without the alignment that it needs: what depended on it was not stored. Waits for all streams of the device; refused while
+    the current stream is being captured."""
     import ctypes
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("attention_status: waits for the device, which a capture does not allow")
     v = ctypes.c_int(0)
     with torch.cuda.device(device):
         _lib.call("amp_b200_attention_status", ctypes.byref(v))

@@ -25,6 +25,7 @@
 // Every mbarrier wait is bounded: a role whose wait ran out hands nothing over any more, whatever depends on it runs out too, nothing
 // is stored (slices: their rows become NaN), the status word is set, and the CTA leaves when its copies and MMAs are done.
 #include "attention_tc.cuh"
+#include <mutex>
 
 namespace amp {
 
@@ -846,14 +847,22 @@ int attention_tc(TaPlan& S, cudaStream_t stream)
     return S.P.bf16 ? ta_launch_dim<__nv_bfloat16>(S, stream) : ta_launch_dim<__half>(S, stream);
 }
 
+// (read and cleared in one step: what another host thread's call sets meanwhile is kept for the next look)
+__device__ int g_at_taken;
+__global__ void attention_status_kernel() { g_at_taken = atomicExch(&g_at_status, 0); }
+
 }  // namespace amp
 
 AMP_API int amp_b200_attention_status(int* out)
 {
     using namespace amp;
-    int v = 0, zero = 0;
-    if (cudaError_t e = cudaMemcpyFromSymbol(&v, g_at_status, sizeof(int))) return cuda_rc(e, "status read");
-    if (v) if (cudaError_t e = cudaMemcpyToSymbol(g_at_status, &zero, sizeof(int))) return cuda_rc(e, "status clear");
+    static std::mutex one;                     // (one look at a time uses g_at_taken)
+    std::lock_guard<std::mutex> lock(one);
+    int v = 0;
+    if (cudaError_t e = cudaDeviceSynchronize()) return cuda_rc(e, "status wait");       // (streams that do not wait for the default one, too)
+    attention_status_kernel<<<1, 1>>>();
+    if (cudaError_t e = cudaGetLastError()) return cuda_rc(e, "status read");
+    if (cudaError_t e = cudaMemcpyFromSymbol(&v, g_at_taken, sizeof(int))) return cuda_rc(e, "status read");
     if (out) *out = v;
     return 0;
 }

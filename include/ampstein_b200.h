@@ -298,7 +298,8 @@ typedef struct amp_attention_args
 } amp_attention_args;
 long amp_b200_attention_workspace(int tokens, int seqs, int heads, int kv_heads, int dim, int ragged, long max_keys, int window, int sinks);
 int amp_b200_attention(const amp_attention_args* args, cudaStream_t stream);
-/* 0, or 1: a bounded wait inside the prompt form ran out, and what depended on it was not stored, since the last call (which clears it) */
+/* 0; or 1, a bounded wait inside the prompt form ran out, or 2, its shared memory was not aligned: what depended on it was not stored. Since
+ * the last call, which clears it. Waits for all streams of the current device: not during a capture. */
 int amp_b200_attention_status(int* out);
 
 /*
