@@ -50,7 +50,6 @@ struct AtPlan
     int cluster;                               // > 0: every (sequence, head, row tile) belongs to a cluster of so many CTAs, which join in shared memory
     int by_segment;                            // join: blockIdx.x is a segment, else the CTA whose range begins inside it
     int pdl;
-    int late;                                  // split form: the launches in front are the prompt form's, of other rows: waited for at the end
     float scale2;                              // scale * log2(e)
     AtPages g;
 };
@@ -274,8 +273,7 @@ void attention_split_kernel(const AtPlan S)
 
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, grp = warp / WR, wr = warp % WR, cta = blockIdx.x;
     const int group = S.group;
-    // (late: what is in front of the prompt form is over, or that form had not let this one begin)
-    if (S.pdl) { if (!S.late) pdl_wait(); pdl_launch_dependents(); }
+    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
 
     // the CTA's range of units
     AtCursor in;
@@ -297,7 +295,7 @@ void attention_split_kernel(const AtPlan S)
     {
         AtCount C;
         C.count<NT>(S, s_scan);
-        if (cta >= C.ctas) { if (S.late) pdl_wait(); return; }
+        if (cta >= C.ctas) return;
         const int u0 = C.begin(cta);
         left = C.begin(cta + 1) - u0;
         int b, front;
@@ -305,7 +303,7 @@ void attention_split_kernel(const AtPlan S)
         in.place(S, b, u0 - front);
         if (in.u == in.units)                                // (the CTA in front ends that segment)
         {
-            if (--left == 0) { if (S.late) pdl_wait(); return; }
+            if (--left == 0) return;
             in.advance(S);
         }
     }
@@ -679,11 +677,11 @@ void attention_split_kernel(const AtPlan S)
         }
         at_cluster_sync();
     }
-    if (S.late) pdl_wait();
 }
 
 // Joins the parts of a segment, row blockIdx.y of it (LOOP: every gridDim.y-th from there): of segment blockIdx.x, or of the one that the range of
-// CTA blockIdx.x is the second to hold. Which parts those are is found while the split kernel's last CTAs still run.
+// CTA blockIdx.x is the second to hold. (Which parts those are is found behind the wait: found in front of it the launch took 1.4 us less, but what it
+// reads for that, positions and lengths, is only visible behind it.)
 template <typename T, int D, bool LOOP>
 __global__ __launch_bounds__(128)
 void attention_join_kernel(const AtPlan S)
@@ -693,6 +691,7 @@ void attention_join_kernel(const AtPlan S)
     __shared__ float4 s_o[4][D / 4];
     __shared__ int s_scan[4], s_found[2];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, group = S.group;
+    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
     AtCount C;
     C.count<128>(S, s_scan);
     AtCursor in;
@@ -722,8 +721,6 @@ void attention_join_kernel(const AtPlan S)
         last = C.cta_of(g0 + in.units - 1);
         join = first < last && (S.by_segment || first == (int) blockIdx.x - 1);
     }
-    if (S.pdl) pdl_wait();
-    if (S.pdl) pdl_launch_dependents();
     if (!join) return;
 
     // part i of the segment: the first is the end of its CTA's range, the others are the beginning of theirs
@@ -1018,15 +1015,16 @@ AMP_API int amp_b200_attention(const amp_attention_args* args, cudaStream_t stre
     {
         // (rows and CTAs are divided in 30 bits)
         AMP_REQUIRE((double) P.tokens * (P.heads / P.kv_heads) + 512 < 1073741824.0 && (double) C.tiles * C.slices * P.kv_heads < 1073741824.0, "attention: too many tokens in one call");
-        // (first: the split form of the other sequences begins on the SMs that its last CTAs leave. us in a graph, before / since: 2333 tokens
-        // of six prompts 40.2 / 35.5, 64 single tokens of 1000 keys beside a prompt of 2048 tokens 130 / 120)
+        // (each form waits for the one in front: positions and lengths may come from the launch before the call, and only a grid's own wait makes
+        // them visible to it. us in a graph with the few-token form begun under the prompt form's end / so: 64 single tokens of 1000 keys beside
+        // a prompt of 2048 tokens 115 / 125, 16 of 4000 beside 64 tokens on 6000 98 / 104; in the other order level)
         TaPlan A;
         A.P = P; A.nq = C.nq; A.tiles = C.tiles; A.slices = C.slices; A.split_rows = P.cu ? AT_SPLIT_ROWS : 0; A.pdl = g_pdl;
         A.scale2 = P.scale * 1.4426950408889634f; A.part_offset = C.tc_offset; A.g = g;
         if ((rc = attention_tc(A, stream))) return rc;
     }
     if (!C.split) return 0;
-    S.grid = C.grid; S.cluster = C.cluster; S.pdl = g_pdl; S.late = g_pdl && C.tc && C.tiles; S.split_rows = P.cu ? AT_SPLIT_ROWS : 1 << 30;
+    S.grid = C.grid; S.cluster = C.cluster; S.pdl = g_pdl; S.split_rows = P.cu ? AT_SPLIT_ROWS : 1 << 30;
     S.scale2 = P.scale * 1.4426950408889634f; S.g = g;
     return P.bf16 ? at_launch_dim<__nv_bfloat16>(S, C.wr, stream) : at_launch_dim<__half>(S, C.wr, stream);
 }

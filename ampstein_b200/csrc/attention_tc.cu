@@ -762,13 +762,13 @@ void attention_tc_join_kernel(const TaPlan S)
     constexpr int ROWS = ta_rows<NQ>;
     __shared__ TaPlace s_place;
     const int t = threadIdx.x, x = S.by_kv.of(blockIdx.x), h = blockIdx.x - x * P.kv_heads, group = S.group;
+    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
     if (t < 32)
     {
         const TaPlace f = ta_find<NQ>(S, x);
         if (t == 0) s_place = f;
     }
     __syncthreads();
-    if (S.pdl) { pdl_wait(); pdl_launch_dependents(); }
     if (!s_place.have) return;
     const AtSeq seq = s_place.s;
     const int row = s_place.tile * ROWS + t, tok = S.by_group.of(row);
