@@ -35,6 +35,7 @@ constexpr unsigned AT_SPIN_LIMIT = 1u << 21;   // looks at a barrier before a wa
 constexpr int TA_LOADERS = 3;                  // warps that load keys and values
 constexpr int TA_AHEAD = 2;                    // tiles on their way when the next is requested
 template <int D> constexpr int ta_poly = D == 64 ? 1 : 0;     // pairs of four whose exponentials are a polynomial's
+constexpr float TA_FAR = 1048576.0f;           // a maximum beyond this (in powers of two) is off by more than 1/16 when it is rounded
 constexpr float TA_SLACK = 8.0f;               // powers of two that a row's maximum may grow before O is scaled again
 
 __device__ __forceinline__ bool ta_wait(uint32_t bar, uint32_t parity)
@@ -427,8 +428,22 @@ void attention_tc_kernel(const TaPlan S)
                     }
                 }
             }
-            const float base = m == -INFINITY ? 0.0f : -m * sc;
-            const f32x2 sc2 = pack_f32x2(sc, sc), base2 = pack_f32x2(base, base);
+            // 2^(s sc - m sc) in one step; where m sc is so large that its own rounding counts, the difference is taken first
+            float by = sc, base = m == -INFINITY ? 0.0f : -m * sc;
+            if (__any_sync(0xffffffffu, fabsf(base) > TA_FAR))
+            {
+                const float at = m == -INFINITY ? 0.0f : -m;
+                #pragma unroll
+                for (int c = 0; c < KB; c += 2)
+                {
+                    const float2 d = unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), pack_f32x2(at, at)), pack_f32x2(sc, sc)));
+                    s[c] = __float_as_uint(d.x);
+                    s[c + 1] = __float_as_uint(d.y);
+                }
+                by = 1.0f;
+                base = 0.0f;
+            }
+            const f32x2 sc2 = pack_f32x2(by, by), base2 = pack_f32x2(base, base);
             #pragma unroll
             for (int half = 0; half < 2; ++half)
             {
