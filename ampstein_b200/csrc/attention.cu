@@ -265,6 +265,7 @@ void attention_split_kernel(const AtPlan S)
     const amp_attention_args& P = S.P;
     constexpr int NT = AT_THREADS, WK = at_wk<WR>, KW = at_kw<D>, H = at_halves<D, WR>, HALF = at_half_bytes<D>;
     constexpr int CH = D / 8, NK = KW / 8, ROWS = at_rows<WR>, UNIT = at_unit<D, WR>;
+    constexpr float TOP = AtType<T>::weight_top;
     constexpr bool KEEP_Q = D <= 128;          // q's fragments stay in registers (256: they are read for every step)
     static_assert(H >= 3, "ring");
     extern __shared__ __align__(128) unsigned char smem[];
@@ -501,17 +502,20 @@ void attention_split_kernel(const AtPlan S)
                         for (int n = 0; n < D / 8; ++n) { o[n][2 * i] *= f; o[n][2 * i + 1] *= f; }
                     }
                 }
-                const float base0 = m[0] == -INFINITY ? 0.0f : m[0], base1 = m[1] == -INFINITY ? 0.0f : m[1];
+                const float base0 = (m[0] == -INFINITY ? 0.0f : m[0]) - TOP, base1 = (m[1] == -INFINITY ? 0.0f : m[1]) - TOP;
+                float sum[2] = { 0.0f, 0.0f };               // (by itself: small weights beside a large l are lost one by one)
                 #pragma unroll
                 for (int n = 0; n < NK; ++n)
                 {
                     s[n][0] = at_exp2(s[n][0] - base0); s[n][1] = at_exp2(s[n][1] - base0);
                     s[n][2] = at_exp2(s[n][2] - base1); s[n][3] = at_exp2(s[n][3] - base1);
-                    l[0] += s[n][0] + s[n][1];
-                    l[1] += s[n][2] + s[n][3];
+                    sum[0] += s[n][0] + s[n][1];
+                    sum[1] += s[n][2] + s[n][3];
                     pf[n / 2][2 * (n & 1)] = AtType<T>::pack(s[n][0], s[n][1]);
                     pf[n / 2][2 * (n & 1) + 1] = AtType<T>::pack(s[n][2], s[n][3]);
                 }
+                l[0] += sum[0];
+                l[1] += sum[1];
             }
         }
         else
@@ -573,6 +577,7 @@ void attention_split_kernel(const AtPlan S)
                 {
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+                    m[i] -= TOP;                             // (what the sums count from)
                     if ((lane & 3) == 0) { s_ml[grp][wr * 16 + (lane >> 2) + 8 * i][0] = m[i]; s_ml[grp][wr * 16 + (lane >> 2) + 8 * i][1] = l[i]; }
                 }
                 __syncthreads();

@@ -7,8 +7,8 @@
 //   P = 2^(scale S - m), a row per thread: no exchange between threads; P goes back over S, in the operands' type
 //   O += P V      P from tensor memory, V as it lies in the cache (N-major), O (128 x D fp32) in tensor memory
 // With two tiles the tensor cores multiply for one while the other's softmax runs; with one tile S has two buffers, and the next
-// Q K^T runs under the softmax. m moves only when a row's maximum has grown by more than 2^8 (the sums stay far from fp32's and the
-// weights from fp16's range), so that O is rarely scaled again. Where the grid leaves SMs idle the keys of a tile are cut into
+// Q K^T runs under the softmax. m moves only when a row's maximum has grown by more than 2^8 (with fp16 the weights begin 2^7 above 1, and stay
+// below 2^15 and a rounding), so that O is rarely scaled again. Where the grid leaves SMs idle the keys of a tile are cut into
 // slices, whose parts a second kernel joins in order.
 //
 // Warps: four per row tile do the softmax (a thread a row, the warp's quarter of tensor memory), then one issues the MMAs, three load
@@ -254,6 +254,7 @@ void attention_tc_kernel(const TaPlan S)
     constexpr int KB = ta_kb<NQ>, ST = ta_stages<D, NQ>, ROWS = ta_rows<NQ>;
     constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = KB * D * 2, CH = D / 8;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+    constexpr float TOP = BF ? 0.0f : AtType<T>::weight_top - TA_SLACK;      // (a maximum that has not moved yet lies up to the slack below)
     // tensor memory: S (two tiles or two buffers), then O
     constexpr int S_STEP = KB, O_COL = 2 * KB, TMEM = O_COL + NQ * (NQ == 2 ? 128 : D) <= 256 ? 256 : 512;
     static_assert(O_COL + (NQ == 2 ? 128 + D : D) <= TMEM && TMEM * ta_ctas<D, NQ> <= 512, "tensor memory");
@@ -429,7 +430,7 @@ void attention_tc_kernel(const TaPlan S)
                 }
             }
             // 2^(s sc - m sc) in one step; where m sc is so large that its own rounding counts, the difference is taken first
-            float by = sc, base = m == -INFINITY ? 0.0f : -m * sc;
+            float by = sc, base = m == -INFINITY ? 0.0f : TOP - m * sc;
             if (__any_sync(0xffffffffu, fabsf(base) > TA_FAR))
             {
                 const float at = m == -INFINITY ? 0.0f : -m;
@@ -441,9 +442,10 @@ void attention_tc_kernel(const TaPlan S)
                     s[c + 1] = __float_as_uint(d.y);
                 }
                 by = 1.0f;
-                base = 0.0f;
+                base = TOP;
             }
             const f32x2 sc2 = pack_f32x2(by, by), base2 = pack_f32x2(base, base);
+            f32x2 sum2 = pack_f32x2(0.0f, 0.0f);             // (by itself: small weights beside a large l are lost one by one)
             #pragma unroll
             for (int half = 0; half < 2; ++half)
             {
@@ -457,7 +459,7 @@ void attention_tc_kernel(const TaPlan S)
                     float2 x;
                     if ((e / 2) % 4 < ta_poly<D>) x = ta_exp2_pair(y);
                     else { x = unpack_f32x2(y); x.x = at_exp2(x.x); x.y = at_exp2(x.y); }
-                    l2 = add_f32x2(l2, pack_f32x2(x.x, x.y));
+                    sum2 = add_f32x2(sum2, pack_f32x2(x.x, x.y));
                     w[e / 2] = AtType<T>::pack(x.x, x.y);
                 }
                 if constexpr (KB == 128) ta_st32(s_t + half * 32, w);
@@ -466,6 +468,7 @@ void attention_tc_kernel(const TaPlan S)
                 ta_fence_before();
                 ta_arrive(pf + 8 * (2 * buf + half));
             }
+            l2 = add_f32x2(l2, sum2);
         }
         const float2 ls = unpack_f32x2(l2);
         l = ls.x + ls.y;
@@ -520,7 +523,7 @@ void attention_tc_kernel(const TaPlan S)
             for (int e = 0; e < 32; ++e)
                 o[e] = __float_as_uint(__uint_as_float(o[e]) + (up[i] >> e & 1 ? INFINITY : 0.0f) + (down[i] >> e & 1 ? -INFINITY : 0.0f));
         };
-        const float m2 = m == -INFINITY ? m : m * sc;
+        const float m2 = m == -INFINITY ? m : m * sc - TOP;  // (what the sums count from)
         if (S.slices > 1)
         {
             // a part: rows side by side, so that a warp writes whole lines; lost: NaN
