@@ -258,7 +258,8 @@ def _rope(name, q, kv, pos, inv_freq, cu, interleaved, mscale, out):
 def rope(q, pos, inv_freq, cu=None, interleaved=False, mscale=1.0, out=None):
     """Rotary positions: the first 2 * len(inv_freq) values of every head of q (rows, heads, dim) turn in pairs (i, i + len(inv_freq)),
     or (2 i, 2 i + 1) with interleaved, by position * inv_freq[i]; cos and sin are multiplied by mscale. fp16 or bf16, any even
-    number of rotated values, heads up to 1024 wide. The angle is exact for any position, the turn is made in fp32 and rounded once.
+    number of rotated values, heads up to 1024 wide. The angle is taken modulo a turn in fp64 (off by less than 2^-21 at positions up to
+    2^30), then rounded to fp32 (pi 2^-24); the turn is made in fp32 and rounded once.
     out: where to (it may be q itself, but must not overlap it otherwise). Returns out."""
     return _rope("rope", q, None, pos, inv_freq, cu, interleaved, mscale, out)
 
@@ -288,7 +289,7 @@ def paged_attention(q, k_cache, v_cache, table, pos, cu=None, window=0, sinks=0,
     h // (heads / kv_heads). scale: 1 / sqrt(dim) by default. Returns out (rows, heads, dim), q's type; lse (rows, heads) float32, if
     given, takes ln sum_j exp(scale * q . k_j). Neither must overlap the other, q or a cache.
 
-    An infinite or NaN key or value reaches the tokens that see it, no others. A token that sees nothing gets 0 (lse -inf). Pages that no token of the call can see are not read, and their table entries may hold
+    An infinite or NaN key or value reaches the tokens that see it, no others. A token that sees nothing, or whose scores are all -inf, gets 0 (lse -inf). Pages that no token of the call can see are not read, and their table entries may hold
     anything; a token with a visible key on a page outside the pool, or beyond the table, gets NaN. Single tokens, a few drafted ones and
     prompt chunks may be mixed in one call with cu."""
     name = "paged_attention"

@@ -13,10 +13,10 @@
 // stages (KW keys, then their values), filled by its own lanes with 16-byte asynchronous copies, and meets nobody else until the segment
 // ends: every warp keeps m, l and o of its rows over its keys. The rings run ahead over the ends of segments.
 //
-// What bounds it: memory, and a fixed 7 us (launch, positions, table, first keys: 4; the second kernel 3), of which sequences
-// that see few keys are spared the second (AT_CLUSTER_KEYS). 32 query heads on 8 key-value heads of 128 values, fp16, us on the device: one sequence of 128 keys 4.3,
-// 512 5.6, 4000 9.9, 131072 86 (6.2 TB/s, 0.96 of the measured copy rate), 32 sequences of
-// 2000 keys 51 (5.1 TB/s), of 100 to 8192 keys 53 (before the end of a segment was counted as a unit, 71: a range of
+// What bounds it: memory, and a fixed 8 us (launch, positions, table, first keys: 4; the second kernel 4), of which sequences
+// that see few keys are spared the second (AT_CLUSTER_KEYS). 32 query heads on 8 key-value heads of 128 values, fp16, us a call in a
+// captured chain: one sequence of 128 keys 4.2, 512 5.6, 4000 10.1, 131072 88.6 (6.1 TB/s, 0.94 of the measured copy rate), 32 sequences of
+// 2000 keys 51.7 (5.1 TB/s), of 100 to 8192 keys 54.3 (counting the end of a segment as a unit took 71 to 53: a range of
 // many short sequences took as long again as its keys). mma.sync and not tcgen05: at 16 rows and 128 values a warp needs 400 issue cycles
 // for the 16 KB that a scheduler's share of the memory brings in 2850. 32 keys per step where the registers allow it: the
 // look-ups, the row maxima and the loop are per step (32 x 2048 keys, 16 / 32 keys: 60.0 / 53.3). Wide heads keep q in shared
@@ -685,8 +685,8 @@ void attention_split_kernel(const AtPlan S)
 }
 
 // Joins the parts of a segment, row blockIdx.y of it (LOOP: every gridDim.y-th from there): of segment blockIdx.x, or of the one that the range of
-// CTA blockIdx.x is the second to hold. (Which parts those are is found behind the wait: found in front of it the launch took 1.4 us less, but what it
-// reads for that, positions and lengths, is only visible behind it.)
+// CTA blockIdx.x is the second to hold. (Which parts those are is found behind the wait: in front of it a call took 1.0 to 1.4 us less, but what is
+// read for that, positions and lengths, is only visible behind it.)
 template <typename T, int D, bool LOOP>
 __global__ __launch_bounds__(128)
 void attention_join_kernel(const AtPlan S)
@@ -822,7 +822,7 @@ static const AtDevice* at_device(int* rc)
 // second kernel follows. Up to AT_WHOLE_KEYS however many segments there are, beyond where at least two CTAs find places for each (the
 // lengths may differ). us, equal ranges / this, when both still divided (each is about 1 us faster since; 32 query heads on 8 key-value heads of 128 values): one sequence of 512 and 1024 keys 8.1 / 6.6
 // and 8.4 / 7.0, of 2048 8.9 / 9.0; four of 300 and 2000 11.5 / 9.4 and 14.6 / 12.8; 32 of 300 19.1 / 13.0; but 32 of 50 to 2000 keys,
-// a CTA each, 29.6 / 39.4
+// a CTA each, 29.6 / 39.4. (Equal ranges take 1.2 more again since their second kernel waits before it looks anything up.)
 constexpr int AT_WHOLE_KEYS = 512, AT_CLUSTER_KEYS = 2048;
 // Rows (tokens x group) up to which a sequence takes the split form, whose ranges follow the lengths; beyond, the prompt form
 constexpr int AT_SPLIT_ROWS = 64;

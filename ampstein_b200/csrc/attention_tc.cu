@@ -2,7 +2,7 @@
 //
 // The query heads that share a key-value head, times a sequence's new tokens, are the rows of one problem (row = token * group + head),
 // so that a tile of 128 rows spans few tokens, keys are fetched once for the whole group, and a short chunk fills its tiles. A CTA takes
-// NQ tiles of 128 rows (two up to 128 values per head, one at 256) and walks the keys that its tokens see in tiles of KB:
+// NQ tiles of 128 rows (one at 256 values per head, and where a tile sees few keys; else two) and walks the keys that its tokens see in tiles of KB:
 //   S = Q K^T     both operands K-major in shared memory, S (128 x KB fp32) in tensor memory
 //   P = 2^(scale S - m), a row per thread: no exchange between threads; P goes back over S, in the operands' type
 //   O += P V      P from tensor memory, V as it lies in the cache (N-major), O (128 x D fp32) in tensor memory
@@ -14,8 +14,8 @@
 // Warps: four per row tile do the softmax (a thread a row, the warp's quarter of tensor memory), then one issues the MMAs, three load
 // keys and values by 16-byte asynchronous copies (a page of any size, strides of any kind).
 //
-// What bounds it (8192 tokens, 32 query heads on 8 key-value heads of 128 values, fp16): 497 us, 1106 TFLOP/s, 0.67 of the measured burst
-// rate; tensor and exponential pipe active in 54 % of the cycles each. A row tile's chain, scores read 0.15 us, maximum 0.2, weights
+// What bounds it (8192 tokens, 32 query heads on 8 key-value heads of 128 values, fp16): 495 us in bursts of four, 1110 TFLOP/s, 0.67 of the
+// measured burst rate (577 among other calls, under the power cap: 950, 0.68 of the measured sustained rate); tensor and exponential pipe active in 54 % of the cycles each. A row tile's chain, scores read 0.15 us, maximum 0.2, weights
 // 0.75, its P V and the next Q K^T 0.5, is longer than the other tile's MMAs, and the rows of a page reach shared memory through three
 // warps at about 0.8 us per tile of keys or values. Measured and taken back: seven loading warps (registers of the softmax), TMA gathers of
 // four rows (67 cycles each: 1121 us) and TMA boxes of a page's rows (level), two threads per row (544), a maximum that lags a
@@ -136,7 +136,7 @@ __device__ __forceinline__ void ta_fence_async() { asm volatile("fence.proxy.asy
 
 // 2^y of two values without the exponential unit, which has 16 results a clock for the SM and would be busy as long as the tensor
 // cores: y = i + f with i the nearest whole number, 2^f on [-1/2, 1/2] by a polynomial of degree 5 (minimax in the relative error, by
-// Remez exchange: 7.5e-8), 2^i through the exponent field. Below 2^-126.5: 0 (the field is 0); a NaN stays one. y <= 127.
+// Remez exchange: 7.5e-8, 1.5e-7 with its coefficients in fp32, 2.1e-7 as it is evaluated here), 2^i through the exponent field. Below 2^-126.5: 0 (the field is 0); a NaN stays one. y <= 127.
 __device__ __forceinline__ float2 ta_exp2_pair(f32x2 y2)
 {
     float2 y = unpack_f32x2(y2);

@@ -272,9 +272,9 @@ int amp_b200_rope(const amp_rope_args* args, cudaStream_t stream);
  * j > p - window or j < sinks; query head h reads key-value head h / (heads / kv_heads):
  *   out = sum_j softmax_j(scale * q . k_j) v_j,   lse = ln sum_j e^(scale * q . k_j)
  * Table entries of pages that no token of the call sees are not read. A token that sees nothing (it stands before position
- * 0: a slot without a sequence) gets 0 and an lse of -inf. A token whose visible keys lie on a page outside the pool, or
+ * 0: a slot without a sequence), or whose scores are all -inf, gets 0 and an lse of -inf. A token whose visible keys lie on a page outside the pool, or
  * that stands beyond the table, gets NaN. Scores, softmax and sums are in fp32, the weights are rounded to the values' type for the
- * product with them. A call gives the same bits every time. dim: 64, 128 or 256.
+ * product with them (fp16: the largest weight is 2^15, in the prompt form 2^7 to 2^15, so that what is lost lies below 2^-32 of it). A call gives the same bits every time. dim: 64, 128 or 256.
  * An infinite or NaN key or value reaches the tokens that see it, no others. out and lse must not overlap each other, q or a cache.
  * workspace: amp_b200_attention_workspace bytes on the device, 16-byte aligned, contents of no matter (ragged: with cu; max_keys =
  * max_pages * page_size; 0 bytes: none is needed); calls that may overlap need one each.
