@@ -372,7 +372,9 @@ class PagedCache:
             self._uses[page] = 1
             pages.append(page)
             changed = True
-        seq[1:3] = at + tokens, at
+        seq[1] = at + tokens
+        if tokens:
+            seq[2] = at
         if changed:
             self._write_row(slot)
         return at

@@ -97,3 +97,12 @@ def test_no_truncation_to_where_given_up_pages_are_seen(cache):
     cache.leave_behind(b, 20, pending=0)                                # a longer window looks back to more of them
     cache.truncate(b, 29)
     assert cache.length(a) == 5 and cache.length(b) == 29
+
+
+def test_an_extension_by_nothing_leaves_the_pending_tokens(cache):
+    slot = cache.add()
+    cache.extend(slot, 21)
+    at = cache.extend(slot, 9)
+    assert cache.extend(slot, 0) == 30
+    cache.leave_behind(slot, 6)
+    check(cache, slot, at, 9, 6, 0)
