@@ -61,6 +61,32 @@ static int cp_check(const int* src, const int* dst, int n, int pages)
     return rc;
 }
 
+// Caches must not share memory (one cache twice may be given: the same bytes to the same places). Their extents in order of address: one of a model's
+// dozens of caches meets none or the one beside it.
+struct CpExtent { uintptr_t from, to; int cache; };
+
+static int cp_overlap(void* const* caches, const long* layer_strides, const long* page_strides, int n, int layers, int pages, long page_bytes)
+{
+    if (n < 2) return 0;
+    auto span = [&](int i) { return Span(caches[i], page_bytes, { { layers, layer_strides[i] }, { pages, page_strides[i] } }); };
+    CpExtent* const e = (CpExtent*) malloc((size_t) n * sizeof(CpExtent));
+    if (!e) return fail(AMP_E_ARG, "copy_pages: out of host memory");
+    for (int i = 0; i < n; ++i) { const Span s = span(i); e[i] = { s.at, s.at + s.extent(0), i }; }
+    qsort(e, n, sizeof(CpExtent), [](const void* a, const void* b) {
+        const uintptr_t x = ((const CpExtent*) a)->from, y = ((const CpExtent*) b)->from;
+        return x < y ? -1 : x > y ? 1 : 0;
+    });
+    int rc = 0;
+    for (int i = 0; i < n && !rc; ++i)
+        for (int j = i + 1; j < n && e[j].from < e[i].to && !rc; ++j)
+        {
+            const Span a = span(e[i].cache), b = span(e[j].cache);
+            if (!apart(a, b) && !a.same(b)) rc = fail(AMP_E_ARG, "copy_pages: caches %d and %d overlap", e[i].cache, e[j].cache);
+        }
+    free(e);
+    return rc;
+}
+
 }  // namespace amp
 
 using namespace amp;
@@ -81,11 +107,7 @@ AMP_API int amp_b200_copy_pages(void* const* caches, const long* layer_strides, 
                     "copy_pages: cache %d: its pages overlap", i);
     }
     if (n_caches == 0 || layers == 0 || page_bytes == 0) return 0;
-    // (one cache twice: the same bytes to the same places)
-    auto span = [&](int i) { return Span(caches[i], page_bytes, { { layers, layer_strides[i] }, { pages, page_strides[i] } }); };
-    for (int i = 1; i < n_caches; ++i)
-        for (int j = 0; j < i; ++j)
-            AMP_REQUIRE(apart(span(i), span(j)) || span(i).same(span(j)), "copy_pages: caches %d and %d overlap", j, i);
+    if (int rc = cp_overlap(caches, layer_strides, page_strides, n_caches, layers, pages, page_bytes)) return rc;
     const long chunks = (page_bytes + CP_CHUNK - 1) / CP_CHUNK;
     CpParams P;
     for (int c0 = 0; c0 < n_caches; c0 += CP_CACHES)
