@@ -265,7 +265,6 @@ void attention_split_kernel(const AtPlan S)
     const amp_attention_args& P = S.P;
     constexpr int NT = AT_THREADS, WK = at_wk<WR>, KW = at_kw<D>, H = at_halves<D, WR>, HALF = at_half_bytes<D>;
     constexpr int CH = D / 8, NK = KW / 8, ROWS = at_rows<WR>, UNIT = at_unit<D, WR>;
-    constexpr float TOP = AtType<T>::weight_top;
     constexpr bool KEEP_Q = D <= 128;          // q's fragments stay in registers (256: they are read for every step)
     static_assert(H >= 3, "ring");
     extern __shared__ __align__(128) unsigned char smem[];
@@ -495,14 +494,14 @@ void attention_split_kernel(const AtPlan S)
                     #pragma unroll
                     for (int i = 0; i < 2; ++i)
                     {
-                        const float f = top[i] > m[i] ? at_exp2(m[i] - top[i]) : 1.0f;
+                        const float f = top[i] > m[i] ? (m[i] == -INFINITY ? 0.0f : at_exp2(at_base<T>(m[i]) - at_base<T>(top[i]))) : 1.0f;
                         m[i] = top[i];
                         l[i] *= f;
                         #pragma unroll
                         for (int n = 0; n < D / 8; ++n) { o[n][2 * i] *= f; o[n][2 * i + 1] *= f; }
                     }
                 }
-                const float base0 = (m[0] == -INFINITY ? 0.0f : m[0]) - TOP, base1 = (m[1] == -INFINITY ? 0.0f : m[1]) - TOP;
+                const float base0 = m[0] == -INFINITY ? 0.0f : at_base<T>(m[0]), base1 = m[1] == -INFINITY ? 0.0f : at_base<T>(m[1]);
                 float sum[2] = { 0.0f, 0.0f };               // (by itself: small weights beside a large l are lost one by one)
                 #pragma unroll
                 for (int n = 0; n < NK; ++n)
@@ -577,7 +576,7 @@ void attention_split_kernel(const AtPlan S)
                 {
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-                    m[i] -= TOP;                             // (what the sums count from)
+                    m[i] = at_base<T>(m[i]);                 // (what the sums count from)
                     if ((lane & 3) == 0) { s_ml[grp][wr * 16 + (lane >> 2) + 8 * i][0] = m[i]; s_ml[grp][wr * 16 + (lane >> 2) + 8 * i][1] = l[i]; }
                 }
                 __syncthreads();

@@ -148,6 +148,14 @@ template <> struct AtType<__nv_bfloat16>
     static __device__ __forceinline__ __nv_bfloat16 from(float a) { return __float2bfloat16_rn(a); }
 };
 
+// What the weights of a row with the maximum m count from. (Far from 0 the maximum itself: there m - 15 is rounded, to m - 16 between 2^24 and
+// 2^28, and 2^16 is infinite in half.)
+template <typename T>
+__device__ __forceinline__ float at_base(float m)
+{
+    return AtType<T>::weight_top == 0.0f || fabsf(m) > 1048576.0f ? m : m - AtType<T>::weight_top;
+}
+
 // An infinite or NaN value times the weight 0 of a row that does not see its key would be NaN. Where keys are seen by some rows only,
 // such values are therefore taken out of the product, and added to the rows that do see them.
 constexpr uint32_t AT_ODD = 0x80008000u;

@@ -13,7 +13,8 @@ H, B = torch.float16, torch.bfloat16
 @pytest.mark.parametrize("wide", [0, 200])
 @pytest.mark.parametrize("count", [1, 6, 150])
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("dtype,power,sign", [(H, 13, 1), (H, 13, -1), (H, 8, 1), (B, 13, 1), (B, 24, 1), (B, 24, -1), (B, 50, 1)])
+@pytest.mark.parametrize("dtype,power,sign", [(H, 13, 1), (H, 13, -1), (H, 8, 1), (B, 13, 1), (B, 24, 1), (B, 24, -1), (B, 50, 1)]
+                         + [(H, p, s) for p in (9, 10, 11, 12) for s in (1, -1)])
 def test_far_scores(dtype, power, sign, d, count, wide):
     """q = 2^power everywhere, key j sign * 2^power (1 + c_j / 64) everywhere: the scores, 2^(2 power) d / 8 (1 + c_j / 64), are exact in fp32 and
     64-bit numbers and lie so far apart that all weights but those of the largest are 0 (2^(2 power - 9) d / 8 > 100 from power 8 on)"""
