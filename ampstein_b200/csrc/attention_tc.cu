@@ -289,7 +289,7 @@ void attention_tc_kernel(const TaPlan S)
         for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
         for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 128);
         mbar_init(&pv_done, 1);
-        mbar_init(&o_full, 1);
+        mbar_init(&o_full, 2);                 // the MMAs, and the warp that issues them (for s_odd)
         mbar_init(&end, 1);
         fence_mbar_init();
     }
@@ -649,7 +649,8 @@ void attention_tc_kernel(const TaPlan S)
                 }
                 if (!ok) break;
             }
-            if (ok) commit(smem_u32(&o_full));
+            // (the end of the MMAs does not say that what the warp itself wrote is visible: its own arrival does)
+            if (ok) { commit(smem_u32(&o_full)); if (lane == 0) ta_arrive(smem_u32(&o_full)); }
         }
         commit(smem_u32(&end));
         ta_wait(smem_u32(&end), 0);            // (bounded; the accumulators are given back only then)
